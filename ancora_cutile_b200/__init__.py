@@ -9,6 +9,7 @@ from .muon import (BatchedProjMuon, DeviceMuon, ExpertMuonScratch, Muon, MuonPla
                    ResidentMuon)
 from .muon_ns import (PE_SCHEDULE, newton_schulz_resident, newton_schulz_resident_e,
                       set_polar_express)
+from .grad_clip import GradClip
 from .hybrid import HybridOptimizer, default_is_muon
 from .resident import ResidentHybrid
 
@@ -17,4 +18,4 @@ __all__ = ["AncoraError", "LIB_PATH", "Context", "DBuf", "Event", "PinnedArray",
            "ExpertMuonScratch", "Muon",
            "MuonPlan", "MuonScratch", "ResidentMuon", "PE_SCHEDULE", "newton_schulz_resident",
            "newton_schulz_resident_e", "set_polar_express", "HybridOptimizer", "default_is_muon",
-           "ResidentHybrid"]
+           "ResidentHybrid", "GradClip"]

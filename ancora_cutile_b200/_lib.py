@@ -13,6 +13,8 @@ LIB_PATH = os.path.join(_HERE, "libancora_b200.so")
 OK, E_INVALID, E_CUDA, E_NOMEM, E_DEVICE, E_NCCL, E_UNSUPPORTED = 0, -1, -2, -3, -4, -5, -6
 GRAD_BF16, GRAD_F32 = 0, 1
 ROUND_RNE, ROUND_SR = 0, 1
+IDS_I32, IDS_I64 = 0, 1
+EMBED_WRITE, EMBED_ADD = 0, 1
 
 
 class AncoraError(RuntimeError):
@@ -32,6 +34,10 @@ class AdamWScalars(C.Structure):
                 ("beta1", "one_minus_beta1", "beta2", "one_minus_beta2", "eps", "lr", "ibc1", "ibc2")]
 
 
+class ClipTensor(C.Structure):
+    _fields_ = [("g", C.c_void_p), ("out", C.c_void_p), ("numel", C.c_uint64)]
+
+
 class MuonOutputs(C.Structure):
     _fields_ = [("fp8", C.c_void_p), ("fp8_scale", C.c_void_p), ("p16_t", C.c_void_p),
                 ("fp8_t", C.c_void_p), ("fp8_scale_t", C.c_void_p)]
@@ -42,6 +48,7 @@ class MuonWeight(C.Structure):
                 ("K", C.c_int32), ("N", C.c_int32), ("owner", C.c_int32), ("_pad", C.c_int32)]
 
 
+_i64 = C.c_int64
 _vp, _i, _u64, _f, _d, _sz = C.c_void_p, C.c_int, C.c_uint64, C.c_float, C.c_double, C.c_size_t
 _pp = C.POINTER(C.c_void_p)
 
@@ -106,12 +113,25 @@ SIGNATURES = {
     "anc_fro_normalize": (_i, [_vp, _vp, _vp, _i, _i, _i, _f, _vp]),
     "anc_fro_normalize_static": (_i, [_i, _vp, _vp, _i, _i, _i, _f, _vp]),
     "anc_grad_accumulate": (_i, [_vp, _vp, _vp, _i, _vp, _u64, _u64, _f, _i, _u64, _u64, _i, _vp]),
+    "anc_clip_plan_create": (_i, [_vp, C.POINTER(ClipTensor), _i, _i, _i, _vp, _pp]),
+    "anc_clip_plan_result": (_i, [_vp, _pp, _pp]),
+    "anc_grad_norm": (_i, [_vp, _f, _f, _f, _vp]),
+    "anc_grad_clip": (_i, [_vp, _f, _f, _f, _vp]),
+    "anc_grad_sumsq": (_i, [_vp, _vp]),
+    "anc_grad_norm_finish": (_i, [_vp, _f, _f, _f, _vp]),
+    "anc_grad_apply": (_i, [_vp, _vp]),
+    "anc_clip_plan_destroy": (_i, [_vp]),
+    "anc_embedding_lookup": (_i, [_vp, _vp, _i, _i64, _vp, _i, _vp, _i, _i64, _i64, _i64, _i64, _f, _vp]),
+    "anc_embedding_grad_workspace": (_i, [_i64, _i64, _i64, C.POINTER(_u64)]),
+    "anc_embedding_grad": (_i, [_vp, _vp, _i, _i64, _vp, _i, _vp, _i, _i64, _i64, _i64, _i64, _f, _i, _i64, _vp,
+                                _u64, _vp]),
     "anc_nccl_load": (_i, [C.c_char_p]),
     "anc_nccl_unique_id": (_i, [_vp]),
     "anc_comm_create": (_i, [_vp, _vp, _i, _i, _pp]),
     "anc_comm_destroy": (_i, [_vp]),
     "anc_comm_allgather_bf16": (_i, [_vp, _vp, _u64, _vp]),
     "anc_comm_reduce_scatter_grads": (_i, [_vp, _vp, _u64, _i, _vp]),
+    "anc_comm_allreduce_f64": (_i, [_vp, _vp, _u64, _vp]),
     "anc_comm_barrier": (_i, [_vp, _vp]),
 }
 

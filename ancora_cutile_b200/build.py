@@ -19,7 +19,8 @@ PKG = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(PKG, "csrc")
 OBJ = os.path.join(PKG, "build")
 LIB = os.path.join(PKG, "libancora_b200.so")
-SOURCES = ["runtime.cu", "adamw.cu", "muon_elem.cu", "ns_gemm.cu", "muon_plan.cu", "grad_prod.cu", "zero1.cu"]
+SOURCES = ["runtime.cu", "adamw.cu", "muon_elem.cu", "ns_gemm.cu", "muon_plan.cu", "grad_prod.cu", "grad_clip.cu",
+           "embedding.cu", "zero1.cu"]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
               "-Xcompiler", "-fPIC,-fvisibility=hidden", "--ftz=false", "--prec-div=true",
               "--prec-sqrt=true", "--fmad=true"]
@@ -57,8 +58,8 @@ def build(force=False, verbose=False, profile=False):
 
 def _build(nvcc, force, verbose, extra):
     os.makedirs(OBJ, exist_ok=True)
-    headers = [os.path.join(CSRC, "anc_internal.h"),
-               os.path.join(PKG, "..", "include", "ancora_b200.h")]
+    headers = [os.path.join(CSRC, f) for f in sorted(os.listdir(CSRC)) if f.endswith((".h", ".cuh"))]
+    headers.append(os.path.join(PKG, "..", "include", "ancora_b200.h"))
     jobs = []
     objs = []
     for src in SOURCES:

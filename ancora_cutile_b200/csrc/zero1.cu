@@ -156,6 +156,15 @@ int anc_comm_reduce_scatter_grads(anc_comm *c, void *arena, uint64_t elems_per_r
   return ANC_OK;
 }
 
+int anc_comm_allreduce_f64(anc_comm *c, double *values, uint64_t count, void *stream) {
+  ANC_REQUIRE(c && values, "NULL argument");
+  if (count == 0) return ANC_OK;
+  anc_device_guard guard(c->ctx->device);
+  ANC_NCCL(g_nccl.AllReduce(values, values, (size_t)count, ncclFloat64, ncclSum, c->comm,
+                            anc_pick_stream(c->ctx, stream)));
+  return ANC_OK;
+}
+
 int anc_comm_barrier(anc_comm *c, void *stream) {
   ANC_REQUIRE(c, "comm is NULL");
   anc_device_guard guard(c->ctx->device);

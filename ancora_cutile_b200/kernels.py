@@ -67,3 +67,42 @@ def grad_accumulate(acc, src=None, g16=None, numel=None, src_dtype="f32", elem_o
                                         int(numel), int(elem_offset), float(np.float32(scale)),
                                         {"rne": L.ROUND_RNE, "sr": L.ROUND_SR}[rounding], int(seed), int(step),
                                         int(bool(zero_after)), C.c_void_p(stream or None)))
+
+
+_IDS = {"i32": L.IDS_I32, "i64": L.IDS_I64}
+_EMBED = {"write": L.EMBED_WRITE, "add": L.EMBED_ADD}
+
+
+def embedding_lookup(table, ids, out, T, V, D, scale=1.0, table_dtype="bf16", out_dtype="bf16", ids_dtype="i64",
+                     table_ld=0, out_ld=0, stream=None, ctx=None):
+    """out[t] = round(scale * table[ids[t]]) for T tokens over a (V, D) table; rows ``*_ld`` elements apart
+    (0: D).  A negative id gives a zero row; an id >= V too, and sets status bit 0x8."""
+    ctx = ctx or get_context()
+    L.check(L.lib().anc_embedding_lookup(ctx.handle, dev_ptr(table), _GRAD[table_dtype], table_ld, dev_ptr(ids),
+                                         _IDS[ids_dtype], dev_ptr(out), _GRAD[out_dtype], out_ld, T, V, D,
+                                         scale, stream or None))
+
+
+def embedding_grad_workspace(T, V, D):
+    """Bytes of scratch ``embedding_grad`` needs for T tokens over a (V, D) table."""
+    n = C.c_uint64()
+    L.check(L.lib().anc_embedding_grad_workspace(int(T), int(V), int(D), C.byref(n)))
+    return n.value
+
+
+def embedding_grad(dy, ids, dw, T, V, D, work, scale=1.0, dy_dtype="bf16", dw_dtype="bf16", ids_dtype="i64",
+                   mode="write", padding_idx=None, dy_ld=0, dw_ld=0, work_bytes=None, stream=None, ctx=None):
+    """The embedding's gradient: dw[v] = round(scale * S_v) over the whole (V, D) table (mode "write") or
+    dw[v] = round(dw[v] + scale * S_v) on the rows some token names (mode "add"), with S_v the float32 sum of
+    dy[t] over the tokens with ids[t] == v, in an order the ids alone fix.  Negative ids and ``padding_idx``
+    contribute nothing.  ``work``: a device buffer of ``embedding_grad_workspace(T, V, D)`` bytes that no
+    other call in flight uses; ``work_bytes`` defaults to its ``nbytes`` and, for a bare address, to the need."""
+    ctx = ctx or get_context()
+    if work_bytes is None:
+        work_bytes = getattr(work, "nbytes", None)
+        if work_bytes is None:
+            work_bytes = embedding_grad_workspace(T, V, D)
+    L.check(L.lib().anc_embedding_grad(ctx.handle, dev_ptr(dy), _GRAD[dy_dtype], dy_ld, dev_ptr(ids),
+                                       _IDS[ids_dtype], dev_ptr(dw), _GRAD[dw_dtype], dw_ld, T, V, D, scale,
+                                       _EMBED[mode], -1 if padding_idx is None else padding_idx, dev_ptr(work),
+                                       work_bytes, stream or None))

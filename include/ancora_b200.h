@@ -344,6 +344,67 @@ ANC_API int anc_grad_accumulate(anc_ctx *ctx, float *acc, const void *src, int s
                                 uint64_t numel, uint64_t elem_offset, float scale, int round_mode,
                                 uint64_t seed, uint64_t step, int zero_after, void *stream);
 
+/* ---------------------------------------------- gradient norm and clipping ---- */
+/* No counterpart in the reference (its optimizer classes step on the gradients as they are).
+ *
+ *   norm   = scale * sqrt(sum of the squares of all elements of all tensors)
+ *   factor = scale * min(1, max_norm / (norm + eps))
+ *   out    = round(g * factor)                                        (anc_grad_clip, anc_grad_apply)
+ *
+ * A plan holds the table of gradient tensors (one type for all, any alignment, sizes from 0) and the block
+ * sums of the reduction.  `out` NULL clips in place; otherwise it must not partly overlap the tensor.
+ * {norm, factor} are two floats in device memory: `result` when given, else inside the plan.  Squares are summed
+ * in float32 by eights and in float64 above, in a fixed order: the same bits every time on one device.  A
+ * NaN in a gradient makes norm and factor NaN, an infinity makes norm infinite and factor 0;
+ * max_norm = +inf never clips.  Calls on one plan must be ordered among themselves (they share its block
+ * sums and its result); calls on different plans need not be.  All calls can be captured into a graph. */
+typedef struct anc_clip_plan anc_clip_plan;
+typedef struct anc_clip_tensor {
+  const void *g;   /* gradient, of the plan's grad_dtype                      */
+  void *out;       /* clipped gradient, of the plan's out_dtype; NULL: in place */
+  uint64_t numel;
+} anc_clip_tensor;
+ANC_API int anc_clip_plan_create(anc_ctx *ctx, const anc_clip_tensor *tensors, int n_tensors, int grad_dtype,
+                                 int out_dtype, float *result, anc_clip_plan **out);
+/* Device addresses of {norm, factor} and of the float64 sum of squares (both may be NULL). */
+ANC_API int anc_clip_plan_result(anc_clip_plan *plan, float **result, double **sumsq);
+/* norm and factor only: one launch. */
+ANC_API int anc_grad_norm(anc_clip_plan *plan, float scale, float max_norm, float eps, void *stream);
+/* anc_grad_norm and anc_grad_apply. */
+ANC_API int anc_grad_clip(anc_clip_plan *plan, float scale, float max_norm, float eps, void *stream);
+/* The two halves of anc_grad_norm, for gradients sharded over ranks: the sum of squares alone, then, after
+ * the caller has added up the ranks' sums in place (anc_comm_allreduce_f64), norm and factor from it. */
+ANC_API int anc_grad_sumsq(anc_clip_plan *plan, void *stream);
+ANC_API int anc_grad_norm_finish(anc_clip_plan *plan, float scale, float max_norm, float eps, void *stream);
+/* out = round(g * factor) with the factor the last norm call left. */
+ANC_API int anc_grad_apply(anc_clip_plan *plan, void *stream);
+/* Waits for the device before it frees the table. */
+ANC_API int anc_clip_plan_destroy(anc_clip_plan *plan);
+
+/* --------------------------------------------- embedding lookup and gradient ---- */
+/* The forward that reads a bf16 parameter the step wrote, and the gradient producer of that parameter.
+ *   table, dw (V,D), dy, out (T,D): bf16 bits or f32, rows `ld` elements apart (0: D), elements of a row
+ *   contiguous, any alignment; ids (T): int32 or int64.  A negative id is padding: a zero row, no
+ *   gradient; its row of dy is not read.  An id >= V sets status bit 0x8 and counts as padding.
+ * Sums and products are float32, rounded once to the output type. */
+#define ANC_IDS_I32 0
+#define ANC_IDS_I64 1
+/* out[t,:] = round(scale * table[ids[t],:]) */
+ANC_API int anc_embedding_lookup(anc_ctx *ctx, const void *table, int table_dtype, int64_t table_ld, const void *ids,
+                                 int ids_dtype, void *out, int out_dtype, int64_t out_ld, int64_t T, int64_t V,
+                                 int64_t D, float scale, void *stream);
+#define ANC_EMBED_WRITE 0 /* dw[v,:] = round(scale * S_v) for every row, zero where no token names v   */
+#define ANC_EMBED_ADD 1   /* dw[v,:] = round(dw[v,:] + scale * S_v) for the rows named, others untouched */
+/* S_v = sum of dy[t,:] over the tokens t with ids[t] == v and v != padding_idx (< 0: none), in an order that
+ * the ids alone fix: the same bits every time.  `work`: caller-owned scratch of at least
+ * anc_embedding_grad_workspace(T, V, D) bytes, 16-byte aligned, contents unspecified; calls that may overlap on
+ * the GPU need one each. */
+ANC_API int anc_embedding_grad_workspace(int64_t T, int64_t V, int64_t D, uint64_t *bytes);
+ANC_API int anc_embedding_grad(anc_ctx *ctx, const void *dy, int dy_dtype, int64_t dy_ld, const void *ids,
+                               int ids_dtype, void *dw, int dw_dtype, int64_t dw_ld, int64_t T, int64_t V, int64_t D,
+                               float scale, int mode, int64_t padding_idx, void *work, uint64_t work_bytes,
+                               void *stream);
+
 /* ----------------------------------------------------------------- ZeRO-1 ---- */
 /* No counterpart in the reference (single GPU, ancora README.md:93).  NCCL is
  * opened with dlopen at first use; nccl_path may be NULL (default search). */
@@ -362,6 +423,8 @@ ANC_API int anc_comm_allgather_bf16(anc_comm *comm, uint16_t *arena, uint64_t el
  * data-parallel replicas. */
 ANC_API int anc_comm_reduce_scatter_grads(anc_comm *comm, void *arena, uint64_t elems_per_rank,
                                           int grad_dtype, void *stream);
+/* In-place sum over all ranks of `count` float64 values (the ranks' sums of squares). */
+ANC_API int anc_comm_allreduce_f64(anc_comm *comm, double *values, uint64_t count, void *stream);
 ANC_API int anc_comm_barrier(anc_comm *comm, void *stream);
 
 #ifdef __cplusplus
