@@ -13,58 +13,75 @@
 // ids, and runs that cross a piece's border are joined from the pieces' partial sums in order.  The work is balanced
 // however often one token occurs.
 #include <cuda_bf16.h>
+#include <mutex>
 #include "anc_internal.h"
 #include "philox.cuh"
 
 namespace {
 
 // ------------------------------------------------------------------ rows in registers
-// A warp holds a slice of kSliceCols columns of a row, eight per lane: eight neighbouring ones where rows
-// are 16-byte aligned vectors of eight (kVec), else every 32nd.
-constexpr int kSliceCols = 256;
-
+// A lane holds eight columns of a row: eight neighbouring ones where rows are 16-byte aligned vectors of
+// eight (kVec), else every L-th of a group of L lanes.
 template <bool kVec>
-__device__ __forceinline__ int col_of(int c0, int lane, int k) {
-  return kVec ? c0 + lane * 8 + k : c0 + k * 32 + lane;
+__device__ __forceinline__ int first_col(int c0, int l) {
+  return kVec ? c0 + l * 8 : c0 + l;
+}
+
+// the eight elements as they lie in memory
+template <bool kF32, bool kVec>
+struct Row8 {
+  uint32_t w[(kF32 || !kVec) ? 8 : 4];
+};
+
+// Predicated loads that leave the registers alone where `on` is false.  They are written as one instruction
+// because the value of an `if` is merged by a register move that waits for the load: a loop
+// that fetched ahead that way had a single load in flight per warp.
+__device__ __forceinline__ void ld_v4(uint32_t &a, uint32_t &b, uint32_t &c, uint32_t &d, const void *p, bool on) {
+  asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.u32 q, %5, 0;\n\t@q ld.global.v4.u32 {%0, %1, %2, %3}, [%4];\n\t}"
+               : "+r"(a), "+r"(b), "+r"(c), "+r"(d)
+               : "l"(p), "r"((uint32_t)on)
+               : "memory");
+}
+__device__ __forceinline__ void ld_1(uint32_t &a, const void *p, bool on) {
+  asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.u32 q, %2, 0;\n\t@q ld.global.u32 %0, [%1];\n\t}"
+               : "+r"(a)
+               : "l"(p), "r"((uint32_t)on)
+               : "memory");
+}
+__device__ __forceinline__ void ld_h(uint32_t &a, const void *p, bool on) {
+  asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.u32 q, %2, 0;\n\t@q ld.global.u16 %0, [%1];\n\t}"
+               : "+r"(a)
+               : "l"(p), "r"((uint32_t)on)
+               : "memory");
 }
 
 template <bool kF32, bool kVec>
-__device__ __forceinline__ void load8(const void *row, int c0, int lane, int D, float x[8]) {
+__device__ __forceinline__ void load_row(Row8<kF32, kVec> &r, const void *row, int c, int L, int D, bool on) {
   if constexpr (kVec) {
-    const int c = c0 + lane * 8;
-    if (c >= D) {
-#pragma unroll
-      for (int k = 0; k < 8; ++k) x[k] = 0.f;
-    } else if constexpr (kF32) {
-      const float4 a = *reinterpret_cast<const float4 *>((const float *)row + c);
-      const float4 b = *reinterpret_cast<const float4 *>((const float *)row + c + 4);
-      x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
-    } else {
-      const uint4 r = *reinterpret_cast<const uint4 *>((const uint16_t *)row + c);
-      const uint32_t w[4] = {r.x, r.y, r.z, r.w};
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        x[2 * k] = __uint_as_float(w[k] << 16);
-        x[2 * k + 1] = __uint_as_float(w[k] & 0xFFFF0000u);
-      }
-    }
+    const uint8_t *q = (const uint8_t *)row + (int64_t)c * (kF32 ? 4 : 2);
+    on = on && c < D;
+    ld_v4(r.w[0], r.w[1], r.w[2], r.w[3], q, on);
+    if constexpr (kF32) ld_v4(r.w[4], r.w[5], r.w[6], r.w[7], q + 16, on);
   } else {
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-      const int c = c0 + k * 32 + lane;
-      x[k] = 0.f;
-      if (c < D) {
-        if constexpr (kF32) x[k] = ((const float *)row)[c];
-        else x[k] = __uint_as_float((uint32_t)((const uint16_t *)row)[c] << 16);
-      }
+      const int ck = c + k * L;
+      if constexpr (kF32) ld_1(r.w[k], (const float *)row + ck, on && ck < D);
+      else ld_h(r.w[k], (const uint16_t *)row + ck, on && ck < D);
     }
   }
 }
 
 template <bool kF32, bool kVec>
-__device__ __forceinline__ void store8(void *row, int c0, int lane, int D, const float x[8]) {
+__device__ __forceinline__ float elem(const Row8<kF32, kVec> &r, int k) {
+  if constexpr (kF32) return __uint_as_float(r.w[k]);
+  else if constexpr (!kVec) return __uint_as_float(r.w[k] << 16);
+  else return __uint_as_float((k & 1) ? (r.w[k >> 1] & 0xFFFF0000u) : (r.w[k >> 1] << 16));
+}
+
+template <bool kF32, bool kVec>
+__device__ __forceinline__ void store_row(void *row, int c, int L, int D, const float x[8]) {
   if constexpr (kVec) {
-    const int c = c0 + lane * 8;
     if (c >= D) return;
     if constexpr (kF32) {
       float4 *d = reinterpret_cast<float4 *>((float *)row + c);
@@ -80,10 +97,10 @@ __device__ __forceinline__ void store8(void *row, int c0, int lane, int D, const
   } else {
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-      const int c = c0 + k * 32 + lane;
-      if (c < D) {
-        if constexpr (kF32) ((float *)row)[c] = x[k];
-        else ((uint16_t *)row)[c] = (uint16_t)bf16_rne(x[k]);
+      const int ck = c + k * L;
+      if (ck < D) {
+        if constexpr (kF32) ((float *)row)[ck] = x[k];
+        else ((uint16_t *)row)[ck] = (uint16_t)bf16_rne(x[k]);
       }
     }
   }
@@ -103,30 +120,66 @@ __device__ __forceinline__ void *row_ptr(void *base, int64_t row, int64_t ld) {
 }
 
 // ------------------------------------------------------------------ lookup
-constexpr int kLookupWarps = 8;
+// The output is taken as one list of vectors of eight columns (of single elements where rows are not
+// aligned); a thread has four of them in flight, kLookupThreads apart, whatever the row length.  Bound
+// by memory: four independent id -> row -> store chains per thread cover the two latencies.
+constexpr int kLookupThreads = 256;
 
-// One warp per (token, slice of kSliceCols columns).
 template <bool kTabF32, bool kOutF32, bool kVec>
-__global__ void __launch_bounds__(kLookupWarps * 32)
+__global__ void __launch_bounds__(kLookupThreads)
 embedding_lookup_kernel(const void *__restrict__ table, int64_t table_ld, const void *__restrict__ ids, int ids64,
-                        void *__restrict__ out, int64_t out_ld, int64_t T, int64_t V, int D, int slices, float scale,
+                        void *__restrict__ out, int64_t out_ld, int64_t V, int D, int64_t total, float scale,
                         uint32_t *status) {
-  const int lane = threadIdx.x & 31;
-  const int64_t units = T * slices;
-  for (int64_t u = (int64_t)blockIdx.x * kLookupWarps + (threadIdx.x >> 5); u < units;
-       u += (int64_t)gridDim.x * kLookupWarps) {
-    const int64_t t = u / slices;
-    const int c0 = (int)(u - t * slices) * kSliceCols;
-    const int64_t id = load_id(ids, ids64, t);
-    float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (id >= 0 && id < V) {
-      load8<kTabF32, kVec>(row_ptr<kTabF32>(table, id, table_ld), c0, lane, D, x);
+  constexpr int U = kVec ? 4 : 8, W = kVec ? 8 : 1;
+  const uint32_t nv = (uint32_t)(D / W);      // vectors per row
+  for (int64_t start = (int64_t)blockIdx.x * (kLookupThreads * U); start < total;
+       start += (int64_t)gridDim.x * (kLookupThreads * U)) {
+    const int64_t row0 = start / nv;
+    const uint32_t rem = (uint32_t)(start - row0 * nv);
+    int64_t t[U], id[U];
+    int c[U];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) x[k] = __fmul_rn(x[k], scale);
-    } else if (id >= V && lane == 0) {
-      atomicOr(status, ANC_DEV_BAD_INDEX);
+    for (int u = 0; u < U; ++u) {
+      const uint32_t o = rem + threadIdx.x + u * kLookupThreads, r = o / nv;
+      t[u] = row0 + r;
+      c[u] = (int)(o - r * nv) * W;
+      if (start + threadIdx.x + u * kLookupThreads >= total) t[u] = row0, c[u] = -1;      // past the end
     }
-    store8<kOutF32, kVec>(row_ptr<kOutF32>(out, t, out_ld), c0, lane, D, x);
+    if (ids64) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) id[u] = ((const int64_t *)ids)[t[u]];
+    } else {
+#pragma unroll
+      for (int u = 0; u < U; ++u) id[u] = ((const int32_t *)ids)[t[u]];
+    }
+    Row8<kTabF32, kVec> x[U];      // !kVec: only the first element
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const bool live = id[u] >= 0 && id[u] < V && c[u] >= 0;
+      const void *row = row_ptr<kTabF32>(table, live ? id[u] : 0, table_ld);
+      x[u] = Row8<kTabF32, kVec>{};
+      if constexpr (kVec) load_row<kTabF32, true>(x[u], row, c[u], 0, D, live);
+      else if constexpr (kTabF32) ld_1(x[u].w[0], (const float *)row + c[u], live);
+      else ld_h(x[u].w[0], (const uint16_t *)row + c[u], live);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (id[u] >= V && c[u] == 0) atomicOr(status, ANC_DEV_BAD_INDEX);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (c[u] < 0) break;
+      void *row = row_ptr<kOutF32>(out, t[u], out_ld);
+      if constexpr (kVec) {
+        float f[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) f[k] = __fmul_rn(elem(x[u], k), scale);
+        store_row<kOutF32, true>(row, c[u], 0, D, f);
+      } else {
+        const float f = __fmul_rn(elem(x[u], 0), scale);
+        if constexpr (kOutF32) ((float *)row)[c[u]] = f;
+        else ((uint16_t *)row)[c[u]] = (uint16_t)bf16_rne(f);
+      }
+    }
   }
 }
 
@@ -135,18 +188,17 @@ embedding_lookup_kernel(const void *__restrict__ table, int64_t table_ld, const 
 // passes for tables of up to 2^18 rows.  Per pass every warp counts the digits of its stretch of the list,
 // the cluster exchanges its CTAs' digit counts through distributed shared memory, and every warp then
 // writes its stretch in order to the places the counts give.  Padding sorts behind the last row of
-// the table as id V.
+// the table as id V.  The passes are bound by latency, not by bytes: loads go out eight rounds at a time,
+// and the lanes of equal digit find each other by nine ballots (the match instruction took 2000 cycles a
+// round with 32 warps at it, the ballots take about 200).
 constexpr int kDigitBits = 9;
 constexpr int kDigits = 1 << kDigitBits;
 constexpr int kSortThreads = 1024;
 constexpr int kSortWarps = kSortThreads / 32;
+constexpr int kSortRounds = 8;
 constexpr size_t kSortSmem = (size_t)(kSortWarps * kDigits + 2 * kDigits + 64) * 4;
+constexpr int kMaxCluster = 8;
 
-__device__ __forceinline__ uint32_t cluster_rank() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
@@ -160,98 +212,179 @@ __device__ __forceinline__ uint32_t ld_cluster(uint32_t addr) {
   asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
   return v;
 }
+__device__ __forceinline__ void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 struct SortArgs {
   const void *ids;
   int ids64;
   int64_t T, V, padding_idx;
-  uint32_t *key[2], *pos[2];
+  uint2 *list[2];                // (id, token)
   int passes;
   uint32_t *status;
 };
 
-__device__ __forceinline__ uint32_t key_of(const SortArgs &a, int64_t t, bool report) {
-  const int64_t id = load_id(a.ids, a.ids64, t);
-  if (id >= a.V && report) atomicOr(a.status, ANC_DEV_BAD_INDEX);
-  return (id < 0 || id >= a.V || id == a.padding_idx) ? (uint32_t)a.V : (uint32_t)id;
+struct ZeroArgs {
+  uint8_t *dw;
+  int64_t row_bytes, pitch, V;
+  int vec;
+};
+
+__device__ __forceinline__ uint32_t key_of(int64_t id, int64_t V, int64_t padding_idx) {
+  return (id < 0 || id >= V || id == padding_idx) ? (uint32_t)V : (uint32_t)id;
+}
+
+// Zeros for the rows no token names.  Launched behind the sort without waiting for it, so it fills the SMs the
+// sort leaves idle; it waits for the sort only before it ends, so that whoever waits for this
+// kernel has the sorted list too.  By `n` threads of which this is number `i0`
+__device__ __forceinline__ void zero_rows(const ZeroArgs &z, int64_t i0, int64_t n) {
+  if (z.vec) {
+    const int64_t per = z.row_bytes / 16, total = per * z.V;
+    if (z.pitch == z.row_bytes) {
+      for (int64_t i = i0; i < total; i += n) reinterpret_cast<uint4 *>(z.dw)[i] = make_uint4(0u, 0u, 0u, 0u);
+    } else {
+      for (int64_t i = i0; i < total; i += n)
+        *reinterpret_cast<uint4 *>(z.dw + (i / per) * z.pitch + (i % per) * 16) = make_uint4(0u, 0u, 0u, 0u);
+    }
+  } else {
+    const int64_t per = z.row_bytes / 2, total = per * z.V;
+    for (int64_t i = i0; i < total; i += n)
+      *reinterpret_cast<uint16_t *>(z.dw + (i / per) * z.pitch + (i % per) * 2) = 0;
+  }
+}
+
+__global__ void __launch_bounds__(256)
+embedding_zero_kernel(ZeroArgs z) {
+  pdl_trigger();
+  zero_rows(z, (int64_t)blockIdx.x * 256 + threadIdx.x, (int64_t)gridDim.x * 256);
+  pdl_wait();
 }
 
 __global__ void __launch_bounds__(kSortThreads, 1)
 embedding_sort_kernel(SortArgs a, uint32_t n_ctas) {
   extern __shared__ uint32_t sm[];
+  pdl_trigger();
+  const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const uint32_t rank = blockIdx.x;
   uint32_t *cnt = sm;                                // [warp][digit]
   uint32_t *tot = sm + kSortWarps * kDigits;         // this CTA's digit counts, read by the whole cluster
   uint32_t *off = tot + kDigits;                     // first place of a digit's keys of this CTA
   uint32_t *wsum = off + kDigits;
-  const uint32_t rank = cluster_rank();
-  const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  // stretches: whole rounds of 32 keys per warp
-  const int64_t per = ((a.T + (int64_t)n_ctas * kSortThreads - 1) / ((int64_t)n_ctas * kSortThreads)) * 32;
+  // stretches: at least eight rounds of 32 keys per warp, so that few keys keep few warps busy
+  int64_t per = ((a.T + (int64_t)n_ctas * kSortThreads - 1) / ((int64_t)n_ctas * kSortThreads)) * 32;
+  if (per < 32 * kSortRounds) per = 32 * kSortRounds;
   const int64_t lo = ((int64_t)rank * kSortWarps + warp) * per;
   const int64_t hi = lo + per < a.T ? lo + per : a.T;
+  const int64_t cta_keys = a.T - (int64_t)rank * kSortWarps * per;
+  const int n_warps = cta_keys <= 0 ? 0 : cta_keys >= kSortWarps * per ? kSortWarps : (int)((cta_keys + per - 1) / per);
+  uint32_t *mine = cnt + warp * kDigits;
+  // kSortRounds rounds of the list, all loads before the first use (places past the end repeat the last one);
+  // the first pass reads the ids.  Returns whether one of this lane's ids lies outside the table.
+  auto fetch = [&](uint2 (&e)[kSortRounds], const uint2 *in, bool first, int64_t i0) {
+    bool bad = false;
+    if (first) {
+      int64_t id[kSortRounds];
+#pragma unroll
+      for (int r = 0; r < kSortRounds; ++r) {
+        const int64_t i = i0 + r * 32 + lane;
+        id[r] = load_id(a.ids, a.ids64, i < a.T ? i : a.T - 1);
+      }
+#pragma unroll
+      for (int r = 0; r < kSortRounds; ++r) {
+        const int64_t i = i0 + r * 32 + lane;
+        e[r] = make_uint2(key_of(id[r], a.V, a.padding_idx), (uint32_t)i);
+        bad = bad || id[r] >= a.V;
+      }
+    } else {
+#pragma unroll
+      for (int r = 0; r < kSortRounds; ++r) {
+        const int64_t i = i0 + r * 32 + lane;
+        e[r] = __ldcg(in + (i < a.T ? i : a.T - 1));
+      }
+    }
+    return bad;
+  };
   for (int p = 0; p < a.passes; ++p) {
     const bool odd = p & 1;
-    const uint32_t *ik = odd ? a.key[0] : a.key[1], *ip = odd ? a.pos[0] : a.pos[1];
-    uint32_t *ok = odd ? a.key[1] : a.key[0], *op = odd ? a.pos[1] : a.pos[0];
+    const uint2 *in = odd ? a.list[0] : a.list[1];
+    uint2 *out = odd ? a.list[1] : a.list[0];
     const int shift = p * kDigitBits;
-    for (uint32_t d = tid; d < kSortWarps * kDigits; d += kSortThreads) cnt[d] = 0u;
-    __syncthreads();
-    for (int64_t i = lo + lane; i < hi; i += 32) {
-      const uint32_t key = p == 0 ? key_of(a, i, true) : __ldcg(ik + i);
-      atomicAdd(&cnt[warp * kDigits + ((key >> shift) & (kDigits - 1))], 1u);
+    for (uint32_t d = lane * 4; d < kDigits; d += 128) *reinterpret_cast<uint4 *>(mine + d) = make_uint4(0u, 0u, 0u, 0u);
+    __syncwarp();
+    for (int64_t i0 = lo; i0 < hi; i0 += 32 * kSortRounds) {
+      uint2 e[kSortRounds];
+      const bool bad = fetch(e, in, p == 0, i0);
+      if (bad) atomicOr(a.status, ANC_DEV_BAD_INDEX);
+#pragma unroll
+      for (int r = 0; r < kSortRounds; ++r)
+        if (i0 + r * 32 + lane < hi) atomicAdd(mine + ((e[r].x >> shift) & (kDigits - 1)), 1u);
     }
     __syncthreads();
     if (tid < kDigits) {
       uint32_t run = 0;
-      for (int w = 0; w < kSortWarps; ++w) {
-        const uint32_t c = cnt[w * kDigits + tid];
-        cnt[w * kDigits + tid] = run;
-        run += c;
+      for (int w0 = 0; w0 < n_warps; w0 += 8) {
+        uint32_t c[8];
+#pragma unroll
+        for (int w = 0; w < 8; ++w) c[w] = cnt[(w0 + w) * kDigits + tid];
+#pragma unroll
+        for (int w = 0; w < 8; ++w) {
+          cnt[(w0 + w) * kDigits + tid] = run;
+          run += c[w];
+        }
       }
       tot[tid] = run;
     }
     cluster_sync();
-    uint32_t before = 0, all = 0;
+    uint32_t before = 0, all = 0, s = 0;
     if (tid < kDigits) {
-      const uint32_t mine = (uint32_t)__cvta_generic_to_shared(tot + tid);
-      for (uint32_t c = 0; c < n_ctas; ++c) {
-        const uint32_t v = ld_cluster(peer_smem(mine, c));
-        if (c < rank) before += v;
-        all += v;
+      const uint32_t slot = (uint32_t)__cvta_generic_to_shared(tot + tid);
+      uint32_t v[kMaxCluster];
+#pragma unroll
+      for (uint32_t c = 0; c < kMaxCluster; ++c) v[c] = c < n_ctas ? ld_cluster(peer_smem(slot, c)) : 0u;
+#pragma unroll
+      for (uint32_t c = 0; c < kMaxCluster; ++c) {
+        if (c < rank) before += v[c];
+        all += v[c];
       }
       // exclusive scan of the digit totals
-      uint32_t s = all;
+      s = all;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t v = __shfl_up_sync(0xFFFFFFFFu, s, o);
-        if (lane >= (uint32_t)o) s += v;
+        const uint32_t u = __shfl_up_sync(0xFFFFFFFFu, s, o);
+        if (lane >= (uint32_t)o) s += u;
       }
       if (lane == 31) wsum[warp] = s;
-      off[tid] = s - all + before;
     }
     __syncthreads();
     if (tid < kDigits) {
       uint32_t base = 0;
-      for (uint32_t w = 0; w < warp; ++w) base += wsum[w];
-      off[tid] += base;
+#pragma unroll
+      for (uint32_t w = 0; w < kDigits / 32; ++w)
+        if (w < warp) base += wsum[w];
+      off[tid] = base + s - all + before;
     }
     __syncthreads();
-    for (int64_t i0 = lo; i0 < hi; i0 += 32) {
-      const int64_t i = i0 + lane;
-      const bool on = i < hi;
-      const uint32_t active = __ballot_sync(0xFFFFFFFFu, on);
-      if (on) {
-        const uint32_t key = p == 0 ? key_of(a, i, false) : __ldcg(ik + i);
-        const uint32_t pos = p == 0 ? (uint32_t)i : __ldcg(ip + i);
-        const uint32_t d = (key >> shift) & (kDigits - 1);
-        const uint32_t peers = __match_any_sync(active, d);
-        const uint32_t at = cnt[warp * kDigits + d];
-        __syncwarp(active);
-        if (lane == (uint32_t)(__ffs(peers) - 1)) cnt[warp * kDigits + d] = at + __popc(peers);
-        __syncwarp(active);
-        const uint32_t dst = off[d] + at + __popc(peers & ((1u << lane) - 1u));
-        ok[dst] = key;
-        op[dst] = pos;
+    for (int64_t i0 = lo; i0 < hi; i0 += 32 * kSortRounds) {
+      uint2 e[kSortRounds];
+      fetch(e, in, p == 0, i0);
+#pragma unroll
+      for (int r = 0; r < kSortRounds; ++r) {
+        if (i0 + r * 32 >= hi) break;
+        const bool on = i0 + r * 32 + lane < hi;
+        const uint32_t d = (e[r].x >> shift) & (kDigits - 1);
+        uint32_t peers = __ballot_sync(0xFFFFFFFFu, on);
+#pragma unroll
+        for (int bit = 0; bit < kDigitBits; ++bit) {
+          const bool set = (d >> bit) & 1u;
+          const uint32_t m = __ballot_sync(0xFFFFFFFFu, set);
+          peers &= set ? m : ~m;
+        }
+        uint32_t at = 0;
+        if (on) at = mine[d];
+        __syncwarp();
+        if (on && lane == (uint32_t)(__ffs(peers) - 1)) mine[d] = at + __popc(peers);
+        __syncwarp();
+        if (on) out[off[d] + at + __popc(peers & ((1u << lane) - 1u))] = e[r];
       }
     }
     __syncwarp();
@@ -259,220 +392,307 @@ embedding_sort_kernel(SortArgs a, uint32_t n_ctas) {
   }
 }
 
-__global__ void __launch_bounds__(256)
-embedding_zero_kernel(uint8_t *dw, int64_t row_bytes, int64_t pitch, int64_t V, int vec) {
-  const int64_t stride = (int64_t)gridDim.x * 256, i0 = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (vec) {
-    const int64_t n = row_bytes / 16, total = n * V;
-    for (int64_t i = i0; i < total; i += stride)
-      *reinterpret_cast<uint4 *>(dw + (pitch == row_bytes ? i * 16 : (i / n) * pitch + (i % n) * 16)) =
-          make_uint4(0u, 0u, 0u, 0u);
-  } else {
-    const int64_t n = row_bytes / 2, total = n * V;
-    for (int64_t i = i0; i < total; i += stride)
-      *reinterpret_cast<uint16_t *>(dw + (i / n) * pitch + (i % n) * 2) = 0;
-  }
-}
-
 // ------------------------------------------------------------------ sums of runs
-constexpr int kRedWarps = 8;
+constexpr int kRedThreads = 256;
+constexpr int kMaxPiece = 1024;      // sorted places per CTA
 
 struct RedArgs {
   const void *dy;
   void *dw;
   int64_t dy_ld, dw_ld, T;
-  const uint32_t *key, *pos;     // sorted
-  float *partial;                // [piece][open at its start, open at its end][slices * 256], register layout
+  const uint2 *list;             // sorted (id, token)
+  float *partial;                // [piece][open at its start, open at its end][slices * 8 * L], register layout
   uint32_t V;
   int D, slices;
-  int per_warp;                  // sorted places per warp, at most 32
+  int L;                         // lanes that share a row's slice: a power of two up to 32
+  int per_part;                  // sorted places per group of L lanes
   float scale;
   int add;
 };
 
 template <bool kDwF32, bool kVec>
-__device__ __forceinline__ void flush_row(const RedArgs &a, uint32_t v, int c0, int lane, const float acc[8]) {
-  void *row = row_ptr<kDwF32>(a.dw, v, a.dw_ld);
+__device__ __forceinline__ void finish_row(const RedArgs &a, void *row, int c, const float acc[8],
+                                           const Row8<kDwF32, kVec> &old) {
   float x[8];
-  if (a.add) {
-    load8<kDwF32, kVec>(row, c0, lane, a.D, x);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) x[k] = __fadd_rn(x[k], __fmul_rn(a.scale, acc[k]));
-  } else {
-#pragma unroll
-    for (int k = 0; k < 8; ++k) x[k] = __fmul_rn(a.scale, acc[k]);
+  for (int k = 0; k < 8; ++k) {
+    x[k] = __fmul_rn(a.scale, acc[k]);
+    if (a.add) x[k] = __fadd_rn(elem(old, k), x[k]);
   }
-  store8<kDwF32, kVec>(row, c0, lane, a.D, x);
+  store_row<kDwF32, kVec>(row, c, a.L, a.D, x);
 }
 
-// A CTA takes one piece of kRedWarps * per_warp sorted places and one slice of columns; its warps take
-// equal parts.  A run inside a warp's part goes straight to the table.  The sums of runs that are open at
-// a part's start or end are left in shared memory and joined in order; what is still open at the
-// piece's start or end goes to `partial`.
+template <bool kDwF32, bool kVec>
+__device__ __forceinline__ void flush_row(const RedArgs &a, uint32_t v, int c, const float acc[8]) {
+  void *row = row_ptr<kDwF32>(a.dw, v, a.dw_ld);
+  Row8<kDwF32, kVec> old = {};
+  load_row<kDwF32, kVec>(old, row, c, a.L, a.D, a.add);
+  finish_row<kDwF32, kVec>(a, row, c, acc, old);
+}
+
+// A CTA takes one piece of the sorted list and one slice of 8 * L columns; each of its groups of L lanes
+// takes per_part places of the piece.  A run inside a part goes straight to the table.  The sums of runs
+// that are open at a part's start or end are left in shared memory and joined in order by the group in whose
+// part the run starts; what is still open at the piece's start or end goes to `partial`.
+//
+// Bound by memory latency unless enough rows are in flight: a group always has the rows of the next kAhead
+// places on the way and, with "add", the old table rows of the runs that end among the next kOldAhead.
 template <bool kDyF32, bool kDwF32, bool kVec>
-__global__ void __launch_bounds__(kRedWarps * 32)
+__global__ void __launch_bounds__(kRedThreads, 2)
 embedding_reduce_kernel(RedArgs a) {
-  __shared__ float open_sum[kRedWarps][2][kSliceCols];
-  __shared__ uint32_t open_key[kRedWarps][2];      // V: nothing open
-  __shared__ uint32_t through[kRedWarps];          // the part is one run, open at both ends (slot 0)
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  __shared__ float open_sum[2][kRedThreads * 8];      // [slot][part][8 * L]
+  __shared__ uint32_t open_key[2][kRedThreads];       // V: nothing open
+  __shared__ uint8_t through[kRedThreads];            // the part is one run, open at both ends (slot 0)
+  __shared__ uint2 list[kMaxPiece + 2];               // the piece's places and one on either side
+  constexpr int kAhead = (kDyF32 || !kVec) ? 4 : 8, kOldAhead = 4;
+  pdl_trigger();
+  const int L = a.L, l = threadIdx.x & (L - 1), part = threadIdx.x / L, parts = kRedThreads / L;
   const int64_t piece = blockIdx.x / a.slices;
-  const int slice = (int)(blockIdx.x - piece * a.slices), c0 = slice * kSliceCols;
-  const int64_t p0 = piece * (kRedWarps * (int64_t)a.per_warp), w0 = p0 + (int64_t)warp * a.per_warp;
-  const int n = (int)(a.T - w0 < a.per_warp ? (a.T - w0 > 0 ? a.T - w0 : 0) : a.per_warp);
-  uint32_t key = a.V, pos = 0, prev = a.V, next = a.V;
-  if (lane < n) {
-    key = __ldg(a.key + w0 + lane);
-    pos = __ldg(a.pos + w0 + lane);
+  const int slice = (int)(blockIdx.x - piece * a.slices), c = first_col<kVec>(slice * 8 * L, l);
+  const int len = parts * a.per_part;
+  const int64_t p0 = piece * len;
+  for (int i = threadIdx.x; i < 2 * parts; i += kRedThreads) open_key[i & 1][i >> 1] = a.V;
+  if (l == 0) through[part] = 0;
+  pdl_wait();
+  int live = 0;      // the padding lies behind the last run
+  for (int i0 = 0; i0 < len + 2; i0 += kRedThreads) {
+    const int i = i0 + threadIdx.x;
+    const int64_t g = p0 + i - 1;
+    uint2 e = make_uint2(a.V, 0u);
+    if (i < len + 2 && g >= 0 && g < a.T) e = __ldcg(a.list + g);
+    if (i < len + 2) list[i] = e;
+    live += __syncthreads_count(i >= 1 && i <= len && e.x < a.V);
   }
+  const uint2 *mine = list + 1 + part * a.per_part;
+  int n = live - part * a.per_part;
+  n = n < 0 ? 0 : n > a.per_part ? a.per_part : n;
   if (n > 0) {
-    if (w0 > 0) prev = __ldg(a.key + w0 - 1);
-    if (w0 + n < a.T) next = __ldg(a.key + w0 + n);
-  }
-  if (lane < 2) open_key[warp][lane] = a.V;
-  if (lane == 0) through[warp] = 0u;
-  __syncwarp();
-  float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  bool from_before = n > 0 && __shfl_sync(0xFFFFFFFFu, key, 0) == prev;
-  constexpr int kBatch = 4;
-  for (int j0 = 0; j0 < n; j0 += kBatch) {
-    float x[kBatch][8];
+    const uint32_t prev = mine[-1].x;
+    Row8<kDyF32, kVec> x[kAhead] = {};
+    Row8<kDwF32, kVec> old[kOldAhead] = {};
+    auto fetch = [&](Row8<kDyF32, kVec> &r, int j) {
+      load_row<kDyF32, kVec>(r, row_ptr<kDyF32>(a.dy, mine[j < n ? j : 0].y, a.dy_ld), c, L, a.D, j < n);
+    };
+    auto fetch_old = [&](Row8<kDwF32, kVec> &r, int j) {
+      const int i = j < n ? j : 0;
+      const uint32_t k = mine[i].x;
+      load_row<kDwF32, kVec>(r, row_ptr<kDwF32>(a.dw, k, a.dw_ld), c, L, a.D,
+                             a.add && j < n && mine[i + 1].x != k && k != prev);
+    };
 #pragma unroll
-    for (int b = 0; b < kBatch; ++b) {
-      const int j = j0 + b;
-      const uint32_t k = __shfl_sync(0xFFFFFFFFu, key, j & 31), t = __shfl_sync(0xFFFFFFFFu, pos, j & 31);
-      if (j < n && k < a.V) load8<kDyF32, kVec>(row_ptr<kDyF32>(a.dy, t, a.dy_ld), c0, lane, a.D, x[b]);
-    }
+    for (int b = 0; b < kAhead; ++b) fetch(x[b], b);
 #pragma unroll
-    for (int b = 0; b < kBatch; ++b) {
-      const int j = j0 + b;
-      const uint32_t k = __shfl_sync(0xFFFFFFFFu, key, j & 31);
-      const uint32_t kn = j + 1 < n ? __shfl_sync(0xFFFFFFFFu, key, (j + 1) & 31) : next;
-      if (j >= n || k >= a.V) continue;
+    for (int b = 0; b < kOldAhead; ++b) fetch_old(old[b], b);
+    float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    for (int j0 = 0; j0 < n; j0 += kAhead) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) acc[e] = __fadd_rn(acc[e], x[b][e]);
-      if (j + 1 < n && kn == k) continue;
-      const bool goes_on = j + 1 >= n && kn == k;
-      if (!from_before && !goes_on) {
-        flush_row<kDwF32, kVec>(a, k, c0, lane, acc);
-      } else {
-        const int s = from_before ? 0 : 1;
+      for (int b = 0; b < kAhead; ++b) {
+        const int j = j0 + b;
+        if (j >= n) break;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) open_sum[warp][s][e * 32 + lane] = acc[e];
-        if (lane == 0) {
-          open_key[warp][s] = k;
-          if (from_before && goes_on) through[warp] = 1u;
+        for (int e = 0; e < 8; ++e) acc[e] = __fadd_rn(acc[e], elem(x[b], e));
+        fetch(x[b], j + kAhead);
+        const uint32_t k = mine[j].x;
+        const bool ends = mine[j + 1].x != k;
+        if (ends || j + 1 == n) {
+          if (ends && k != prev) {
+            finish_row<kDwF32, kVec>(a, row_ptr<kDwF32>(a.dw, k, a.dw_ld), c, acc, old[b % kOldAhead]);
+          } else {
+            const int s = k == prev ? 0 : 1;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) open_sum[s][part * 8 * L + e * L + l] = acc[e];
+            if (l == 0) {
+              open_key[s][part] = k;
+              if (s == 0 && !ends) through[part] = 1;
+            }
+          }
+#pragma unroll
+          for (int e = 0; e < 8; ++e) acc[e] = 0.f;
         }
+        fetch_old(old[b % kOldAhead], j + kOldAhead);
       }
-      from_before = false;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) acc[e] = 0.f;
     }
   }
   __syncthreads();
-  // Join the parts in order; warp 0, each lane its eight columns of every part.
-  if (warp != 0) return;
-  float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  bool have = false, started_before = false;
-  float *part = a.partial + (piece * 2 * a.slices + slice) * (int64_t)kSliceCols;
-  const int64_t slot = (int64_t)a.slices * kSliceCols;
-  for (int w = 0; w < kRedWarps; ++w) {
-    const uint32_t k0 = open_key[w][0];
-    if (k0 != a.V) {
-      if (!have) started_before = true;       // only the piece's first part can continue an unseen run
+  float *partial = a.partial + (piece * 2 * a.slices + slice) * (int64_t)(8 * L) + l;
+  const int64_t slot = (int64_t)a.slices * 8 * L;
+  // the run this part starts and leaves open
+  const uint32_t ko = open_key[1][part];
+  if (ko != a.V) {
+    float sum[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) sum[e] = have ? __fadd_rn(sum[e], open_sum[w][0][e * 32 + lane]) : open_sum[w][0][e * 32 + lane];
-      have = true;
-      if (!through[w]) {
-        if (started_before) {
+    for (int e = 0; e < 8; ++e) sum[e] = open_sum[1][part * 8 * L + e * L + l];
+    bool open = true;
+    for (int q = part + 1; q < parts && open; ++q) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) part[e * 32 + lane] = sum[e];
-        } else {
-          flush_row<kDwF32, kVec>(a, k0, c0, lane, sum);
-        }
-        have = started_before = false;
-      }
+      for (int e = 0; e < 8; ++e) sum[e] = __fadd_rn(sum[e], open_sum[0][q * 8 * L + e * L + l]);
+      open = through[q];
     }
-    if (open_key[w][1] != a.V) {
+    if (!open) {
+      flush_row<kDwF32, kVec>(a, ko, c, sum);
+    } else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) sum[e] = open_sum[w][1][e * 32 + lane];
-      have = true;
+      for (int e = 0; e < 8; ++e) partial[slot + e * L] = sum[e];
     }
   }
-  if (have) {
-    float *p = part + (started_before ? 0 : slot);
+  // the run that was open before the piece
+  if (part == 0 && open_key[0][0] != a.V) {
+    float sum[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) p[e * 32 + lane] = sum[e];
+    for (int e = 0; e < 8; ++e) sum[e] = open_sum[0][e * L + l];
+    for (int q = 1; q < parts && through[q - 1]; ++q) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sum[e] = __fadd_rn(sum[e], open_sum[0][q * 8 * L + e * L + l]);
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) partial[e * L] = sum[e];
   }
 }
 
 // Runs that cross pieces.  A CTA takes one piece and one slice; if a run starts in the piece and is still
-// open at its end, its warps add the partial sums of the pieces it covers, each warp a stretch, and the
-// stretches are added in order.
+// open at its end, its groups add the partial sums of the pieces it covers, group i those of every parts-th piece
+// from the i-th, and the groups' sums are added in order.
 template <bool kDwF32, bool kVec>
-__global__ void __launch_bounds__(kRedWarps * 32)
+__global__ void __launch_bounds__(kRedThreads)
 embedding_join_kernel(RedArgs a, int64_t pieces) {
-  __shared__ float sums[kRedWarps][kSliceCols];
+  __shared__ float sums[kRedThreads * 8];
   __shared__ int64_t s_last;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  pdl_trigger();
+  const int L = a.L, l = threadIdx.x & (L - 1), part = threadIdx.x / L, parts = kRedThreads / L;
   const int64_t piece = blockIdx.x / a.slices;
-  const int slice = (int)(blockIdx.x - piece * a.slices), c0 = slice * kSliceCols;
-  const int64_t len = kRedWarps * (int64_t)a.per_warp, p0 = piece * len, p1 = p0 + len;
+  const int slice = (int)(blockIdx.x - piece * a.slices), c = first_col<kVec>(slice * 8 * L, l);
+  const int64_t len = (int64_t)parts * a.per_part, p0 = piece * len, p1 = p0 + len;
+  pdl_wait();
   if (p1 >= a.T) return;
-  const uint32_t k = __ldg(a.key + p1 - 1);
-  if (k >= a.V || __ldg(a.key + p1) != k) return;
-  if (p0 > 0 && __ldg(a.key + p0 - 1) == k) return;        // the run starts in an earlier piece
-  if (warp == 0) {      // last piece of the run: pieces start with k up to there
+  const uint32_t k = __ldcg(&a.list[p1 - 1].x), k1 = __ldcg(&a.list[p1].x), kp = p0 > 0 ? __ldcg(&a.list[p0 - 1].x) : a.V;
+  if (k >= a.V || k1 != k || kp == k) return;      // no open run, or one that starts in an earlier piece
+  if (threadIdx.x < 32) {      // last piece of the run: pieces start with k up to there
     int64_t last = piece;
     for (int64_t q0 = piece + 1; q0 < pieces; q0 += 32) {
-      const bool same = q0 + lane < pieces && __ldg(a.key + (q0 + lane) * len) == k;
+      const int64_t q = q0 + threadIdx.x;
+      const bool same = q < pieces && __ldcg(&a.list[q * len].x) == k;
       const uint32_t m = __ballot_sync(0xFFFFFFFFu, same);
       last += __popc(m);
       if (m != 0xFFFFFFFFu) break;
     }
-    if (lane == 0) s_last = last;
+    if (threadIdx.x == 0) s_last = last;
   }
   __syncthreads();
-  const int64_t last = s_last, count = last - piece;      // pieces piece + 1 .. last
-  const int64_t slot = (int64_t)a.slices * kSliceCols;
-  const float *base = a.partial + (int64_t)slice * kSliceCols + lane;
-  const int64_t q0 = piece + 1 + count * warp / kRedWarps, q1 = piece + 1 + count * (warp + 1) / kRedWarps;
+  const int64_t count = s_last - piece;      // pieces piece + 1 .. s_last
+  const int64_t slot = (int64_t)a.slices * 8 * L;
+  const float *base = a.partial + (int64_t)slice * 8 * L + l;
   float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-  for (int64_t q = q0; q < q1; ++q) {
+  for (int64_t q = piece + 1 + part; q <= s_last; q += parts) {
     const float *p = base + q * 2 * slot;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) acc[e] = __fadd_rn(acc[e], p[e * 32]);
+    for (int e = 0; e < 8; ++e) acc[e] = __fadd_rn(acc[e], __ldcg(p + e * L));
   }
 #pragma unroll
-  for (int e = 0; e < 8; ++e) sums[warp][e * 32 + lane] = acc[e];
+  for (int e = 0; e < 8; ++e) sums[part * 8 * L + e * L + l] = acc[e];
   __syncthreads();
-  if (warp != 0) return;
+  if (part != 0) return;
   const float *first = base + (piece * 2 + 1) * slot;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    acc[e] = first[e * 32];
-    for (int w = 0; w < kRedWarps; ++w) acc[e] = __fadd_rn(acc[e], sums[w][e * 32 + lane]);
+  for (int e = 0; e < 8; ++e) acc[e] = __ldcg(first + e * L);
+  for (int w = 0; w < parts && w < count; ++w)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) acc[e] = __fadd_rn(acc[e], sums[w * 8 * L + e * L + l]);
+  flush_row<kDwF32, kVec>(a, k, c, acc);
+}
+
+// ------------------------------------------------------------------ few tokens
+// Up to kSmallT tokens need no sort: every CTA links the equal ids of the list in shared memory, and
+// the group of lanes of each id's first token adds the rows along the links.  One launch.
+constexpr int kSmallT = 128;
+
+template <bool kDyF32, bool kDwF32, bool kVec>
+__global__ void __launch_bounds__(kRedThreads)
+embedding_small_kernel(RedArgs a, const void *__restrict__ ids, int ids64, int64_t padding_idx, uint32_t *status) {
+  __shared__ uint32_t key[kSmallT];
+  __shared__ int16_t link[kSmallT];            // next token with the same id, -1: none
+  __shared__ uint8_t head[kSmallT];
+  constexpr int kBatch = 4;
+  const int T = (int)a.T;
+  if ((int)threadIdx.x < T) {
+    const int64_t id = load_id(ids, ids64, threadIdx.x);
+    key[threadIdx.x] = key_of(id, a.V, padding_idx);
+    if (id >= (int64_t)a.V && blockIdx.x == 0) atomicOr(status, ANC_DEV_BAD_INDEX);
   }
-  flush_row<kDwF32, kVec>(a, k, c0, lane, acc);
+  __syncthreads();
+  if ((int)threadIdx.x < T) {
+    const uint32_t k = key[threadIdx.x];
+    int next = -1;
+    bool first = k < a.V;
+    for (int t = T - 1; t >= 0; --t) {
+      const bool same = key[t] == k;
+      if (same && t > (int)threadIdx.x) next = t;
+      if (same && t < (int)threadIdx.x) first = false;
+    }
+    link[threadIdx.x] = (int16_t)next;
+    head[threadIdx.x] = first;
+  }
+  __syncthreads();
+  pdl_wait();      // the zeros of the table, when the whole table is written
+  const int L = a.L, l = threadIdx.x & (L - 1);
+  const int64_t u = (int64_t)blockIdx.x * (kRedThreads / L) + threadIdx.x / L;
+  const int64_t t0 = u / a.slices;
+  if (t0 >= T || !head[t0]) return;
+  const int c = first_col<kVec>((int)(u - t0 * a.slices) * 8 * L, l);
+  void *row = row_ptr<kDwF32>(a.dw, key[t0], a.dw_ld);
+  Row8<kDwF32, kVec> old = {};
+  load_row<kDwF32, kVec>(old, row, c, L, a.D, a.add);
+  float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  for (int t = (int)t0; t >= 0;) {
+    Row8<kDyF32, kVec> x[kBatch] = {};
+    int m = 0;
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b) {
+      load_row<kDyF32, kVec>(x[b], row_ptr<kDyF32>(a.dy, t < 0 ? 0 : t, a.dy_ld), c, L, a.D, t >= 0);
+      if (t >= 0) {
+        t = link[t];
+        m = b + 1;
+      }
+    }
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b)
+      if (b < m) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) acc[e] = __fadd_rn(acc[e], elem(x[b], e));
+      }
+  }
+  finish_row<kDwF32, kVec>(a, row, c, acc, old);
 }
 
 // ------------------------------------------------------------------ host side
+constexpr int kMaxPart = 32, kMinPart = 4;
+constexpr int64_t kFullGrid = 888;       // CTAs the reduction should have at least
+
 struct Shape {
-  int slices, per_warp;
-  int64_t pieces;
+  int L, slices, per_part;
+  int64_t pieces, max_pieces;
 };
 
 Shape shape_of(int64_t T, int64_t D) {
   Shape s;
-  s.slices = (int)((D + kSliceCols - 1) / kSliceCols);
-  s.per_warp = 32;
-  s.pieces = (T + kRedWarps * s.per_warp - 1) / (kRedWarps * s.per_warp);
+  s.L = 1;
+  while (s.L < 32 && s.L * 8 < D) s.L *= 2;
+  s.slices = (int)((D + s.L * 8 - 1) / (s.L * 8));
+  // parts as long as leaves enough of them to fill the GPU
+  const int64_t parts_per_cta = kRedThreads / s.L;
+  s.per_part = kMaxPiece / parts_per_cta < kMaxPart ? (int)(kMaxPiece / parts_per_cta) : kMaxPart;
+  while (s.per_part > kMinPart && (T / (parts_per_cta * s.per_part)) * s.slices < kFullGrid) s.per_part /= 2;
+  s.pieces = (T + parts_per_cta * s.per_part - 1) / (parts_per_cta * s.per_part);
+  // most pieces any smaller T has: the workspace for T serves every smaller T
+  const int64_t most = 2 * (kFullGrid / s.slices) + 4;
+  const int64_t finest = (T + parts_per_cta * kMinPart - 1) / (parts_per_cta * kMinPart);
+  const int64_t bound = most < finest ? most : finest;
+  s.max_pieces = s.pieces > bound ? s.pieces : bound;
   return s;
 }
 
 struct Workspace {
-  size_t key[2], pos[2], partial, total;
+  size_t list[2], partial, total;
 };
 
 Workspace workspace_of(int64_t T, int64_t D) {
@@ -481,13 +701,11 @@ Workspace workspace_of(int64_t T, int64_t D) {
   Workspace w;
   size_t at = 0;
   for (int i = 0; i < 2; ++i) {
-    w.key[i] = at;
-    at += up((size_t)T * 4);
-    w.pos[i] = at;
-    at += up((size_t)T * 4);
+    w.list[i] = at;
+    at += up((size_t)T * sizeof(uint2));
   }
   w.partial = at;
-  at += up((size_t)s.pieces * 2 * s.slices * kSliceCols * 4);
+  at += up((size_t)s.max_pieces * 2 * s.slices * 8 * s.L * 4);
   w.total = at ? at : 256;
   return w;
 }
@@ -504,6 +722,18 @@ int check_sizes(int64_t T, int64_t V, int64_t D) {
 int check_dtype(int d, const char *what) {
   ANC_REQUIRE(d == ANC_GRAD_BF16 || d == ANC_GRAD_F32, "bad %s %d", what, d);
   return ANC_OK;
+}
+
+// Raises the sort's shared-memory limit once per device.
+cudaError_t sort_kernel_ready(int device) {
+  static std::mutex mu;
+  static bool done[64] = {};
+  std::lock_guard<std::mutex> lock(mu);
+  if (device >= 0 && device < 64 && done[device]) return cudaSuccess;
+  const cudaError_t e =
+      cudaFuncSetAttribute(embedding_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSortSmem);
+  if (e == cudaSuccess && device >= 0 && device < 64) done[device] = true;
+  return e;
 }
 
 bool rows_are_vectors(const void *p, int64_t ld, int f32, int64_t D) {
@@ -534,14 +764,13 @@ int anc_embedding_lookup(anc_ctx *ctx, const void *table, int table_dtype, int64
               "pointer not aligned to its element size");
   anc_device_guard guard(ctx->device);
   cudaStream_t st = anc_pick_stream(ctx, stream);
-  const int slices = (int)((D + kSliceCols - 1) / kSliceCols);
-  int64_t blocks = (T * slices + kLookupWarps - 1) / kLookupWarps;
-  const int64_t cap = (int64_t)ctx->sm_count * 64;
-  if (blocks > cap) blocks = cap;
   const bool vec = rows_are_vectors(table, table_ld, tf, D) && rows_are_vectors(out, out_ld, of, D);
+  const int64_t total = T * (vec ? D / 8 : D), per_block = kLookupThreads * (vec ? 4 : 8);
+  int64_t blocks = (total + per_block - 1) / per_block;
+  if (blocks > (1 << 30)) blocks = 1 << 30;
 #define ANC_LOOKUP(F, O, VEC)                                                                             \
-  embedding_lookup_kernel<F, O, VEC><<<(unsigned)blocks, kLookupWarps * 32, 0, st>>>(                     \
-      table, table_ld, ids, i64, out, out_ld, T, V, (int)D, slices, scale, ctx->d_status)
+  embedding_lookup_kernel<F, O, VEC><<<(unsigned)blocks, kLookupThreads, 0, st>>>(                        \
+      table, table_ld, ids, i64, out, out_ld, V, (int)D, total, scale, ctx->d_status)
 #define ANC_LOOKUP_V(F, O)                \
   do {                                    \
     if (vec) ANC_LOOKUP(F, O, true);      \
@@ -592,31 +821,48 @@ int anc_embedding_grad(anc_ctx *ctx, const void *dy, int dy_dtype, int64_t dy_ld
   if (T == 0 && mode == ANC_EMBED_ADD) return ANC_OK;
   anc_device_guard guard(ctx->device);
   cudaStream_t st = anc_pick_stream(ctx, stream);
-  if (mode == ANC_EMBED_WRITE) {
-    const int64_t row = D * (wf ? 4 : 2), pitch = dw_ld * (wf ? 4 : 2);
-    const int vec = ((uintptr_t)dw & 15) == 0 && pitch % 16 == 0 && row % 16 == 0;
-    const int64_t items = V * (row / (vec ? 16 : 2));
-    int64_t blocks = (items + 255) / 256;
-    const int64_t cap = (int64_t)ctx->sm_count * 16;
-    if (blocks > cap) blocks = cap;
-    embedding_zero_kernel<<<(unsigned)blocks, 256, 0, st>>>((uint8_t *)dw, row, pitch, V, vec);
-    ANC_CUDA(cudaGetLastError());
-  }
+  ZeroArgs za = {};
+  za.dw = (uint8_t *)dw;
+  za.row_bytes = D * (wf ? 4 : 2);
+  za.pitch = dw_ld * (wf ? 4 : 2);
+  za.V = V;
+  za.vec = ((uintptr_t)dw & 15) == 0 && za.pitch % 16 == 0 && za.row_bytes % 16 == 0;
+  const bool write = mode == ANC_EMBED_WRITE, small = T <= kSmallT;
+  cudaLaunchAttribute pdl[1];
+  pdl[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  pdl[0].val.programmaticStreamSerializationAllowed = 1;
+  auto launch_zero = [&](int n_attrs) {
+    const int64_t items = V * (za.row_bytes / (za.vec ? 16 : 2)), cap = (int64_t)ctx->sm_count * 16;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)((items + 255) / 256 < cap ? (items + 255) / 256 : cap));
+    cfg.blockDim = dim3(256);
+    cfg.stream = st;
+    cfg.attrs = pdl;
+    cfg.numAttrs = n_attrs;
+    return cudaLaunchKernelEx(&cfg, embedding_zero_kernel, za);
+  };
+  if (write && small) ANC_CUDA(launch_zero(0));
   if (T == 0) return ANC_OK;
   uint8_t *wp = (uint8_t *)work;
   SortArgs sa;
   sa.ids = ids; sa.ids64 = i64; sa.T = T; sa.V = V; sa.padding_idx = padding_idx;
-  for (int i = 0; i < 2; ++i) {
-    sa.key[i] = (uint32_t *)(wp + ws.key[i]);
-    sa.pos[i] = (uint32_t *)(wp + ws.pos[i]);
-  }
+  for (int i = 0; i < 2; ++i) sa.list[i] = (uint2 *)(wp + ws.list[i]);
   int bits = 0;
   while (((uint64_t)V >> bits) != 0) ++bits;
   sa.passes = (bits + kDigitBits - 1) / kDigitBits;
   sa.status = ctx->d_status;
-  const uint32_t n_ctas = T <= 4096 ? 1 : T <= 8192 ? 2 : T <= 16384 ? 4 : 8;
-  {
-    ANC_CUDA(cudaFuncSetAttribute(embedding_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSortSmem));
+  const Shape sh = shape_of(T, D);
+  RedArgs ra;
+  ra.dy = dy; ra.dw = dw; ra.dy_ld = dy_ld; ra.dw_ld = dw_ld; ra.T = T;
+  ra.list = sa.list[(sa.passes - 1) & 1];
+  ra.partial = (float *)(wp + ws.partial);
+  ra.V = (uint32_t)V; ra.D = (int)D; ra.slices = sh.slices; ra.L = sh.L; ra.per_part = sh.per_part; ra.scale = scale;
+  ra.add = !write;
+  const int64_t grid = small ? (T * sh.slices + kRedThreads / sh.L - 1) / (kRedThreads / sh.L) : sh.pieces * sh.slices;
+  ANC_REQUIRE(grid <= 0x7FFFFFFF, "T x D too large");
+  if (!small) {
+    ANC_CUDA(sort_kernel_ready(ctx->device));
+    const uint32_t n_ctas = T <= 4096 ? 1 : T <= 8192 ? 2 : T <= 16384 ? 4 : 8;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(n_ctas);
     cfg.blockDim = dim3(kSortThreads);
@@ -630,22 +876,24 @@ int anc_embedding_grad(anc_ctx *ctx, const void *dy, int dy_dtype, int64_t dy_ld
     cfg.attrs = at;
     cfg.numAttrs = 1;
     ANC_CUDA(cudaLaunchKernelEx(&cfg, embedding_sort_kernel, sa, n_ctas));
+    if (write) ANC_CUDA(launch_zero(1));
   }
-  const Shape sh = shape_of(T, D);
-  RedArgs ra;
-  ra.dy = dy; ra.dw = dw; ra.dy_ld = dy_ld; ra.dw_ld = dw_ld; ra.T = T;
-  ra.key = sa.key[(sa.passes - 1) & 1];
-  ra.pos = sa.pos[(sa.passes - 1) & 1];
-  ra.partial = (float *)(wp + ws.partial);
-  ra.V = (uint32_t)V; ra.D = (int)D; ra.slices = sh.slices; ra.per_warp = sh.per_warp; ra.scale = scale;
-  ra.add = mode == ANC_EMBED_ADD;
-  const int64_t grid = sh.pieces * sh.slices;
-  ANC_REQUIRE(grid <= 0x7FFFFFFF, "T x D too large");
+  // the following launches start while their predecessor drains and wait for it on the device
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)grid);
+  cfg.blockDim = dim3(kRedThreads);
+  cfg.stream = st;
+  cfg.attrs = pdl;
+  cfg.numAttrs = small && !write ? 0 : 1;
   const bool vec = rows_are_vectors(dy, dy_ld, yf, D) && rows_are_vectors(dw, dw_ld, wf, D);
 #define ANC_REDUCE(Y, W, VEC)                                                                        \
   do {                                                                                               \
-    embedding_reduce_kernel<Y, W, VEC><<<(unsigned)grid, kRedWarps * 32, 0, st>>>(ra);               \
-    if (sh.pieces > 1) embedding_join_kernel<W, VEC><<<(unsigned)grid, kRedWarps * 32, 0, st>>>(ra, sh.pieces); \
+    if (small) {                                                                                     \
+      ANC_CUDA(cudaLaunchKernelEx(&cfg, embedding_small_kernel<Y, W, VEC>, ra, ids, i64, padding_idx, ctx->d_status)); \
+    } else {                                                                                         \
+      ANC_CUDA(cudaLaunchKernelEx(&cfg, embedding_reduce_kernel<Y, W, VEC>, ra));                    \
+      if (sh.pieces > 1) ANC_CUDA(cudaLaunchKernelEx(&cfg, embedding_join_kernel<W, VEC>, ra, sh.pieces)); \
+    }                                                                                                \
   } while (0)
 #define ANC_REDUCE_V(Y, W)                \
   do {                                    \
