@@ -92,6 +92,7 @@ SIGNATURES = {
     "anc_adamw_plan_set_schedule": (_i, [_vp, C.POINTER(AdamWScalars), _i, _u64]),
     "anc_adamw_plan_set_counter": (_i, [_vp, _u64, _vp]),
     "anc_adamw_step_scheduled": (_i, [_vp, _i, _u64, _i, _vp]),
+    "anc_adamw_plan_set_grad_scale": (_i, [_vp, _vp]),
     "anc_adamw_plan_destroy": (_i, [_vp]),
     "anc_muon_plan_create": (_i, [_vp, C.POINTER(MuonWeight), _i, _i, _i, _i, _pp]),
     "anc_muon_plan_create_ex": (_i, [_vp, C.POINTER(MuonWeight), C.POINTER(MuonOutputs), _i, _i, _i, _i, _pp]),
@@ -99,6 +100,7 @@ SIGNATURES = {
     "anc_muon_plan_num_groups": (_i, [_vp, C.POINTER(_i)]),
     "anc_muon_plan_group_info": (_i, [_vp, _i, C.POINTER(C.c_int32)]),
     "anc_muon_step_range": (_i, [_vp, _i, _i, _i, _d, _f, _i, _i, C.POINTER(_f), _f, _vp]),
+    "anc_muon_plan_set_grad_scale": (_i, [_vp, _vp]),
     "anc_muon_plan_set_timing": (_i, [_vp, _i]),
     "anc_muon_plan_last_timing": (_i, [_vp, C.POINTER(_f), C.POINTER(_d), C.POINTER(_i)]),
     "anc_muon_plan_scratch_bytes": (_i, [_vp, C.POINTER(_u64)]),

@@ -101,6 +101,11 @@ class ResidentAdamW:
         L.check(L.lib().anc_adamw_step_scheduled(self.handle, _ROUND[self.rounding], self.seed,
                                                  int(bool(advance)), C.c_void_p(si or None)))
 
+    def set_grad_scale(self, scale):
+        """Every later step multiplies the gradients by the float32 at this device address as it loads them
+        (``GradClip.factor_ptr``); None: not."""
+        L.check(L.lib().anc_adamw_plan_set_grad_scale(self.handle, dev_ptr(scale)))
+
     def free(self):
         if self.handle:
             L.lib().anc_adamw_plan_destroy(self.handle)

@@ -107,10 +107,14 @@ __device__ __forceinline__ void load_grad8(const void *g, uint64_t i, float out[
 }
 
 // The update of one 8-element group held in registers and its stores (i = offset inside the chunk).
-template <bool kSR>
+template <bool kSR, bool kScaled>
 __device__ __forceinline__ void finish8(const Chunk &ch, uint32_t i, float g[8], float p[8], float m[8],
                                         float v[8], const Scalars &s, uint32_t seed_lo, uint32_t seed_hi,
-                                        uint32_t step_lo, uint32_t step_hi) {
+                                        uint32_t step_lo, uint32_t step_hi, float gscale) {
+  if constexpr (kScaled) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) g[k] = __fmul_rn(g[k], gscale);
+  }
 #pragma unroll
   for (int k = 0; k < 8; ++k) adamw_elem(g[k], p[k], m[k], v[k], ch.wd, s);
   uint32_t h[8];
@@ -140,9 +144,9 @@ __device__ __forceinline__ void finish8(const Chunk &ch, uint32_t i, float g[8],
 // A chunk the bulk copies cannot serve (a tensor whose pointers are not 16-byte aligned, or the
 // ragged last chunk of a tensor): plain loads, 128-bit where the alignment allows, then
 // element by element.  Same arithmetic, same Philox block per 8 elements.
-template <bool kGradF32, bool kSR>
+template <bool kGradF32, bool kSR, bool kScaled>
 __device__ __forceinline__ void direct_chunk(const Chunk &ch, int tid, const Scalars &s, uint32_t seed_lo,
-                                             uint32_t seed_hi, uint32_t step_lo, uint32_t step_hi) {
+                                             uint32_t seed_hi, uint32_t step_lo, uint32_t step_hi, float gscale) {
   const uint32_t groups = ch.aligned ? (ch.count >> 3) : 0u;
   for (uint32_t gi = tid; gi < groups; gi += kThreads) {
     const uint32_t i = gi * 8;
@@ -157,12 +161,13 @@ __device__ __forceinline__ void direct_chunk(const Chunk &ch, int tid, const Sca
     p[0] = p0.x; p[1] = p0.y; p[2] = p0.z; p[3] = p0.w; p[4] = p1.x; p[5] = p1.y; p[6] = p1.z; p[7] = p1.w;
     m[0] = m0.x; m[1] = m0.y; m[2] = m0.z; m[3] = m0.w; m[4] = m1.x; m[5] = m1.y; m[6] = m1.z; m[7] = m1.w;
     v[0] = v0.x; v[1] = v0.y; v[2] = v0.z; v[3] = v0.w; v[4] = v1.x; v[5] = v1.y; v[6] = v1.z; v[7] = v1.w;
-    finish8<kSR>(ch, i, g, p, m, v, s, seed_lo, seed_hi, step_lo, step_hi);
+    finish8<kSR, kScaled>(ch, i, g, p, m, v, s, seed_lo, seed_hi, step_lo, step_hi, gscale);
   }
   for (uint32_t i = (groups << 3) + tid; i < ch.count; i += kThreads) {
     float g;
     if constexpr (kGradF32) g = ((const float *)ch.g)[i];
     else g = __uint_as_float((uint32_t)((const uint16_t *)ch.g)[i] << 16);
+    if constexpr (kScaled) g = __fmul_rn(g, gscale);
     float p = ch.p[i], m = ch.m[i], v = ch.v[i];
     adamw_elem(g, p, m, v, ch.wd, s);
     uint32_t h;
@@ -187,12 +192,14 @@ __device__ __forceinline__ void direct_chunk(const Chunk &ch, int tid, const Sca
 // g) that fill it; the eight computing warps wait for the
 // stage, take eight elements per thread from shared memory, hand the stage back and update + store
 // from registers.
-template <bool kGradF32, bool kSR>
+// kScaled: every gradient is first multiplied by *grad_scale (one more rounded product), the clipping factor
+// that anc_grad_norm left in device memory.
+template <bool kGradF32, bool kSR, bool kScaled>
 __global__ void __launch_bounds__(kBlock, 1)
 adamw_multi_kernel(const Chunk *__restrict__ chunks, uint32_t n_chunks, Scalars s, uint32_t seed_lo,
                    uint32_t seed_hi, uint32_t step_lo, uint32_t step_hi, uint32_t *status,
                    const Scalars *__restrict__ sched, const unsigned long long *__restrict__ counter,
-                   unsigned long long sched_first, uint32_t sched_len) {
+                   unsigned long long sched_first, uint32_t sched_len, const float *__restrict__ grad_scale) {
   using R = Ring<kGradF32>;
   extern __shared__ __align__(128) uint8_t ring[];
   __shared__ __align__(8) uint64_t bars[2 * R::kStages];
@@ -248,6 +255,8 @@ adamw_multi_kernel(const Chunk *__restrict__ chunks, uint32_t n_chunks, Scalars 
     }
     return;
   }
+  float gscale = 1.f;
+  if constexpr (kScaled) gscale = *grad_scale;
   const uint32_t grp = (uint32_t)warp / (kThreads / 32);
   const int tid = threadIdx.x & (kThreads - 1);          // thread within its group
   uint32_t it = grp;
@@ -273,11 +282,11 @@ adamw_multi_kernel(const Chunk *__restrict__ chunks, uint32_t n_chunks, Scalars 
       }
       __syncwarp();
       if (lane == 0) anc_ring::mbar_arrive(empty0 + 8 * slot);
-      if (act) finish8<kSR>(ch, (uint32_t)t * 8u, g, p, m, v, s, seed_lo, seed_hi, step_lo, step_hi);
+      if (act) finish8<kSR, kScaled>(ch, (uint32_t)t * 8u, g, p, m, v, s, seed_lo, seed_hi, step_lo, step_hi, gscale);
     } else {
       __syncwarp();
       if (lane == 0) anc_ring::mbar_arrive(empty0 + 8 * slot);
-      direct_chunk<kGradF32, kSR>(ch, tid, s, seed_lo, seed_hi, step_lo, step_hi);
+      direct_chunk<kGradF32, kSR, kScaled>(ch, tid, s, seed_lo, seed_hi, step_lo, step_hi, gscale);
     }
   }
 }
@@ -299,6 +308,7 @@ struct anc_adamw_plan {
   unsigned long long *d_counter = nullptr;
   unsigned long long sched_first = 0;
   uint32_t sched_len = 0;
+  const float *grad_scale = nullptr;       // optional device-resident factor on every gradient
 };
 
 static int adamw_build_chunks(anc_adamw_plan *pl, uint64_t begin, uint64_t end) {
@@ -385,7 +395,10 @@ int anc_adamw_plan_create(anc_ctx *ctx, const anc_adamw_tensor *tensors, int n_t
     cudaError_t e = cudaSuccess;
 #define ANC_ADAMW_SMEM(F32, SR)                                                                      \
   if (e == cudaSuccess)                                                                              \
-    e = cudaFuncSetAttribute(adamw_multi_kernel<F32, SR>, cudaFuncAttributeMaxDynamicSharedMemorySize, \
+    e = cudaFuncSetAttribute(adamw_multi_kernel<F32, SR, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, \
+                             (int)Ring<F32>::kSmemBytes);                                            \
+  if (e == cudaSuccess)                                                                              \
+    e = cudaFuncSetAttribute(adamw_multi_kernel<F32, SR, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, \
                              (int)Ring<F32>::kSmemBytes)
     ANC_ADAMW_SMEM(true, true);
     ANC_ADAMW_SMEM(true, false);
@@ -437,9 +450,15 @@ int anc_adamw_step(anc_adamw_plan *plan, const anc_adamw_scalars *sc, int roundi
   if (grid > (uint32_t)ctx->sm_count) grid = (uint32_t)ctx->sm_count;
   const uint32_t sl = (uint32_t)seed, sh = (uint32_t)(seed >> 32);
   const uint32_t tl = (uint32_t)step, th = (uint32_t)(step >> 32);
-#define ANC_ADAMW_LAUNCH(F32, SR)                                                                  \
-  adamw_multi_kernel<F32, SR><<<grid, kBlock, Ring<F32>::kSmemBytes, st>>>(                 \
-      plan->d_chunks, plan->n_chunks, s, sl, sh, tl, th, ctx->d_status, nullptr, nullptr, 0ull, 0u)
+  const float *gs = plan->grad_scale;
+#define ANC_ADAMW_LAUNCH_C(F32, SR, SC)                                                            \
+  adamw_multi_kernel<F32, SR, SC><<<grid, kBlock, Ring<F32>::kSmemBytes, st>>>(             \
+      plan->d_chunks, plan->n_chunks, s, sl, sh, tl, th, ctx->d_status, nullptr, nullptr, 0ull, 0u, gs)
+#define ANC_ADAMW_LAUNCH(F32, SR)                \
+  do {                                           \
+    if (gs) ANC_ADAMW_LAUNCH_C(F32, SR, true);   \
+    else ANC_ADAMW_LAUNCH_C(F32, SR, false);     \
+  } while (0)
   const bool f32 = plan->grad_dtype == ANC_GRAD_F32;
   const bool sr = rounding == ANC_ROUND_SR;
   if (f32 && sr) ANC_ADAMW_LAUNCH(true, true);
@@ -447,6 +466,7 @@ int anc_adamw_step(anc_adamw_plan *plan, const anc_adamw_scalars *sc, int roundi
   else if (sr) ANC_ADAMW_LAUNCH(false, true);
   else ANC_ADAMW_LAUNCH(false, false);
 #undef ANC_ADAMW_LAUNCH
+#undef ANC_ADAMW_LAUNCH_C
   ANC_CUDA(cudaGetLastError());
   return ANC_OK;
 }
@@ -496,10 +516,16 @@ int anc_adamw_step_scheduled(anc_adamw_plan *plan, int rounding, uint64_t seed, 
     uint32_t grid = plan->n_chunks;
     if (grid > (uint32_t)ctx->sm_count) grid = (uint32_t)ctx->sm_count;
     const uint32_t sl = (uint32_t)seed, sh = (uint32_t)(seed >> 32);
-#define ANC_ADAMW_LAUNCH_S(F32, SR)                                                                 \
-  adamw_multi_kernel<F32, SR><<<grid, kBlock, Ring<F32>::kSmemBytes, st>>>(                  \
+    const float *gs = plan->grad_scale;
+#define ANC_ADAMW_LAUNCH_C(F32, SR, SC)                                                             \
+  adamw_multi_kernel<F32, SR, SC><<<grid, kBlock, Ring<F32>::kSmemBytes, st>>>(              \
       plan->d_chunks, plan->n_chunks, s, sl, sh, 0u, 0u, ctx->d_status, plan->d_sched,              \
-      plan->d_counter, plan->sched_first, plan->sched_len)
+      plan->d_counter, plan->sched_first, plan->sched_len, gs)
+#define ANC_ADAMW_LAUNCH_S(F32, SR)              \
+  do {                                           \
+    if (gs) ANC_ADAMW_LAUNCH_C(F32, SR, true);   \
+    else ANC_ADAMW_LAUNCH_C(F32, SR, false);     \
+  } while (0)
     const bool f32 = plan->grad_dtype == ANC_GRAD_F32;
     const bool sr = rounding == ANC_ROUND_SR;
     if (f32 && sr) ANC_ADAMW_LAUNCH_S(true, true);
@@ -507,12 +533,20 @@ int anc_adamw_step_scheduled(anc_adamw_plan *plan, int rounding, uint64_t seed, 
     else if (sr) ANC_ADAMW_LAUNCH_S(false, true);
     else ANC_ADAMW_LAUNCH_S(false, false);
 #undef ANC_ADAMW_LAUNCH_S
+#undef ANC_ADAMW_LAUNCH_C
     ANC_CUDA(cudaGetLastError());
   }
   if (advance) {
     adamw_advance_kernel<<<1, 1, 0, st>>>(plan->d_counter);
     ANC_CUDA(cudaGetLastError());
   }
+  return ANC_OK;
+}
+
+int anc_adamw_plan_set_grad_scale(anc_adamw_plan *plan, const float *scale) {
+  ANC_REQUIRE(plan, "plan is NULL");
+  ANC_REQUIRE(((uintptr_t)scale & 3) == 0, "scale not aligned to 4 bytes");
+  plan->grad_scale = scale;
   return ANC_OK;
 }
 

@@ -85,7 +85,7 @@ int anc_encode_tile_map(anc_tmap *out, const void *ptr, int elem_bytes, uint64_t
 // the entries with tr != 0, unused storage for the others.
 int anc_launch_momentum_group(anc_ctx *ctx, const void *d_table, const anc_tmap *d_maps, uint16_t *xbase,
                               int n_w, int elems_per_w, int grad_dtype, float momentum, int nesterov,
-                              float *partial, cudaStream_t st);
+                              float *partial, const float *grad_scale, cudaStream_t st);
 // partial: per matrix, per_matrix sums of squares (warp_sums == 0: fro_partial's blocks) or per_matrix
 // groups of eight warp sums (warp_sums != 0: the momentum kernel's 64x64 tiles).
 // sched (nullable): 2 + E scheduler words of the chain kernel, cleared here

@@ -276,10 +276,12 @@ __device__ __forceinline__ uint8_t *ring_base(uint8_t *raw) {
   return raw + ((128u - (anc_ring::smem_u32(raw) & 127u)) & 127u);   // box loads want 128-byte aligned stages
 }
 
-template <bool kGradF32, int kGroups>
+// kScaled: every gradient is first multiplied by *grad_scale (the clipping factor).
+template <bool kGradF32, int kGroups, bool kScaled>
 __global__ void __launch_bounds__(kGroups * kThreads + 32, 1)
 momentum_ring_kernel(const MomW *__restrict__ table, const anc_tmap *__restrict__ maps, uint16_t *xbase, int n_w,
-                     int tiles_per_w, float mu, int nesterov, float *__restrict__ partial, uint32_t *status) {
+                     int tiles_per_w, float mu, int nesterov, float *__restrict__ partial, uint32_t *status,
+                     const float *grad_scale) {
   using R = TileRing<kGradF32 ? 8 : 6>;
   constexpr uint32_t kGB = kGradF32 ? 4u : 2u;
   extern __shared__ __align__(128) uint8_t ring_raw[];
@@ -339,6 +341,8 @@ momentum_ring_kernel(const MomW *__restrict__ table, const anc_tmap *__restrict_
   uint16_t (*sm)[kTile + kPad] = sm2[grp];
   const int c8 = (tid & 7) * 8;
   const int r0 = tid >> 3;
+  float gscale = 1.f;
+  if constexpr (kScaled) gscale = *grad_scale;
   uint32_t it = grp;
   for (int b = blockIdx.x + grp * (int)gridDim.x; b < total; b += kGroups * (int)gridDim.x, it += kGroups) {
     const uint32_t slot = it % R::kStages, ph = (it / R::kStages) & 1u;
@@ -362,6 +366,10 @@ momentum_ring_kernel(const MomW *__restrict__ table, const anc_tmap *__restrict_
       else
         anc_ring::ld8_bf16(reinterpret_cast<const uint16_t *>(st + kRingHdr + kTileElems * 4) + k * (kThreads * 8),
                            tid, gg[k]);
+      if constexpr (kScaled) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) gg[k][j] = __fmul_rn(gg[k][j], gscale);
+      }
     }
     __syncwarp();
     if (lane == 0) anc_ring::mbar_arrive(empty0 + 8 * slot);
@@ -936,11 +944,16 @@ static cudaError_t ring_kernels_ready(int device) {
   static bool done[64] = {};
   std::lock_guard<std::mutex> lock(mu);
   if (device >= 0 && device < 64 && done[device]) return cudaSuccess;
-  cudaError_t e = cudaFuncSetAttribute(momentum_ring_kernel<true, kMomGroups>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       (int)TileRing<8>::kSmemBytes);
-  if (e == cudaSuccess)
-    e = cudaFuncSetAttribute(momentum_ring_kernel<false, kMomGroups>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             (int)TileRing<6>::kSmemBytes);
+  cudaError_t e = cudaSuccess;
+#define ANC_MOM_SMEM(F32, SC)                                                                            \
+  if (e == cudaSuccess)                                                                                  \
+  e = cudaFuncSetAttribute(momentum_ring_kernel<F32, kMomGroups, SC>, cudaFuncAttributeMaxDynamicSharedMemorySize, \
+                           (int)TileRing<(F32) ? 8 : 6>::kSmemBytes)
+  ANC_MOM_SMEM(true, false);
+  ANC_MOM_SMEM(true, true);
+  ANC_MOM_SMEM(false, false);
+  ANC_MOM_SMEM(false, true);
+#undef ANC_MOM_SMEM
   if (e == cudaSuccess)
     e = cudaFuncSetAttribute(update_ring_kernel<kUpdGroups>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                              (int)TileRing<6>::kSmemBytes);
@@ -975,20 +988,22 @@ int anc_launch_fro_partial(anc_ctx *ctx, const uint16_t *X, float *partial, int 
 
 int anc_launch_momentum_group(anc_ctx *ctx, const void *d_table, const anc_tmap *d_maps, uint16_t *xbase,
                               int n_w, int elems_per_w, int grad_dtype, float momentum, int nesterov,
-                              float *partial, cudaStream_t st) {
+                              float *partial, const float *grad_scale, cudaStream_t st) {
   const int tpw = elems_per_w / (kTile * kTile);
   const long long total = (long long)n_w * tpw;
   int grid = (int)(total < (long long)ctx->sm_count ? total : (long long)ctx->sm_count);   // one CTA per SM
   if (grid == 0) return ANC_OK;
   ANC_CUDA(ring_kernels_ready(ctx->device));
-  if (grad_dtype == ANC_GRAD_F32)
-    ANC_CUDA(launch_pdl_ex(momentum_ring_kernel<true, kMomGroups>, grid, kMomGroups * kThreads + 32, TileRing<8>::kSmemBytes, st,
-                           (const MomW *)d_table, d_maps, xbase, n_w, tpw, momentum, nesterov, partial,
-                           ctx->d_status));
-  else
-    ANC_CUDA(launch_pdl_ex(momentum_ring_kernel<false, kMomGroups>, grid, kMomGroups * kThreads + 32, TileRing<6>::kSmemBytes, st,
-                           (const MomW *)d_table, d_maps, xbase, n_w, tpw, momentum, nesterov, partial,
-                           ctx->d_status));
+#define ANC_MOM(F32, SC)                                                                               \
+  ANC_CUDA(launch_pdl_ex(momentum_ring_kernel<F32, kMomGroups, SC>, grid, kMomGroups * kThreads + 32,  \
+                         TileRing<(F32) ? 8 : 6>::kSmemBytes, st, (const MomW *)d_table, d_maps, xbase, \
+                         n_w, tpw, momentum, nesterov, partial, ctx->d_status, grad_scale))
+  const bool f32 = grad_dtype == ANC_GRAD_F32;
+  if (f32 && grad_scale) ANC_MOM(true, true);
+  else if (f32) ANC_MOM(true, false);
+  else if (grad_scale) ANC_MOM(false, true);
+  else ANC_MOM(false, false);
+#undef ANC_MOM
   return ANC_OK;
 }
 

@@ -45,6 +45,7 @@ struct anc_muon_plan {
   float *partial = nullptr;       // per-tile sums of squares written by the momentum kernel
   uint32_t *sched = nullptr;      // scheduler words of the chain kernel: 2 + largest batch
   uint64_t scratch_bytes = 0;
+  const float *grad_scale = nullptr;   // optional device-resident factor on every gradient
   bool timing = false;
   std::vector<TimedSpan> spans;
   double last_flops = 0.0;
@@ -291,7 +292,7 @@ int step_chunk(anc_muon_plan *pl, const ChunkRef &c, double lr, float momentum, 
   uint16_t *X = pl->X, *Y = pl->Y;
   begin_span(0);
   int rc = anc_launch_momentum_group(ctx, g.d_mom + c.w0, g.d_maps + 3 * (size_t)c.w0, X, E, epw, pl->grad_dtype,
-                                     momentum, nesterov, pl->partial, st);
+                                     momentum, nesterov, pl->partial, pl->grad_scale, st);
   end_span();
   if (rc) return rc;
   begin_span(1);
@@ -373,6 +374,13 @@ int anc_muon_step_range(anc_muon_plan *pl, int group, int first, int count, doub
   ChunkRef c = {group, first, count};
   return step_chunk(pl, c, lr, momentum, nesterov, ns_steps, coeffs, eps,
                     anc_pick_stream(pl->ctx, stream));
+}
+
+int anc_muon_plan_set_grad_scale(anc_muon_plan *pl, const float *scale) {
+  ANC_REQUIRE(pl, "plan is NULL");
+  ANC_REQUIRE(((uintptr_t)scale & 3) == 0, "scale not aligned to 4 bytes");
+  pl->grad_scale = scale;
+  return ANC_OK;
 }
 
 int anc_muon_plan_set_timing(anc_muon_plan *pl, int on) {

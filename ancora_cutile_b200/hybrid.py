@@ -11,6 +11,7 @@ Extra keyword arguments (all default to the reference's behaviour):
   rounding   "rne" | "sr"        AdamW bf16 copy: round-to-nearest-even or Philox SR
   seed                           SR stream seed
   rank, world, comm              ZeRO-1 sharding over one node's GPUs
+  max_grad_norm                  clip the gradients by their global norm inside the step (None: not)
 """
 import numpy as np
 
@@ -101,7 +102,8 @@ class HybridOptimizer:
 
     def __init__(self, params, is_muon=default_is_muon, no_decay=None, muon_kw=None, adamw_kw=None,
                  si=None, muon_device=False, grad_dtype="f32", rounding="rne", seed=0,
-                 rank=0, world=1, comm=None, schedule=None, max_batch=0, expert_muon=False, ctx=None):
+                 rank=0, world=1, comm=None, schedule=None, max_batch=0, expert_muon=False, ctx=None,
+                 max_grad_norm=None):
         muon_kw = dict(lr=0.02, momentum=0.95, ns_steps=5, **(muon_kw or {}))
         adamw_kw = adamw_kw or dict(lr=3e-4, betas=(0.9, 0.95), eps=1e-8, wd=0.01)
         if no_decay is None:
@@ -138,9 +140,23 @@ class HybridOptimizer:
             no_decay_names=tuple(n for n in self.adamw_names if no_decay(n, params[n])),
             adamw_kw=adamw_kw, muon_kw=muon_kw, grad_dtype=grad_dtype, rounding=rounding, seed=seed,
             rank=rank, world=world, comm=comm, schedule=_UNSET if schedule is None else schedule,
-            max_batch=max_batch, ctx=ctx)
+            max_batch=max_batch, ctx=ctx, max_grad_norm=max_grad_norm)
         self.muon = _Part(self, "muon", self.muon_names, self.engine.muon_kw)
         self.adamw = _Part(self, "adamw", self.adamw_names, self.engine.adamw_kw)
+
+    @property
+    def max_grad_norm(self):
+        """Largest global gradient norm the step lets through (None: no clipping); may be set between steps.
+        With it set, ``.muon.step`` / ``.adamw.step`` on their own are refused: the norm spans both."""
+        return self.engine.max_grad_norm
+
+    @max_grad_norm.setter
+    def max_grad_norm(self, v):
+        self.engine.max_grad_norm = v
+
+    def grad_norm(self):
+        """(norm, factor) of the last clipped step."""
+        return self.engine.grad_norm(self.si)
 
     # ---- expert stacks <-> the engine's per-matrix entries
     def _expand(self, grads, names=None):

@@ -74,6 +74,11 @@ class MuonPlan:
                                             float(momentum), int(bool(nesterov)), int(ns_steps), flat,
                                             float(eps), C.c_void_p(si or None)))
 
+    def set_grad_scale(self, scale):
+        """Every later step multiplies the gradients by the float32 at this device address as it loads them
+        (``GradClip.factor_ptr``); None: not."""
+        L.check(L.lib().anc_muon_plan_set_grad_scale(self.handle, dev_ptr(scale)))
+
     def set_timing(self, on):
         L.check(L.lib().anc_muon_plan_set_timing(self.handle, int(bool(on))))
 

@@ -27,6 +27,8 @@ from . import _lib as L
 from .adamw import ResidentAdamW
 from .bf16 import bits_to_f32, f32_to_bf16_bits
 from .buffers import DBuf, Event, PinnedArray, get_context
+from . import kernels
+from .grad_clip import GradClip
 from .muon import MuonPlan, _UNSET, _schedule
 from .layout import ArenaLayout
 
@@ -36,10 +38,14 @@ def _numel(shape):
 
 
 class ResidentHybrid:
+    _clip, _max_grad_norm, _embed_work = None, None, ()
+
     def __init__(self, params, muon_names, no_decay_names=(), adamw_kw=None, muon_kw=None,
                  grad_dtype="bf16", rounding="sr", seed=0, rank=0, world=1, comm=None,
-                 schedule=_UNSET, max_batch=0, ctx=None):
+                 schedule=_UNSET, max_batch=0, ctx=None, max_grad_norm=None):
         """params: {name: fp32 ndarray} (every rank passes the same dict).
+        max_grad_norm: the step multiplies the gradients by min(1, max_grad_norm / (norm + 1e-6)), norm over all
+        parameters of all ranks; None: not.  Also an attribute that may be set between steps.
         comm: zero1.Comm; the updated bf16 parameters are exchanged with one NCCL all-gather per
         unit, issued on a second stream as soon as the unit is computed (``nccl_overlap``; set it
         to False for plain all-gathers after the step)."""
@@ -135,6 +141,8 @@ class ResidentHybrid:
         self._pin_w = None
         self._streams = None
         self._comm_stream = None
+        self._embed_work = []                  # scratch of embedding_grad; the last is the largest
+        self.max_grad_norm = max_grad_norm
 
     # ---------------------------------------------------------------- locations
     def _loc(self, name):
@@ -176,6 +184,8 @@ class ResidentHybrid:
                 pl = ResidentAdamW(self._adamw_tensors, grad_dtype=self.grad_dtype, rounding=self.rounding,
                                    seed=self.seed, ctx=self.ctx)
                 pl.set_range(u[1], u[2])
+                if self._max_grad_norm is not None:
+                    pl.set_grad_scale(self._clip.factor_ptr)
                 self._sub_plans.append(pl)
                 units.append(("adamw", pl, u[1], u[2]))
         return units
@@ -187,6 +197,99 @@ class ResidentHybrid:
             return 0, unit[2], unit[3] - unit[2]
         g = self._gmap[unit[4]]
         return 1, g["base"] + self.rank * g["per"] + unit[5] * g["elems"], unit[3] * g["elems"]
+
+    # ---------------------------------------------------------------- gradient clipping
+    @property
+    def max_grad_norm(self):
+        return self._max_grad_norm
+
+    @max_grad_norm.setter
+    def max_grad_norm(self, v):
+        if v is not None:
+            v = float(v)
+            if not v >= 0.0:
+                raise ValueError(f"max_grad_norm must not be negative or NaN, got {v}")
+            if self.world > 1 and self.comm is None:
+                raise ValueError("max_grad_norm with world > 1 needs a communicator: the norm spans all ranks")
+            if self._clip is None:
+                self._clip = self._make_clip()
+        scale = None if v is None else self._clip.factor_ptr
+        for pl in [self.adamw] + self._sub_plans + ([self.muon] if self.muon is not None else []):
+            pl.set_grad_scale(scale)
+        self._max_grad_norm = v
+
+    def _make_clip(self):
+        """Norm plan over this rank's own gradients: its range of every AdamW tensor (the arena's gaps are not
+        anybody's) and its matrices of every group."""
+        it, ts = self._gdt.itemsize, []
+        for n in self.adamw_names:
+            s, e = self.owned_range(n)
+            if e > s:
+                ts.append(dict(g=self.a_g.ptr + (self.a_off[n] + s) * it, numel=e - s))
+        for g in self.groups:
+            k = len(g["names"][self.rank])
+            if k:
+                ts.append(dict(g=self.m_g.ptr + (g["base"] + self.rank * g["per"]) * it, numel=k * g["elems"]))
+        return GradClip(ts, grad_dtype=self.grad_dtype, ctx=self.ctx)
+
+    def _norm_grads(self, si):
+        """{norm, factor} of the gradients now in the arenas, left in device memory; the sweeps of the
+        step read the factor there."""
+        if self._max_grad_norm is None:
+            return
+        if self.world > 1:
+            self._clip.sumsq(si)
+            self.comm.allreduce_f64(self._clip.sumsq_ptr, 1, si)
+            self._clip.finish(self._max_grad_norm, stream=si)
+        else:
+            self._clip.norm(self._max_grad_norm, stream=si)
+
+    def grad_norm(self, si=None):
+        """(norm, factor) the last step with ``max_grad_norm`` set saw; waits for ``si``."""
+        if self._clip is None:
+            raise RuntimeError("max_grad_norm was never set")
+        return self._clip.read(si or self.ctx.stream)
+
+    # ---------------------------------------------------------------- embedding rows
+    def _table(self, name):
+        shape = self.shapes[name]
+        if len(shape) != 2:
+            raise ValueError(f"{name} is not a (rows, row length) table: {shape}")
+        return shape
+
+    def embedding_lookup(self, name, ids, out, T, scale=1.0, out_dtype="bf16", ids_dtype="i64", si=None):
+        """out[t] = round(scale * weight[ids[t]]) for T tokens: the bf16 rows of ``name`` the last step wrote
+        (``kernels.embedding_lookup``)."""
+        V, D = self._table(name)
+        kernels.embedding_lookup(self.p16_view(name), ids, out, T, V, D, scale=scale, out_dtype=out_dtype,
+                                 ids_dtype=ids_dtype, stream=si or self.ctx.stream, ctx=self.ctx)
+
+    def embedding_grad(self, name, dy, ids, T, scale=1.0, dy_dtype="bf16", ids_dtype="i64", mode="write",
+                       into="grad", padding_idx=None, si=None):
+        """The gradient of ``embedding_lookup`` (``kernels.embedding_grad``) into the gradient arena
+        (``into="grad"``) or, with mode "add", straight into the float32 accumulator (``into="acc"``, after
+        ``enable_grad_accumulation``).  ``mode="add"`` onto the gradient arena is for a tied table whose head
+        gradient is already there.  Calls on one engine share scratch and must be ordered; scratch grows
+        at the first call with more tokens, which must not be captured."""
+        V, D = self._table(name)
+        if into == "grad":
+            dw, dt = self.grad_view(name), self.grad_dtype
+        elif into == "acc":
+            if getattr(self, "acc_a", None) is None:
+                raise RuntimeError("enable_grad_accumulation first")
+            if mode != "add":
+                raise ValueError("the accumulator is only added to")
+            _, _, o = self._loc(name)
+            acc = self.acc_a if name in self.a_off else self.acc_m
+            dw, dt = acc.slice_elems(o, V * D, (V, D)), "f32"
+        else:
+            raise ValueError(f"into must be 'grad' or 'acc', got {into!r}")
+        need = kernels.embedding_grad_workspace(T, V, D)
+        if not self._embed_work or self._embed_work[-1].nbytes < need:
+            self._embed_work.append(DBuf.empty((need,), np.uint8, self.ctx))   # a captured graph may hold the old one
+        kernels.embedding_grad(dy, ids, dw, T, V, D, self._embed_work[-1], scale=scale, dy_dtype=dy_dtype,
+                               dw_dtype=dt, ids_dtype=ids_dtype, mode=mode, padding_idx=padding_idx,
+                               stream=si or self.ctx.stream, ctx=self.ctx)
 
     # ---------------------------------------------------------------- the step
     def _compute_unit(self, unit, si):
@@ -216,6 +319,7 @@ class ResidentHybrid:
         parameters are exchanged by NCCL all-gathers, one per arena group."""
         si = si or self.ctx.stream
         self.t += 1
+        self._norm_grads(si)
         multi = exchange and self.world > 1
         if multi and self.nccl_overlap:
             # NCCL all-gather of each unit on a second stream as soon as the unit is computed
@@ -251,6 +355,8 @@ class ResidentHybrid:
         units (kind "muon"), for callers that drive the two sub-optimizers separately as the
         reference's ``opt.muon.step`` / ``opt.adamw.step`` do (ancora/optim/hybrid.py:45-47)."""
         assert kind in ("adamw", "muon")
+        if self._max_grad_norm is not None:
+            raise RuntimeError("max_grad_norm clips by the norm of all gradients: call step, or set it to None")
         si = si or self.ctx.stream
         if kind == "adamw":
             self.t += 1
@@ -301,7 +407,6 @@ class ResidentHybrid:
     def accumulate_grads(self, si=None):
         """acc += the gradients now in the gradient arenas (one sweep per arena, all regions: a
         data-parallel replica holds local gradients for every parameter)."""
-        from . import kernels
         for acc, g, n in ((self.acc_a, self.a_g, self.a_padded), (self.acc_m, self.m_g, self.m_total)):
             kernels.grad_accumulate(acc, g, None, n, src_dtype="bf16", stream=si, ctx=self.ctx)
         self.acc_count += 1
@@ -313,7 +418,6 @@ class ResidentHybrid:
         ``scale`` defaults to 1 / (micro-batches * world).  Stochastic rounding draws from the
         producer's own Philox stream (seed + 1 of the step's by default, counter = position in the
         arena and the number of the step about to run), so it is reproducible for a fixed world size."""
-        from . import kernels
         self.accumulate_grads(si)
         multi = reduce and self.world > 1
         if multi:
@@ -350,9 +454,11 @@ class ResidentHybrid:
         self._graph_limit = self.t + horizon
         self._graph_next = self.t + 1
         self._graph_seed = self.seed
+        self._graph_max_norm = self._max_grad_norm
         lib = L.lib()
         L.check(lib.anc_graph_begin(self.ctx.handle, si))
         try:
+            self._norm_grads(si)
             for u in self.units:
                 if u[0] == "adamw":
                     u[1].step_scheduled(si, advance=True)
@@ -373,6 +479,8 @@ class ResidentHybrid:
         si = si or self.ctx.stream
         if self.seed != self._graph_seed:
             raise RuntimeError("the stochastic-rounding seed changed since capture_step: capture again")
+        if self._max_grad_norm != self._graph_max_norm:
+            raise RuntimeError("max_grad_norm changed since capture_step: capture again")
         if not (self._graph_first <= self.t + 1 <= self._graph_limit):
             raise RuntimeError(f"step {self.t + 1} lies outside the captured schedule "
                                f"[{self._graph_first}, {self._graph_limit}]: capture_step again")
@@ -537,6 +645,13 @@ class ResidentHybrid:
         h2d = d2h = 0
         gi = 0
         gspans = []
+        if self._max_grad_norm is not None:
+            # the norm needs every gradient: all uploads first, then compute and downloads unit by unit
+            for k, u in enumerate(units):
+                h2d += self._h2d_unit(u, s_in)
+            ev_in[nu - 1].record(s_in)
+            L.check(lib.anc_stream_wait_event(si, ev_in[nu - 1].handle))
+            self._norm_grads(si)
         for op, what in sched:
             if op == "gather":
                 ev = ev_g[gi]
@@ -552,9 +667,10 @@ class ResidentHybrid:
                     gspans.append((str(what), g0, g1))
                 continue
             k, u = what, units[what]
-            h2d += self._h2d_unit(u, s_in)
-            ev_in[k].record(s_in)
-            L.check(lib.anc_stream_wait_event(si, ev_in[k].handle))
+            if self._max_grad_norm is None:
+                h2d += self._h2d_unit(u, s_in)
+                ev_in[k].record(s_in)
+                L.check(lib.anc_stream_wait_event(si, ev_in[k].handle))
             self._compute_unit(u, si)
             ev_c[k].record(si)
             L.check(lib.anc_stream_wait_event(s_out, ev_c[k].handle))
@@ -670,6 +786,12 @@ class ResidentHybrid:
         for pl in self._sub_plans:
             pl.free()
         self._sub_plans = []
+        if self._clip is not None:
+            self._clip.free()
+            self._clip = None
+        for b in self._embed_work:
+            b.free()
+        self._embed_work = []
         if self.muon is not None:
             self.muon.free()
             self.muon = None

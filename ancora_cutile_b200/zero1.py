@@ -120,6 +120,10 @@ class Comm:
                                                       L.GRAD_BF16 if grad_dtype == "bf16" else L.GRAD_F32,
                                                       C.c_void_p(stream or None)))
 
+    def allreduce_f64(self, ptr, count, stream=None):
+        """In-place sum over the ranks of ``count`` float64 values."""
+        L.check(L.lib().anc_comm_allreduce_f64(self.handle, ptr, int(count), C.c_void_p(stream or None)))
+
     def barrier(self, stream=None):
         L.check(L.lib().anc_comm_barrier(self.handle, C.c_void_p(stream or None)))
 

@@ -166,6 +166,11 @@ ANC_API int anc_adamw_step_scheduled(anc_adamw_plan *plan, int rounding, uint64_
  * table, so a captured graph stays valid after eager steps or a restored state moved the
  * step number.  Synchronises `stream` first. */
 ANC_API int anc_adamw_plan_set_counter(anc_adamw_plan *plan, uint64_t step, void *stream);
+/* Gradients are multiplied by *scale (a float in device memory, read by every later launch of the plan; NULL:
+ * not multiplied) as the sweep loads them: where anc_grad_norm leaves its factor, clipping costs no sweep of its
+ * own.  One float32 product ahead of the arithmetic above; *scale must be written on the step's stream or
+ * before it. */
+ANC_API int anc_adamw_plan_set_grad_scale(anc_adamw_plan *plan, const float *scale);
 ANC_API int anc_adamw_plan_destroy(anc_adamw_plan *plan);
 
 /* ------------------------------------------------------------------- Muon ---- */
@@ -235,6 +240,8 @@ ANC_API int anc_muon_plan_group_info(anc_muon_plan *plan, int group, int32_t inf
 ANC_API int anc_muon_step_range(anc_muon_plan *plan, int group, int first, int count, double lr,
                                 float momentum, int nesterov, int ns_steps, const float *coeffs,
                                 float eps, void *stream);
+/* As anc_adamw_plan_set_grad_scale, for the momentum sweep. */
+ANC_API int anc_muon_plan_set_grad_scale(anc_muon_plan *plan, const float *scale);
 /* Per-phase device time accumulated over every anc_muon_step since the previous call
  * (timing enabled with anc_muon_plan_set_timing(plan, 1); CUDA events on the step's
  * stream, no synchronisation inside the step): ms spent in momentum, normalise,

@@ -130,3 +130,39 @@ def test_embedding_oracle_gradient_is_the_derivative_of_the_lookup():
     dw, count, _ = embed_ref.grad(c, ids, V, 0.5)
     assert list(count) == [1, 0, 3, 0, 0, 0, 1]
     assert abs((f(W + E) - f(W - E)) / 2 - float((dw * E).sum())) < 1e-12 * 100
+
+
+@pytest.mark.parametrize("family", ["dense", "moe"])
+@pytest.mark.parametrize("world", [1, 2, 4, 8])
+def test_ranks_norm_spans_cover_every_element_once(monkeypatch, world, family):
+    """What each rank's norm plan reads: over all ranks every parameter element exactly once, no arena gap."""
+    from types import SimpleNamespace
+
+    from ancora_cutile_b200 import resident, shapes as S
+    from ancora_cutile_b200.hybrid import muon_names_for
+    from ancora_cutile_b200.layout import ArenaLayout
+    shp = (S.qwen3_0_6b_shapes(n_layers=5, hidden=256, ffn=768, vocab=1001) if family == "dense" else
+           S.moe_family_shapes(n_layers=4, hidden=256, ffn=768, experts=3, expert_ffn=128, vocab=777))
+    shp["odd_norm"] = (13,)
+    monkeypatch.setattr(resident, "GradClip", lambda ts, **kw: ts)
+    a_base, m_base, it = 1 << 20, 1 << 40, 2
+    seen = {}
+    for rank in range(world):
+        lay = ArenaLayout(shp, muon_names_for(shp), rank, world)
+        eng = SimpleNamespace(_gdt=np.dtype(np.uint16), adamw_names=lay.adamw_names, owned_range=lay.owned_range,
+                              a_off=lay.a_off, a_g=SimpleNamespace(ptr=a_base), m_g=SimpleNamespace(ptr=m_base),
+                              groups=lay.groups, rank=rank, grad_dtype="bf16", ctx=None)
+        for t in resident.ResidentHybrid._make_clip(eng):
+            base = m_base if t["g"] >= m_base else a_base
+            lo = (t["g"] - base) // it
+            seen.setdefault(base, []).append((lo, lo + t["numel"]))
+    offs = {n: (a_base if n in lay.a_off else m_base, lay.a_off.get(n, lay.m_off.get(n, 0))) for n in shp}
+    for base in (a_base, m_base):
+        got = np.zeros(max(lay.a_padded, lay.m_total), np.int8)
+        for lo, hi in seen[base]:
+            got[lo:hi] += 1
+        want = np.zeros_like(got)
+        for n, (b, o) in offs.items():
+            if b == base:
+                want[o:o + int(np.prod(shp[n]))] += 1
+        assert np.array_equal(got, want)
