@@ -16,6 +16,7 @@
 #include <mutex>
 #include "anc_internal.h"
 #include "philox.cuh"
+#include "pred_load.cuh"
 
 namespace {
 
@@ -32,28 +33,6 @@ template <bool kF32, bool kVec>
 struct Row8 {
   uint32_t w[(kF32 || !kVec) ? 8 : 4];
 };
-
-// Predicated loads that leave the registers alone where `on` is false.  They are written as one instruction
-// because the value of an `if` is merged by a register move that waits for the load: a loop
-// that fetched ahead that way had a single load in flight per warp.
-__device__ __forceinline__ void ld_v4(uint32_t &a, uint32_t &b, uint32_t &c, uint32_t &d, const void *p, bool on) {
-  asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.u32 q, %5, 0;\n\t@q ld.global.v4.u32 {%0, %1, %2, %3}, [%4];\n\t}"
-               : "+r"(a), "+r"(b), "+r"(c), "+r"(d)
-               : "l"(p), "r"((uint32_t)on)
-               : "memory");
-}
-__device__ __forceinline__ void ld_1(uint32_t &a, const void *p, bool on) {
-  asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.u32 q, %2, 0;\n\t@q ld.global.u32 %0, [%1];\n\t}"
-               : "+r"(a)
-               : "l"(p), "r"((uint32_t)on)
-               : "memory");
-}
-__device__ __forceinline__ void ld_h(uint32_t &a, const void *p, bool on) {
-  asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.u32 q, %2, 0;\n\t@q ld.global.u16 %0, [%1];\n\t}"
-               : "+r"(a)
-               : "l"(p), "r"((uint32_t)on)
-               : "memory");
-}
 
 template <bool kF32, bool kVec>
 __device__ __forceinline__ void load_row(Row8<kF32, kVec> &r, const void *row, int c, int L, int D, bool on) {

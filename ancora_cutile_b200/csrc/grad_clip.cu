@@ -17,6 +17,11 @@
 // Order.  Thread sums, the shuffle tree, the warps of a block, the blocks: all in an order that depends on
 // the table and the number of SMs alone, never on timing.  The last block to finish (an integer ticket)
 // adds the block sums in index order, so one launch gives the norm.
+//
+// Launches.  The norm is one launch of resident blocks, each with an equal share of all vectors of all tensors.
+// Clipping reads the gradients twice (the factor is known only after all of them), in two launches; what
+// fits the registers of the resident blocks is read once, in one launch whose blocks wait for one
+// another between the two halves.
 #include <algorithm>
 #include <cuda_bf16.h>
 #include <math.h>
@@ -24,129 +29,106 @@
 #include <vector>
 #include "anc_internal.h"
 #include "philox.cuh"
+#include "pred_load.cuh"
 
 namespace {
 
 constexpr int kThreads = 256;
 constexpr int kVecPerThread = 4;                              // vectors of 8 elements a thread has in flight
-constexpr int kChunkVec = kThreads * kVecPerThread;           // vectors per chunk
+constexpr int kChunkVec = kThreads * kVecPerThread;           // vectors per chunk of the scaling sweep
 constexpr int kChunkElems = kChunkVec * 8;
-constexpr int kCtasPerSm = 8;
+constexpr uint32_t kWaitPolls = 1u << 22;                     // of the one-launch clip; about a second
 
-// One tensor.  Elements [head, head + 8 * nvec) are read as 16-byte aligned vectors, the up to 7 before
-// and after them one by one.  Without a common alignment of input and output nvec is 0 and all elements
-// go one by one.
+// One tensor.  The norm reads elements [head, head + 8 * nvec) as 16-byte aligned vectors and the up to 7 on
+// either side one by one.  The scaling sweep wants input and output aligned together: from shead on, snvec
+// vectors; without a common alignment snvec is 0 and all its elements go one by one.
 struct Entry {
   const void *g;
   void *out;
   uint64_t numel;
-  uint64_t chunk0;      // chunks of the tensors before this one
-  uint64_t nvec;
-  uint32_t head;
-  uint32_t _pad;
+  uint64_t vec0;        // vectors of the tensors before this one (a tensor counts one at least)
+  uint64_t nvec, snvec;
+  uint32_t chunk0;      // chunks of the tensors before this one
+  uint16_t head, shead;
 };
-static_assert(sizeof(Entry) == 48, "table entry");
+static_assert(sizeof(Entry) == 56, "table entry");
 
 template <bool kF32>
 __device__ __forceinline__ float load1(const void *p, uint64_t i) {
-  if constexpr (kF32) return __ldg((const float *)p + i);
-  else return __uint_as_float((uint32_t)__ldg((const uint16_t *)p + i) << 16);
+  if constexpr (kF32) return ((const float *)p)[i];
+  else return __uint_as_float((uint32_t)((const uint16_t *)p)[i] << 16);
 }
 
 // eight elements as they lie in memory
 template <bool kF32>
 struct Raw {
-  uint4 a, b;
-};
-template <>
-struct Raw<false> {
-  uint4 a;
+  uint32_t w[kF32 ? 8 : 4];
 };
 template <bool kF32>
-__device__ __forceinline__ Raw<kF32> load_raw(const void *p, uint64_t i) {
-  Raw<kF32> r;
-  if constexpr (kF32) {
-    r.a = __ldg(reinterpret_cast<const uint4 *>((const float *)p + i));
-    r.b = __ldg(reinterpret_cast<const uint4 *>((const float *)p + i) + 1);
-  } else {
-    r.a = __ldg(reinterpret_cast<const uint4 *>((const uint16_t *)p + i));
-  }
-  return r;
+__device__ __forceinline__ void load_raw(Raw<kF32> &r, const void *p, uint64_t i, bool on) {
+  const uint8_t *q = (const uint8_t *)p + i * (kF32 ? 4 : 2);
+  ld_v4(r.w[0], r.w[1], r.w[2], r.w[3], q, on);
+  if constexpr (kF32) ld_v4(r.w[4], r.w[5], r.w[6], r.w[7], q + 16, on);
 }
 template <bool kF32>
 __device__ __forceinline__ void widen(const Raw<kF32> &r, float x[8]) {
-  const uint32_t w[4] = {r.a.x, r.a.y, r.a.z, r.a.w};
   if constexpr (kF32) {
-    const uint32_t u[4] = {r.b.x, r.b.y, r.b.z, r.b.w};
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      x[k] = __uint_as_float(w[k]);
-      x[4 + k] = __uint_as_float(u[k]);
-    }
+    for (int k = 0; k < 8; ++k) x[k] = __uint_as_float(r.w[k]);
   } else {
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      x[2 * k] = __uint_as_float(w[k] << 16);
-      x[2 * k + 1] = __uint_as_float(w[k] & 0xFFFF0000u);
+      x[2 * k] = __uint_as_float(r.w[k] << 16);
+      x[2 * k + 1] = __uint_as_float(r.w[k] & 0xFFFF0000u);
     }
   }
 }
 
-__device__ __forceinline__ double sumsq8(const float x[8]) {
+template <bool kF32>
+__device__ __forceinline__ double sumsq8(const Raw<kF32> &r) {
+  float x[8];
+  widen<kF32>(r, x);
   float s = x[0] * x[0];
 #pragma unroll
   for (int k = 1; k < 8; ++k) s = fmaf(x[k], x[k], s);
   if (s >= 8.0779357e-28f && s <= 1.3292280e36f) return (double)s;     // 2^-90, 2^120
+  uint32_t any = 0;
+#pragma unroll
+  for (int k = 0; k < (kF32 ? 8 : 4); ++k) any |= r.w[k];
+  if (any == 0) return 0.0;            // rows of an embedding that no token named
   double d = 0.0;
 #pragma unroll
   for (int k = 0; k < 8; ++k) d = fma((double)x[k], (double)x[k], d);
   return d;
 }
 
-// index of the tensor that holds chunk c (the table is never empty and c is below the number of chunks)
-__device__ __forceinline__ uint32_t find_entry(const Entry *__restrict__ tab, uint32_t n, uint64_t c) {
-  uint32_t lo = 0, hi = n;
-  while (hi - lo > 1) {
-    const uint32_t mid = (lo + hi) >> 1;
-    if (tab[mid].chunk0 <= c) lo = mid;
-    else hi = mid;
+// Index of the tensor that holds place `c` of the space whose starts `start(i)` gives: every warp narrows the
+// table 32-fold per round, all lanes' loads at once.
+template <typename F>
+__device__ __forceinline__ uint32_t find_entry(uint32_t n, uint64_t c, F start) {
+  uint32_t lo = 0;
+  while (n > 1) {
+    const uint32_t step = (n + 31) / 32, i = (threadIdx.x & 31) * step;
+    const bool le = i < n && start(lo + i) <= c;
+    const uint32_t k = __popc(__ballot_sync(0xFFFFFFFFu, le)) - 1;      // starts ascend: the last that is <= c
+    lo += k * step;
+    n = n - k * step < step ? n - k * step : step;
   }
   return lo;
 }
 
+// the elements of a tensor outside its vectors: fewer than 8 on either side
 template <bool kF32>
-__device__ __forceinline__ double chunk_sumsq(const Entry &e, uint64_t local) {
+__device__ __forceinline__ double loose_sumsq(const Entry &e, uint32_t head, uint64_t nvec) {
   double acc = 0.0;
-  if (e.nvec) {
-    const uint64_t v0 = local * kChunkVec + threadIdx.x;
-    Raw<kF32> r[kVecPerThread];
-#pragma unroll
-    for (int k = 0; k < kVecPerThread; ++k)
-      if (v0 + (uint64_t)k * kThreads < e.nvec) r[k] = load_raw<kF32>(e.g, e.head + (v0 + (uint64_t)k * kThreads) * 8);
-#pragma unroll
-    for (int k = 0; k < kVecPerThread; ++k)
-      if (v0 + (uint64_t)k * kThreads < e.nvec) {
-        float x[8];
-        widen<kF32>(r[k], x);
-        acc += sumsq8(x);
-      }
-    if (local == 0) {      // the elements outside the vectors: fewer than 8 on either side
-      const uint64_t after = e.head + e.nvec * 8;
-      if (threadIdx.x < e.head) {
-        const double x = load1<kF32>(e.g, threadIdx.x);
-        acc = fma(x, x, acc);
-      }
-      if (after + threadIdx.x < e.numel) {
-        const double x = load1<kF32>(e.g, after + threadIdx.x);
-        acc = fma(x, x, acc);
-      }
-    }
-  } else {
-    const uint64_t end = e.numel < (local + 1) * kChunkElems ? e.numel : (local + 1) * kChunkElems;
-    for (uint64_t i = local * kChunkElems + threadIdx.x; i < end; i += kThreads) {
-      const double x = load1<kF32>(e.g, i);
-      acc = fma(x, x, acc);
-    }
+  const uint64_t after = head + nvec * 8;
+  if (threadIdx.x < head) {
+    const double x = load1<kF32>(e.g, threadIdx.x);
+    acc = fma(x, x, acc);
+  }
+  for (uint64_t i = after + threadIdx.x; i < e.numel; i += kThreads) {
+    const double x = load1<kF32>(e.g, i);
+    acc = fma(x, x, acc);
   }
   return acc;
 }
@@ -181,25 +163,15 @@ __device__ __forceinline__ void finish_norm(const NormOut &o, double sumsq) {
   o.result[1] = (float)((double)o.scale * c);
 }
 
-template <bool kF32>
-__global__ void __launch_bounds__(kThreads)
-grad_sumsq_kernel(const Entry *__restrict__ tab, uint32_t n_tab, uint64_t n_chunks, double *__restrict__ partial,
-                  uint32_t *ticket, NormOut o, int finish) {
-  // this block's chunks: a contiguous share, so that one search finds the first tensor
-  const uint64_t c0 = n_chunks * blockIdx.x / gridDim.x, c1 = n_chunks * (blockIdx.x + 1ull) / gridDim.x;
+__device__ __forceinline__ double sum_partials(const double *partial, uint32_t n) {
   double acc = 0.0;
-  if (c0 < c1) {
-    uint32_t ti = find_entry(tab, n_tab, c0);
-    Entry e = tab[ti];
-    uint64_t next = ti + 1 < n_tab ? tab[ti + 1].chunk0 : n_chunks;
-    for (uint64_t c = c0; c < c1; ++c) {
-      while (c >= next) {
-        e = tab[++ti];
-        next = ti + 1 < n_tab ? tab[ti + 1].chunk0 : n_chunks;
-      }
-      acc += chunk_sumsq<kF32>(e, c - e.chunk0);
-    }
-  }
+  for (uint32_t b = threadIdx.x; b < n; b += kThreads) acc += __ldcg(partial + b);
+  return block_sum(acc);
+}
+
+// the thread sums of all blocks into the norm, by the last block to get here
+__device__ __forceinline__ void reduce_blocks(double acc, double *partial, uint32_t *ticket, const NormOut &o,
+                                              int finish) {
   acc = block_sum(acc);
   __shared__ bool last;
   if (threadIdx.x == 0) {
@@ -210,14 +182,44 @@ grad_sumsq_kernel(const Entry *__restrict__ tab, uint32_t n_tab, uint64_t n_chun
   __syncthreads();
   if (!last) return;
   __threadfence();
-  acc = 0.0;
-  for (uint32_t b = threadIdx.x; b < gridDim.x; b += kThreads) acc += __ldcg(partial + b);
-  acc = block_sum(acc);
+  acc = sum_partials(partial, gridDim.x);
   if (threadIdx.x == 0) {
     *ticket = 0u;                        // ready for the next launch
     *o.sumsq = acc;
     if (finish) finish_norm(o, acc);
   }
+}
+
+// Bound by the read of the gradients; a block's share is contiguous, so one search finds its first tensor.
+template <bool kF32>
+__global__ void __launch_bounds__(kThreads)
+grad_sumsq_kernel(const Entry *__restrict__ tab, uint32_t n_tab, uint64_t n_vec, double *__restrict__ partial,
+                  uint32_t *ticket, NormOut o, int finish) {
+  const uint64_t v0 = n_vec * blockIdx.x / gridDim.x, v1 = n_vec * (blockIdx.x + 1ull) / gridDim.x;
+  double acc = 0.0;
+  if (v0 < v1) {
+    uint32_t ti = find_entry(n_tab, v0, [&](uint32_t i) { return tab[i].vec0; });
+    for (uint64_t v = v0; v < v1; ++ti) {
+      const Entry e = tab[ti];
+      const uint64_t end = e.vec0 + (e.nvec ? e.nvec : 1);
+      const uint64_t a = v - e.vec0, b = (end < v1 ? end : v1) - e.vec0;
+      if (a == 0) acc += loose_sumsq<kF32>(e, e.head, e.nvec);
+      if (e.nvec) {
+        for (uint64_t i0 = a + threadIdx.x; i0 < b; i0 += kChunkVec) {
+          Raw<kF32> r[kVecPerThread] = {};
+#pragma unroll
+          for (int k = 0; k < kVecPerThread; ++k) {
+            const uint64_t i = i0 + (uint64_t)k * kThreads;
+            load_raw<kF32>(r[k], e.g, e.head + i * 8, i < b);
+          }
+#pragma unroll
+          for (int k = 0; k < kVecPerThread; ++k) acc += sumsq8<kF32>(r[k]);
+        }
+      }
+      v = e.vec0 + b;
+    }
+  }
+  reduce_blocks(acc, partial, ticket, o, finish);
 }
 
 __global__ void grad_norm_finish_kernel(NormOut o) { finish_norm(o, *o.sumsq); }
@@ -228,61 +230,143 @@ __device__ __forceinline__ void store1(void *p, uint64_t i, float x) {
   else ((uint16_t *)p)[i] = (uint16_t)bf16_rne(x);
 }
 
+// One chunk of one tensor in registers, between its load and its scaled store.
 template <bool kF32, bool kOutF32>
-__global__ void __launch_bounds__(kThreads)
-grad_scale_kernel(const Entry *__restrict__ tab, uint32_t n_tab, uint64_t n_chunks, const float *__restrict__ result,
-                  int in_place) {
-  const float f = result[1];
-  if (in_place && f == 1.0f) return;     // every element would be written back as it is
-  const uint64_t c0 = n_chunks * blockIdx.x / gridDim.x, c1 = n_chunks * (blockIdx.x + 1ull) / gridDim.x;
-  if (c0 >= c1) return;
-  uint32_t ti = find_entry(tab, n_tab, c0);
-  Entry e = tab[ti];
-  uint64_t next = ti + 1 < n_tab ? tab[ti + 1].chunk0 : n_chunks;
-  for (uint64_t c = c0; c < c1; ++c) {
-    while (c >= next) {
-      e = tab[++ti];
-      next = ti + 1 < n_tab ? tab[ti + 1].chunk0 : n_chunks;
-    }
-    const uint64_t local = c - e.chunk0;
-    if (e.nvec) {
-      const uint64_t v0 = local * kChunkVec + threadIdx.x;
-      Raw<kF32> r[kVecPerThread];
+struct Chunk {
+  Entry e;
+  uint64_t local;        // chunk within the tensor
+  Raw<kF32> r[kVecPerThread];
+
+  __device__ __forceinline__ uint64_t vec(int k) const { return local * kChunkVec + threadIdx.x + (uint64_t)k * kThreads; }
+
+  __device__ __forceinline__ void load(const Entry *__restrict__ tab, uint32_t n_tab, uint32_t c) {
+    e = tab[find_entry(n_tab, c, [&](uint32_t i) { return (uint64_t)tab[i].chunk0; })];
+    local = c - e.chunk0;
 #pragma unroll
-      for (int k = 0; k < kVecPerThread; ++k)
-        if (v0 + (uint64_t)k * kThreads < e.nvec) r[k] = load_raw<kF32>(e.g, e.head + (v0 + (uint64_t)k * kThreads) * 8);
-#pragma unroll
-      for (int k = 0; k < kVecPerThread; ++k)
-        if (v0 + (uint64_t)k * kThreads < e.nvec) {
-          const uint64_t i = e.head + (v0 + (uint64_t)k * kThreads) * 8;
-          float x[8];
-          widen<kF32>(r[k], x);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) x[j] = __fmul_rn(x[j], f);
-          if constexpr (kOutF32) {
-            float4 *d = reinterpret_cast<float4 *>((float *)e.out + i);
-            d[0] = make_float4(x[0], x[1], x[2], x[3]);
-            d[1] = make_float4(x[4], x[5], x[6], x[7]);
-          } else {
-            uint32_t h[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) h[j] = bf16_rne(x[j]);
-            *reinterpret_cast<uint4 *>((uint16_t *)e.out + i) =
-                make_uint4(h[0] | (h[1] << 16), h[2] | (h[3] << 16), h[4] | (h[5] << 16), h[6] | (h[7] << 16));
-          }
-        }
-      if (local == 0) {
-        const uint64_t after = e.head + e.nvec * 8;
-        if (threadIdx.x < e.head) store1<kOutF32>(e.out, threadIdx.x, __fmul_rn(load1<kF32>(e.g, threadIdx.x), f));
-        if (after + threadIdx.x < e.numel)
-          store1<kOutF32>(e.out, after + threadIdx.x, __fmul_rn(load1<kF32>(e.g, after + threadIdx.x), f));
-      }
-    } else {
-      const uint64_t end = e.numel < (local + 1) * kChunkElems ? e.numel : (local + 1) * kChunkElems;
-      for (uint64_t i = local * kChunkElems + threadIdx.x; i < end; i += kThreads)
-        store1<kOutF32>(e.out, i, __fmul_rn(load1<kF32>(e.g, i), f));
+    for (int k = 0; k < kVecPerThread; ++k) {
+      r[k] = Raw<kF32>{};
+      load_raw<kF32>(r[k], e.g, e.shead + vec(k) * 8, vec(k) < e.snvec);
     }
   }
+  // elements that are not in vectors: the ends of the tensor, or all of the chunk
+  template <typename F>
+  __device__ __forceinline__ void loose(F f) const {
+    if (e.snvec == 0) {
+      const uint64_t end = e.numel < (local + 1) * kChunkElems ? e.numel : (local + 1) * kChunkElems;
+#pragma unroll 4
+      for (uint64_t i = local * kChunkElems + threadIdx.x; i < end; i += kThreads) f(i);
+    } else if (local == 0) {
+      const uint64_t after = e.shead + e.snvec * 8;
+      if (threadIdx.x < e.shead) f((uint64_t)threadIdx.x);
+      if (after + threadIdx.x < e.numel) f(after + threadIdx.x);
+    }
+  }
+  __device__ __forceinline__ double sumsq() const {
+    double acc = 0.0;
+#pragma unroll
+    for (int k = 0; k < kVecPerThread; ++k) acc += sumsq8<kF32>(r[k]);
+    loose([&](uint64_t i) {
+      const double x = load1<kF32>(e.g, i);
+      acc = fma(x, x, acc);
+    });
+    return acc;
+  }
+  __device__ __forceinline__ void store(float f) const {
+#pragma unroll
+    for (int k = 0; k < kVecPerThread; ++k) {
+      if (vec(k) >= e.snvec) break;
+      const uint64_t i = e.shead + vec(k) * 8;
+      float x[8];
+      widen<kF32>(r[k], x);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = __fmul_rn(x[j], f);
+      if constexpr (kOutF32) {
+        float4 *d = reinterpret_cast<float4 *>((float *)e.out + i);
+        d[0] = make_float4(x[0], x[1], x[2], x[3]);
+        d[1] = make_float4(x[4], x[5], x[6], x[7]);
+      } else {
+        uint32_t h[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) h[j] = bf16_rne(x[j]);
+        *reinterpret_cast<uint4 *>((uint16_t *)e.out + i) =
+            make_uint4(h[0] | (h[1] << 16), h[2] | (h[3] << 16), h[4] | (h[5] << 16), h[6] | (h[7] << 16));
+      }
+    }
+    loose([&](uint64_t i) { store1<kOutF32>(e.out, i, __fmul_rn(load1<kF32>(e.g, i), f)); });
+  }
+};
+
+// The norm of what fits a resident block per chunk: many small tensors are then read side by side, where an
+// equal share of all vectors walks through them one after another (25 tensors, 2.5 M elements: 6.4 against
+// 9.3 us).
+template <bool kF32>
+__global__ void __launch_bounds__(kThreads)
+grad_sumsq_chunk_kernel(const Entry *__restrict__ tab, uint32_t n_tab, double *partial, uint32_t *ticket, NormOut o,
+                        int finish) {
+  Chunk<kF32, false> ch;
+  ch.load(tab, n_tab, blockIdx.x);
+  reduce_blocks(ch.sumsq(), partial, ticket, o, finish);
+}
+
+// A block per chunk, not resident blocks with a loop: blocks that start in address order keep DRAM streaming
+// (1.19 GB of bf16 in and out: 346 us against 395-408 with 1184 resident blocks, 366 for a memcpy).
+template <bool kF32, bool kOutF32>
+__global__ void __launch_bounds__(kThreads)
+grad_scale_kernel(const Entry *__restrict__ tab, uint32_t n_tab, const float *__restrict__ result, int in_place) {
+  const float f = result[1];
+  if (in_place && f == 1.0f) return;     // every element would be written back as it is
+  Chunk<kF32, kOutF32> ch;
+  ch.load(tab, n_tab, blockIdx.x);
+  ch.store(f);
+}
+
+// Norm and scaling in one launch: a block per chunk, all resident at once (a cooperative launch), the
+// chunk in registers while the blocks wait for one another's sums.  The wait is bounded: when it runs out,
+// status bit 0x10 is set and nothing is written.
+template <bool kF32, bool kOutF32>
+__global__ void __launch_bounds__(kThreads)
+grad_clip_fused_kernel(const Entry *__restrict__ tab, uint32_t n_tab, double *partial, uint32_t *ticket, NormOut o,
+                       int in_place, uint32_t *status) {
+  Chunk<kF32, kOutF32> ch;
+  ch.load(tab, n_tab, blockIdx.x);
+  double acc = block_sum(ch.sumsq());
+  __shared__ bool ok;
+  if (threadIdx.x == 0) {
+    partial[blockIdx.x] = acc;
+    __threadfence();
+    atomicAdd(ticket, 1u);
+    ok = false;
+    for (uint32_t i = 0; i < kWaitPolls && !ok; ++i) {
+      uint32_t seen;
+      asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(seen) : "l"(ticket) : "memory");
+      ok = seen >= gridDim.x;
+    }
+    // the last block to leave makes the counters ready for the next launch
+    if (atomicAdd(ticket + 1, 1u) == gridDim.x - 1) {
+      ticket[0] = 0u;
+      ticket[1] = 0u;
+    }
+    if (!ok) atomicOr(status, ANC_DEV_TIMEOUT_DEP);
+  }
+  __syncthreads();
+  if (!ok) return;
+  acc = sum_partials(partial, gridDim.x);
+  __shared__ float s_f;
+  if (threadIdx.x == 0) {
+    float res[2];
+    NormOut mine = o;
+    mine.result = res;
+    finish_norm(mine, acc);
+    s_f = res[1];
+    if (blockIdx.x == 0) {
+      *o.sumsq = acc;
+      o.result[0] = res[0];
+      o.result[1] = res[1];
+    }
+  }
+  __syncthreads();
+  if (in_place && s_f == 1.0f) return;
+  ch.store(s_f);
 }
 
 }  // namespace
@@ -291,8 +375,9 @@ struct anc_clip_plan {
   anc_ctx *ctx;
   int grad_f32, out_f32, in_place;
   uint32_t n_tab;
-  uint64_t n_chunks;
-  uint32_t grid;
+  uint64_t n_vec, n_chunks;
+  uint32_t grid;             // blocks of the norm
+  int fused;                 // all chunks resident at once: one launch clips
   uint8_t *d_mem;            // one allocation: table, block sums, sum of squares, ticket, result
   Entry *d_tab;
   double *d_partial, *d_sumsq;
@@ -322,25 +407,38 @@ int check_scalars(float scale, float max_norm, float eps) {
 }
 
 int launch_sumsq(const anc_clip_plan *pl, const NormOut &o, int finish, cudaStream_t st) {
-  if (pl->grad_f32)
-    grad_sumsq_kernel<true><<<pl->grid, kThreads, 0, st>>>(pl->d_tab, pl->n_tab, pl->n_chunks, pl->d_partial,
+  if (pl->fused) {
+    if (pl->grad_f32)
+      grad_sumsq_chunk_kernel<true><<<(unsigned)pl->n_chunks, kThreads, 0, st>>>(pl->d_tab, pl->n_tab, pl->d_partial,
+                                                                                 pl->d_ticket, o, finish);
+    else
+      grad_sumsq_chunk_kernel<false><<<(unsigned)pl->n_chunks, kThreads, 0, st>>>(pl->d_tab, pl->n_tab, pl->d_partial,
+                                                                                  pl->d_ticket, o, finish);
+  } else if (pl->grad_f32)
+    grad_sumsq_kernel<true><<<pl->grid, kThreads, 0, st>>>(pl->d_tab, pl->n_tab, pl->n_vec, pl->d_partial,
                                                            pl->d_ticket, o, finish);
   else
-    grad_sumsq_kernel<false><<<pl->grid, kThreads, 0, st>>>(pl->d_tab, pl->n_tab, pl->n_chunks, pl->d_partial,
+    grad_sumsq_kernel<false><<<pl->grid, kThreads, 0, st>>>(pl->d_tab, pl->n_tab, pl->n_vec, pl->d_partial,
                                                             pl->d_ticket, o, finish);
   ANC_CUDA(cudaGetLastError());
   return ANC_OK;
 }
 
+using ScaleKernel = void (*)(const Entry *, uint32_t, const float *, int);
+using FusedKernel = void (*)(const Entry *, uint32_t, double *, uint32_t *, NormOut, int, uint32_t *);
+
+ScaleKernel scale_kernel(const anc_clip_plan *pl) {
+  if (pl->grad_f32) return pl->out_f32 ? grad_scale_kernel<true, true> : grad_scale_kernel<true, false>;
+  return pl->out_f32 ? grad_scale_kernel<false, true> : grad_scale_kernel<false, false>;
+}
+FusedKernel fused_kernel(const anc_clip_plan *pl) {
+  if (pl->grad_f32) return pl->out_f32 ? grad_clip_fused_kernel<true, true> : grad_clip_fused_kernel<true, false>;
+  return pl->out_f32 ? grad_clip_fused_kernel<false, true> : grad_clip_fused_kernel<false, false>;
+}
+
 int launch_scale(const anc_clip_plan *pl, cudaStream_t st) {
   if (pl->n_chunks == 0) return ANC_OK;
-#define ANC_SCALE(F, O) \
-  grad_scale_kernel<F, O><<<pl->grid, kThreads, 0, st>>>(pl->d_tab, pl->n_tab, pl->n_chunks, pl->d_result, pl->in_place)
-  if (pl->grad_f32 && pl->out_f32) ANC_SCALE(true, true);
-  else if (pl->grad_f32) ANC_SCALE(true, false);
-  else if (pl->out_f32) ANC_SCALE(false, true);
-  else ANC_SCALE(false, false);
-#undef ANC_SCALE
+  scale_kernel(pl)<<<(unsigned)pl->n_chunks, kThreads, 0, st>>>(pl->d_tab, pl->n_tab, pl->d_result, pl->in_place);
   ANC_CUDA(cudaGetLastError());
   return ANC_OK;
 }
@@ -359,7 +457,7 @@ int anc_clip_plan_create(anc_ctx *ctx, const anc_clip_tensor *tensors, int n_ten
   *out = nullptr;
   const uint64_t gs = grad_dtype == ANC_GRAD_F32 ? 4 : 2, os = out_dtype == ANC_GRAD_F32 ? 4 : 2;
   bool all_in_place = true;
-  uint64_t chunks = 0;
+  uint64_t chunks = 0, vecs = 0;
   std::vector<Entry> tab;
   std::vector<Span> spans;
   try {
@@ -377,22 +475,27 @@ int anc_clip_plan_create(anc_ctx *ctx, const anc_clip_tensor *tensors, int n_ten
       e.out = t.out ? t.out : const_cast<void *>(t.g);
       all_in_place = all_in_place && e.out == e.g;
       e.numel = t.numel;
-      e.chunk0 = chunks;
-      e.head = 0;
-      e.nvec = 0;
-      e._pad = 0;
+      e.vec0 = vecs;
+      e.chunk0 = (uint32_t)chunks;
+      e.head = (uint16_t)(((16 - ((uintptr_t)e.g & 15)) & 15) / gs);
+      e.nvec = t.numel >= e.head + 8u ? (t.numel - e.head) / 8 : 0;
+      if (!e.nvec) e.head = 0;
+      e.shead = 0;
+      e.snvec = 0;
       for (uint32_t h = 0; h < 8; ++h) {
         if ((((uintptr_t)e.g + h * gs) & 15) || (((uintptr_t)e.out + h * os) & 15)) continue;
         if (t.numel >= h + 8) {
-          e.head = h;
-          e.nvec = (t.numel - h) / 8;
+          e.shead = (uint16_t)h;
+          e.snvec = (t.numel - h) / 8;
         }
         break;
       }
       // what a call reads and writes: outputs lie over nothing else of the call
       spans.push_back({(uintptr_t)e.g, (uintptr_t)e.g + t.numel * gs, e.out == e.g});
       if (e.out != e.g) spans.push_back({(uintptr_t)e.out, (uintptr_t)e.out + t.numel * os, true});
-      chunks += e.nvec ? (e.nvec + kChunkVec - 1) / kChunkVec : (t.numel + kChunkElems - 1) / kChunkElems;
+      vecs += e.nvec ? e.nvec : 1;
+      chunks += e.snvec ? (e.snvec + kChunkVec - 1) / kChunkVec : (t.numel + kChunkElems - 1) / kChunkElems;
+      ANC_REQUIRE(chunks <= 0x7FFFFFFF, "tensors too large for one plan");
       tab.push_back(e);
     }
     std::sort(spans.begin(), spans.end(), [](const Span &a, const Span &b) { return a.lo < b.lo; });
@@ -420,11 +523,25 @@ int anc_clip_plan_create(anc_ctx *ctx, const anc_clip_tensor *tensors, int n_ten
   pl->in_place = all_in_place ? 1 : 0;
   pl->n_tab = (uint32_t)tab.size();
   pl->n_chunks = chunks;
-  const uint64_t cap = (uint64_t)ctx->sm_count * kCtasPerSm;
-  pl->grid = (uint32_t)(chunks < cap ? (chunks ? chunks : 1) : cap);
+  pl->n_vec = vecs;
+  // the norm's blocks: as many as are resident at once, each with four vectors per thread at least
+  int norm_per_sm = 0, fused_per_sm = 0;
+  cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(
+      &norm_per_sm, pl->grad_f32 ? grad_sumsq_kernel<true> : grad_sumsq_kernel<false>, kThreads, 0);
+  if (e == cudaSuccess)
+    e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&fused_per_sm, fused_kernel(pl), kThreads, 0);
+  if (e != cudaSuccess) {
+    delete pl;
+    return anc_cuda_fail(e, "clip kernel occupancy");
+  }
+  const uint64_t cap = (uint64_t)ctx->sm_count * (norm_per_sm > 0 ? norm_per_sm : 1);
+  const uint64_t want = (vecs + kChunkVec - 1) / kChunkVec;
+  pl->grid = (uint32_t)(want < cap ? (want ? want : 1) : cap);
+  pl->fused = chunks > 0 && chunks <= (uint64_t)fused_per_sm * ctx->sm_count;
+  const uint64_t n_part = pl->fused && chunks > pl->grid ? chunks : pl->grid;
   const size_t tab_bytes = (tab.size() * sizeof(Entry) + 255) / 256 * 256;
-  const size_t part_bytes = ((size_t)pl->grid * sizeof(double) + 255) / 256 * 256;
-  cudaError_t e = cudaMalloc((void **)&pl->d_mem, tab_bytes + part_bytes + 256);
+  const size_t part_bytes = ((size_t)n_part * sizeof(double) + 255) / 256 * 256;
+  e = cudaMalloc((void **)&pl->d_mem, tab_bytes + part_bytes + 256);
   if (e == cudaSuccess && !tab.empty())
     e = cudaMemcpy(pl->d_mem, tab.data(), tab.size() * sizeof(Entry), cudaMemcpyHostToDevice);
   if (e == cudaSuccess) e = cudaMemset(pl->d_mem + tab_bytes + part_bytes, 0, 256);
@@ -481,8 +598,28 @@ int anc_grad_apply(anc_clip_plan *plan, void *stream) {
 }
 
 int anc_grad_clip(anc_clip_plan *plan, float scale, float max_norm, float eps, void *stream) {
-  int rc = anc_grad_norm(plan, scale, max_norm, eps, stream);
-  return rc ? rc : anc_grad_apply(plan, stream);
+  ANC_REQUIRE(plan, "plan is NULL");
+  int rc = check_scalars(scale, max_norm, eps);
+  if (rc) return rc;
+  anc_device_guard guard(plan->ctx->device);
+  cudaStream_t st = anc_pick_stream(plan->ctx, stream);
+  const NormOut o = norm_out(plan, scale, max_norm, eps);
+  if (!plan->fused) {
+    rc = launch_sumsq(plan, o, 1, st);
+    return rc ? rc : launch_scale(plan, st);
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)plan->n_chunks);
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeCooperative;
+  at[0].val.cooperative = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  ANC_CUDA(cudaLaunchKernelEx(&cfg, fused_kernel(plan), (const Entry *)plan->d_tab, plan->n_tab, plan->d_partial,
+                              plan->d_ticket, o, plan->in_place, plan->ctx->d_status));
+  return ANC_OK;
 }
 
 int anc_clip_plan_destroy(anc_clip_plan *plan) {
