@@ -163,20 +163,19 @@ embedding_lookup_kernel(const void *__restrict__ table, int64_t table_ld, const 
 }
 
 // ------------------------------------------------------------------ sort
-// Stable least-significant-digit radix sort of (id, token) by one cluster of CTAs, nine bits a pass: two
-// passes for tables of up to 2^18 rows.  Per pass every warp counts the digits of its stretch of the list,
+// Stable least-significant-digit radix sort of (id, token) by one cluster of CTAs, up to nine bits a pass:
+// two passes for tables of up to 2^18 rows.  Per pass every warp counts the digits of its stretch of the list,
 // the cluster exchanges its CTAs' digit counts through distributed shared memory, and every warp then
-// writes its stretch in order to the places the counts give.  Padding sorts behind the last row of
-// the table as id V.  The passes are bound by latency, not by bytes: loads go out eight rounds at a time,
-// and the lanes of equal digit find each other by nine ballots (the match instruction took 2000 cycles a
-// round with 32 warps at it, the ballots take about 200).
+// writes its stretch to the places the counts give.  Padding sorts behind the last row of the table as id V.
+// The passes are bound by latency, not by bytes: hence many CTAs with short stretches, all loads of a stretch
+// before their first use, and the ranks of a stretch of up to eight rounds kept in registers from the
+// counting to the writing.  (Lanes of equal digit: a word per digit in shared memory; a round took SORTNOTE.)
 constexpr int kDigitBits = 9;
 constexpr int kDigits = 1 << kDigitBits;
-constexpr int kSortThreads = 1024;
+constexpr int kSortThreads = kDigits;              // a thread per digit
 constexpr int kSortWarps = kSortThreads / 32;
 constexpr int kSortRounds = 8;
-constexpr size_t kSortSmem = (size_t)(kSortWarps * kDigits + 2 * kDigits + 64) * 4;
-constexpr int kMaxCluster = 8;
+constexpr uint32_t kMaxCluster = 16;
 
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -186,9 +185,12 @@ __device__ __forceinline__ uint32_t peer_smem(uint32_t addr, uint32_t rank) {
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(addr), "r"(rank));
   return a;
 }
-__device__ __forceinline__ uint32_t ld_cluster(uint32_t addr) {
-  uint32_t v;
-  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+__device__ __forceinline__ uint4 ld_cluster(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(addr)
+               : "memory");
   return v;
 }
 __device__ __forceinline__ void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
@@ -197,183 +199,252 @@ __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;"
 struct SortArgs {
   const void *ids;
   int ids64;
-  int64_t T, V, padding_idx;
+  uint32_t T;
+  int64_t V, padding_idx;
   uint2 *list[2];                // (id, token)
   int passes;
+  uint32_t *clear;               // words to clear: flags of the reduction, then the bitmap of named rows
+  uint32_t n_clear;
+  uint32_t *named;               // bitmap of the rows some token names (nullptr: not wanted)
   uint32_t *status;
-};
-
-struct ZeroArgs {
-  uint8_t *dw;
-  int64_t row_bytes, pitch, V;
-  int vec;
 };
 
 __device__ __forceinline__ uint32_t key_of(int64_t id, int64_t V, int64_t padding_idx) {
   return (id < 0 || id >= V || id == padding_idx) ? (uint32_t)V : (uint32_t)id;
 }
 
-// Zeros for the rows no token names.  Launched behind the sort without waiting for it, so it fills the SMs the
-// sort leaves idle; it waits for the sort only before it ends, so that whoever waits for this
-// kernel has the sorted list too.  By `n` threads of which this is number `i0`
-__device__ __forceinline__ void zero_rows(const ZeroArgs &z, int64_t i0, int64_t n) {
-  if (z.vec) {
-    const int64_t per = z.row_bytes / 16, total = per * z.V;
-    if (z.pitch == z.row_bytes) {
-      for (int64_t i = i0; i < total; i += n) reinterpret_cast<uint4 *>(z.dw)[i] = make_uint4(0u, 0u, 0u, 0u);
-    } else {
-      for (int64_t i = i0; i < total; i += n)
-        *reinterpret_cast<uint4 *>(z.dw + (i / per) * z.pitch + (i % per) * 16) = make_uint4(0u, 0u, 0u, 0u);
-    }
-  } else {
-    const int64_t per = z.row_bytes / 2, total = per * z.V;
-    for (int64_t i = i0; i < total; i += n)
-      *reinterpret_cast<uint16_t *>(z.dw + (i / per) * z.pitch + (i % per) * 2) = 0;
-  }
-}
-
-__global__ void __launch_bounds__(256)
-embedding_zero_kernel(ZeroArgs z) {
-  pdl_trigger();
-  zero_rows(z, (int64_t)blockIdx.x * 256 + threadIdx.x, (int64_t)gridDim.x * 256);
-  pdl_wait();
-}
+struct SortShared {
+  uint32_t cnt[kSortWarps][kDigits];     // per warp: counts, then places of the warp's first keys
+  uint32_t lanes[kSortWarps][kDigits];   // per warp: the lanes that hold a digit, one round at a time
+  uint32_t tot[kDigits];                 // this CTA's digit counts, read by the whole cluster
+  uint32_t off[kDigits];                 // first place of a digit's keys of this CTA
+  uint32_t share[2][4][kDigits];         // counts of a quarter of the cluster: all, and those before this CTA
+  uint32_t wsum[kSortWarps];
+  uint2 list[kSortThreads * kSortRounds];   // the list between passes when one CTA sorts
+};
 
 __global__ void __launch_bounds__(kSortThreads, 1)
 embedding_sort_kernel(SortArgs a, uint32_t n_ctas) {
-  extern __shared__ uint32_t sm[];
+  extern __shared__ __align__(16) uint8_t sort_smem[];
+  SortShared &sh = *reinterpret_cast<SortShared *>(sort_smem);
   pdl_trigger();
-  const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const uint32_t rank = blockIdx.x;
-  uint32_t *cnt = sm;                                // [warp][digit]
-  uint32_t *tot = sm + kSortWarps * kDigits;         // this CTA's digit counts, read by the whole cluster
-  uint32_t *off = tot + kDigits;                     // first place of a digit's keys of this CTA
-  uint32_t *wsum = off + kDigits;
-  // stretches: at least eight rounds of 32 keys per warp, so that few keys keep few warps busy
-  int64_t per = ((a.T + (int64_t)n_ctas * kSortThreads - 1) / ((int64_t)n_ctas * kSortThreads)) * 32;
-  if (per < 32 * kSortRounds) per = 32 * kSortRounds;
-  const int64_t lo = ((int64_t)rank * kSortWarps + warp) * per;
-  const int64_t hi = lo + per < a.T ? lo + per : a.T;
-  const int64_t cta_keys = a.T - (int64_t)rank * kSortWarps * per;
-  const int n_warps = cta_keys <= 0 ? 0 : cta_keys >= kSortWarps * per ? kSortWarps : (int)((cta_keys + per - 1) / per);
-  uint32_t *mine = cnt + warp * kDigits;
+  const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, rank = blockIdx.x;
+  for (uint32_t i = rank * kSortThreads + tid; i < a.n_clear; i += n_ctas * kSortThreads) a.clear[i] = 0u;
+  // every warp's stretch: the same number of whole rounds of 32 keys
+  const uint32_t rounds = (a.T + n_ctas * kSortThreads - 1) / (n_ctas * kSortThreads);
+  const uint64_t lo64 = (uint64_t)(rank * kSortWarps + warp) * rounds * 32;
+  const uint32_t lo = lo64 < a.T ? (uint32_t)lo64 : a.T;
+  const uint32_t hi = a.T - lo < rounds * 32 ? a.T : lo + rounds * 32;
+  const bool short_stretch = rounds <= kSortRounds;
+  const bool single = n_ctas == 1 && short_stretch;      // the list stays in shared memory between passes
+  uint32_t *mine = sh.cnt[warp], *lanes = sh.lanes[warp];
   // kSortRounds rounds of the list, all loads before the first use (places past the end repeat the last one);
   // the first pass reads the ids.  Returns whether one of this lane's ids lies outside the table.
-  auto fetch = [&](uint2 (&e)[kSortRounds], const uint2 *in, bool first, int64_t i0) {
+  auto fetch = [&](uint2 (&e)[kSortRounds], const uint2 *in, bool first, uint32_t i0) {
     bool bad = false;
     if (first) {
       int64_t id[kSortRounds];
 #pragma unroll
       for (int r = 0; r < kSortRounds; ++r) {
-        const int64_t i = i0 + r * 32 + lane;
+        const uint32_t i = i0 + r * 32 + lane;
         id[r] = load_id(a.ids, a.ids64, i < a.T ? i : a.T - 1);
       }
 #pragma unroll
       for (int r = 0; r < kSortRounds; ++r) {
-        const int64_t i = i0 + r * 32 + lane;
-        e[r] = make_uint2(key_of(id[r], a.V, a.padding_idx), (uint32_t)i);
+        e[r] = make_uint2(key_of(id[r], a.V, a.padding_idx), i0 + r * 32 + lane);
         bad = bad || id[r] >= a.V;
       }
     } else {
 #pragma unroll
       for (int r = 0; r < kSortRounds; ++r) {
-        const int64_t i = i0 + r * 32 + lane;
-        e[r] = __ldcg(in + (i < a.T ? i : a.T - 1));
+        const uint32_t i = i0 + r * 32 + lane;
+        const uint32_t j = i < a.T ? i : a.T - 1;
+        if (single) e[r] = sh.list[j < kSortThreads * kSortRounds ? j : 0];
+        else e[r] = __ldcg(in + j);
       }
     }
     return bad;
   };
+  // Places of this lane's keys among the warp's keys of the same digit so far.  The lanes of equal digit find
+  // each other by setting their bits in a word per digit.
+  auto rank_in = [&](uint32_t (&place)[kSortRounds], const uint2 (&e)[kSortRounds], int shift, uint32_t i0) {
+#pragma unroll
+    for (int r = 0; r < kSortRounds; ++r) {
+      if (i0 + r * 32 >= hi) break;
+      const bool on = i0 + r * 32 + lane < hi;
+      const uint32_t d = (e[r].x >> shift) & (kDigits - 1);
+      if (on) atomicOr(lanes + d, 1u << lane);
+      __syncwarp();
+      const uint32_t peers = lanes[d], at = mine[d];
+      __syncwarp();
+      if (on && lane == (uint32_t)(__ffs(peers) - 1)) {
+        mine[d] = at + __popc(peers);
+        lanes[d] = 0u;
+      }
+      __syncwarp();
+      place[r] = at + __popc(peers & ((1u << lane) - 1u));
+    }
+  };
+  for (uint32_t d = lane * 4; d < kDigits; d += 128) *reinterpret_cast<uint4 *>(lanes + d) = make_uint4(0u, 0u, 0u, 0u);
   for (int p = 0; p < a.passes; ++p) {
-    const bool odd = p & 1;
+    const bool odd = p & 1, last = p + 1 == a.passes;
     const uint2 *in = odd ? a.list[0] : a.list[1];
     uint2 *out = odd ? a.list[1] : a.list[0];
     const int shift = p * kDigitBits;
+    auto put = [&](uint32_t dst, uint2 e, bool on) {
+      if (on) {
+        if (single && !last) sh.list[dst] = e;
+        else out[dst] = e;
+      }
+      if (last && a.named) {
+        const uint32_t before = __shfl_up_sync(0xFFFFFFFFu, e.x, 1);
+        if (on && e.x < (uint32_t)a.V && (lane == 0 || before != e.x))
+          atomicOr(a.named + (e.x >> 5), 1u << (e.x & 31));
+      }
+    };
     for (uint32_t d = lane * 4; d < kDigits; d += 128) *reinterpret_cast<uint4 *>(mine + d) = make_uint4(0u, 0u, 0u, 0u);
     __syncwarp();
-    for (int64_t i0 = lo; i0 < hi; i0 += 32 * kSortRounds) {
-      uint2 e[kSortRounds];
-      const bool bad = fetch(e, in, p == 0, i0);
-      if (bad) atomicOr(a.status, ANC_DEV_BAD_INDEX);
+    uint2 e[kSortRounds];
+    uint32_t place[kSortRounds];
+    for (uint32_t i0 = lo; i0 < hi; i0 += 32 * kSortRounds) {
+      if (fetch(e, in, p == 0, i0)) atomicOr(a.status, ANC_DEV_BAD_INDEX);
+      if (short_stretch) {
+        rank_in(place, e, shift, i0);
+      } else {
 #pragma unroll
-      for (int r = 0; r < kSortRounds; ++r)
-        if (i0 + r * 32 + lane < hi) atomicAdd(mine + ((e[r].x >> shift) & (kDigits - 1)), 1u);
+        for (int r = 0; r < kSortRounds; ++r)
+          if (i0 + r * 32 + lane < hi) atomicAdd(mine + ((e[r].x >> shift) & (kDigits - 1)), 1u);
+      }
     }
     __syncthreads();
-    if (tid < kDigits) {
-      uint32_t run = 0;
-      for (int w0 = 0; w0 < n_warps; w0 += 8) {
-        uint32_t c[8];
+    uint32_t all = 0, before = 0, run = 0, c[kSortWarps];
 #pragma unroll
-        for (int w = 0; w < 8; ++w) c[w] = cnt[(w0 + w) * kDigits + tid];
+    for (int w = 0; w < kSortWarps; ++w) c[w] = sh.cnt[w][tid];
 #pragma unroll
-        for (int w = 0; w < 8; ++w) {
-          cnt[(w0 + w) * kDigits + tid] = run;
-          run += c[w];
+    for (int w = 0; w < kSortWarps; ++w) {
+      sh.cnt[w][tid] = run;
+      run += c[w];
+    }
+    sh.tot[tid] = run;
+    if (single) __syncthreads();
+    else cluster_sync();
+    {
+      // a quarter of the threads per quarter of the cluster, four digits each
+      const uint32_t quad = tid & 127, quarter = tid >> 7;
+      const uint32_t slot = (uint32_t)__cvta_generic_to_shared(sh.tot + quad * 4);
+      uint4 v[kMaxCluster / 4];
+#pragma unroll
+      for (uint32_t j = 0; j < kMaxCluster / 4; ++j) {
+        const uint32_t q = j * 4 + quarter;
+        v[j] = ld_cluster(peer_smem(slot, q < n_ctas ? q : rank));
+      }
+      uint4 sum_all = make_uint4(0u, 0u, 0u, 0u), sum_before = sum_all;
+#pragma unroll
+      for (uint32_t j = 0; j < kMaxCluster / 4; ++j) {
+        const uint32_t q = j * 4 + quarter, in_all = q < n_ctas ? 0xFFFFFFFFu : 0u, in_before = q < rank ? 0xFFFFFFFFu : 0u;
+        sum_all.x += v[j].x & in_all; sum_all.y += v[j].y & in_all;
+        sum_all.z += v[j].z & in_all; sum_all.w += v[j].w & in_all;
+        sum_before.x += v[j].x & in_before; sum_before.y += v[j].y & in_before;
+        sum_before.z += v[j].z & in_before; sum_before.w += v[j].w & in_before;
+      }
+      *reinterpret_cast<uint4 *>(&sh.share[0][quarter][quad * 4]) = sum_all;
+      *reinterpret_cast<uint4 *>(&sh.share[1][quarter][quad * 4]) = sum_before;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      all += sh.share[0][q][tid];
+      before += sh.share[1][q][tid];
+    }
+    uint32_t sum = all;      // exclusive scan of the digit totals
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t u = __shfl_up_sync(0xFFFFFFFFu, sum, o);
+      if (lane >= (uint32_t)o) sum += u;
+    }
+    if (lane == 31) sh.wsum[warp] = sum;
+    __syncthreads();
+    uint32_t base = 0;
+#pragma unroll
+    for (uint32_t w = 0; w < kSortWarps; ++w)
+      if (w < warp) base += sh.wsum[w];
+    sh.off[tid] = base + sum - all + before;
+    __syncthreads();
+    if (short_stretch) {
+      if (lo < hi) {
+#pragma unroll
+        for (int r = 0; r < kSortRounds; ++r) {
+          if (lo + r * 32 >= hi) break;
+          const uint32_t d = (e[r].x >> shift) & (kDigits - 1);
+          put(sh.off[d] + mine[d] + place[r], e[r], lo + r * 32 + lane < hi);
         }
       }
-      tot[tid] = run;
-    }
-    cluster_sync();
-    uint32_t before = 0, all = 0, s = 0;
-    if (tid < kDigits) {
-      const uint32_t slot = (uint32_t)__cvta_generic_to_shared(tot + tid);
-      uint32_t v[kMaxCluster];
+    } else {
+      for (uint32_t i0 = lo; i0 < hi; i0 += 32 * kSortRounds) {
+        fetch(e, in, p == 0, i0);
+        rank_in(place, e, shift, i0);
 #pragma unroll
-      for (uint32_t c = 0; c < kMaxCluster; ++c) v[c] = c < n_ctas ? ld_cluster(peer_smem(slot, c)) : 0u;
-#pragma unroll
-      for (uint32_t c = 0; c < kMaxCluster; ++c) {
-        if (c < rank) before += v[c];
-        all += v[c];
-      }
-      // exclusive scan of the digit totals
-      s = all;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t u = __shfl_up_sync(0xFFFFFFFFu, s, o);
-        if (lane >= (uint32_t)o) s += u;
-      }
-      if (lane == 31) wsum[warp] = s;
-    }
-    __syncthreads();
-    if (tid < kDigits) {
-      uint32_t base = 0;
-#pragma unroll
-      for (uint32_t w = 0; w < kDigits / 32; ++w)
-        if (w < warp) base += wsum[w];
-      off[tid] = base + s - all + before;
-    }
-    __syncthreads();
-    for (int64_t i0 = lo; i0 < hi; i0 += 32 * kSortRounds) {
-      uint2 e[kSortRounds];
-      fetch(e, in, p == 0, i0);
-#pragma unroll
-      for (int r = 0; r < kSortRounds; ++r) {
-        if (i0 + r * 32 >= hi) break;
-        const bool on = i0 + r * 32 + lane < hi;
-        const uint32_t d = (e[r].x >> shift) & (kDigits - 1);
-        uint32_t peers = __ballot_sync(0xFFFFFFFFu, on);
-#pragma unroll
-        for (int bit = 0; bit < kDigitBits; ++bit) {
-          const bool set = (d >> bit) & 1u;
-          const uint32_t m = __ballot_sync(0xFFFFFFFFu, set);
-          peers &= set ? m : ~m;
+        for (int r = 0; r < kSortRounds; ++r) {
+          if (i0 + r * 32 >= hi) break;
+          put(sh.off[(e[r].x >> shift) & (kDigits - 1)] + place[r], e[r], i0 + r * 32 + lane < hi);
         }
-        uint32_t at = 0;
-        if (on) at = mine[d];
-        __syncwarp();
-        if (on && lane == (uint32_t)(__ffs(peers) - 1)) mine[d] = at + __popc(peers);
-        __syncwarp();
-        if (on) out[off[d] + at + __popc(peers & ((1u << lane) - 1u))] = e[r];
       }
     }
     __syncwarp();
-    cluster_sync();     // the next pass reads what other CTAs wrote, and overwrites tot
+    if (single) __syncthreads();
+    else cluster_sync();     // the next pass reads what other CTAs wrote, and overwrites tot
   }
+}
+
+// ------------------------------------------------------------------ zeros, and reading ahead
+struct ZeroArgs {
+  uint8_t *dw;
+  int64_t row_bytes, pitch, V;
+  int vec;                       // rows are 16-byte aligned vectors
+};
+
+// zeros in rows [first, last) but those of the bitmap, by the threads of one block
+__device__ __forceinline__ void zero_rows(const ZeroArgs &z, int64_t first, int64_t last, const uint32_t *named) {
+  const uint32_t per = (uint32_t)(z.vec ? z.row_bytes / 16 : z.row_bytes / 2);
+  const int64_t n = (last - first) * per;
+  for (int64_t i0 = 0; i0 < n; i0 += (int64_t)1 << 30) {      // 32-bit division inside
+    const int64_t row0 = first + i0 / per;
+    const uint32_t rem = (uint32_t)(i0 % per), m = (uint32_t)(n - i0 < ((int64_t)1 << 30) ? n - i0 : (int64_t)1 << 30);
+    for (uint32_t i = threadIdx.x; i < m; i += blockDim.x) {
+      const uint32_t r = (rem + i) / per, c = rem + i - r * per;
+      const int64_t row = row0 + r;
+      if (named && ((named[row >> 5] >> (row & 31)) & 1u)) continue;
+      uint8_t *p = z.dw + row * z.pitch;
+      if (z.vec) *reinterpret_cast<uint4 *>(p + (int64_t)c * 16) = make_uint4(0u, 0u, 0u, 0u);
+      else *reinterpret_cast<uint16_t *>(p + (int64_t)c * 2) = 0;
+    }
+  }
+}
+
+constexpr int kSideThreads = 256;
+constexpr uint32_t kPrefetchBytes = 8192;      // per instruction
+
+// What the SMs that do not sort do meanwhile: zeros in the first rows of the table (write), or the first
+// rows of dy into L2 (add).  Launched behind the sort without waiting for it; it waits for the sort only
+// before it ends, so that whoever waits for this kernel has the sorted list too.
+__global__ void __launch_bounds__(kSideThreads)
+embedding_side_kernel(ZeroArgs z, int64_t rows_per_block, const uint8_t *ahead, uint64_t ahead_bytes) {
+  pdl_trigger();
+  const int64_t first = blockIdx.x * rows_per_block, last = first + rows_per_block < z.V ? first + rows_per_block : z.V;
+  if (first < last) zero_rows(z, first, last, nullptr);
+  const uint64_t step = (uint64_t)gridDim.x * kPrefetchBytes;
+  if (threadIdx.x == 0)
+    for (uint64_t o = (uint64_t)blockIdx.x * kPrefetchBytes; o < ahead_bytes; o += step) {
+      const uint32_t n = (uint32_t)(ahead_bytes - o < kPrefetchBytes ? ahead_bytes - o : kPrefetchBytes);
+      asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(ahead + o), "r"(n) : "memory");
+    }
+  pdl_wait();
 }
 
 // ------------------------------------------------------------------ sums of runs
 constexpr int kRedThreads = 256;
 constexpr int kMaxPiece = 1024;      // sorted places per CTA
+constexpr uint32_t kWaitPolls = 1u << 20;
 
 struct RedArgs {
   const void *dy;
@@ -387,6 +458,12 @@ struct RedArgs {
   int per_part;                  // sorted places per group of L lanes
   float scale;
   int add;
+  uint32_t n_red, n_zero;        // blocks that add up runs, blocks that write zeros
+  uint32_t *flags;               // [piece][slice]: the partial sum of the run open at the piece's end is there
+  uint32_t *status;
+  ZeroArgs z;                    // zeros in rows from z_first on that `named` does not hold
+  int64_t z_first, z_per_block;
+  const uint32_t *named;
 };
 
 template <bool kDwF32, bool kVec>
@@ -409,13 +486,19 @@ __device__ __forceinline__ void flush_row(const RedArgs &a, uint32_t v, int c, c
   finish_row<kDwF32, kVec>(a, row, c, acc, old);
 }
 
-// A CTA takes one piece of the sorted list and one slice of 8 * L columns; each of its groups of L lanes
+// A block takes one piece of the sorted list and one slice of 8 * L columns; each of its groups of L lanes
 // takes per_part places of the piece.  A run inside a part goes straight to the table.  The sums of runs
 // that are open at a part's start or end are left in shared memory and joined in order by the group in whose
-// part the run starts; what is still open at the piece's start or end goes to `partial`.
+// part the run starts.  A run that is open at the piece's end leaves its sum in `partial`, raises the
+// piece's flag, and is finished by the block in whose piece it ends: that block waits for the flags of the pieces
+// before it (blocks start in index order, and a block raises its flag before it waits for anything; the
+// wait is bounded) and adds their sums in order.
 //
 // Bound by memory latency unless enough rows are in flight: a group always has the rows of the next kAhead
 // places on the way and, with "add", the old table rows of the runs that end among the next kOldAhead.
+//
+// When the whole table is written, blocks that write zeros into the rows no token names are dealt evenly
+// among the others, so that the two kinds of traffic overlap.
 template <bool kDyF32, bool kDwF32, bool kVec>
 __global__ void __launch_bounds__(kRedThreads, 2)
 embedding_reduce_kernel(RedArgs a) {
@@ -424,12 +507,24 @@ embedding_reduce_kernel(RedArgs a) {
   __shared__ uint8_t through[kRedThreads];            // the part is one run, open at both ends (slot 0)
   __shared__ uint2 list[kMaxPiece + 2];               // the piece's places and one on either side
   constexpr int kAhead = (kDyF32 || !kVec) ? 4 : 8, kOldAhead = 4;
-  pdl_trigger();
+  __shared__ uint32_t s_first;
+  uint32_t block = blockIdx.x;
+  if (a.n_zero) {
+    const uint64_t total = (uint64_t)a.n_red + a.n_zero;
+    block = (uint32_t)((uint64_t)blockIdx.x * a.n_red / total);
+    if ((uint32_t)((blockIdx.x + 1ull) * a.n_red / total) == block) {
+      pdl_wait();
+      const int64_t first = a.z_first + (int64_t)(blockIdx.x - block) * a.z_per_block;
+      const int64_t last = first + a.z_per_block < a.z.V ? first + a.z_per_block : a.z.V;
+      if (first < last) zero_rows(a.z, first, last, a.named);
+      return;
+    }
+  }
   const int L = a.L, l = threadIdx.x & (L - 1), part = threadIdx.x / L, parts = kRedThreads / L;
-  const int64_t piece = blockIdx.x / a.slices;
-  const int slice = (int)(blockIdx.x - piece * a.slices), c = first_col<kVec>(slice * 8 * L, l);
+  const uint32_t piece = block / a.slices;
+  const int slice = (int)(block - piece * a.slices), c = first_col<kVec>(slice * 8 * L, l);
   const int len = parts * a.per_part;
-  const int64_t p0 = piece * len;
+  const int64_t p0 = (int64_t)piece * len;
   for (int i = threadIdx.x; i < 2 * parts; i += kRedThreads) open_key[i & 1][i >> 1] = a.V;
   if (l == 0) through[part] = 0;
   pdl_wait();
@@ -493,8 +588,19 @@ embedding_reduce_kernel(RedArgs a) {
     }
   }
   __syncthreads();
-  float *partial = a.partial + (piece * 2 * a.slices + slice) * (int64_t)(8 * L) + l;
-  const int64_t slot = (int64_t)a.slices * 8 * L;
+  // [piece][slice][8 * L]: the sum of the run that is open at the piece's end, over this piece
+  float *partial = a.partial + slice * (8 * L) + l;
+  const int64_t pitch = (int64_t)a.slices * 8 * L;
+  auto publish = [&](const float (&sum)[8]) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) partial[piece * pitch + e * L] = sum[e];
+    __syncwarp(L == 32 ? 0xFFFFFFFFu : ((1u << L) - 1u) << (threadIdx.x & 31 & ~(L - 1)));
+    if (l == 0) {
+      __threadfence();
+      asm volatile("st.release.gpu.global.u32 [%0], %1;" ::"l"(a.flags + (int64_t)piece * a.slices + slice), "r"(1u)
+                   : "memory");
+    }
+  };
   // the run this part starts and leaves open
   const uint32_t ko = open_key[1][part];
   if (ko != a.V) {
@@ -507,77 +613,73 @@ embedding_reduce_kernel(RedArgs a) {
       for (int e = 0; e < 8; ++e) sum[e] = __fadd_rn(sum[e], open_sum[0][q * 8 * L + e * L + l]);
       open = through[q];
     }
-    if (!open) {
-      flush_row<kDwF32, kVec>(a, ko, c, sum);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) partial[slot + e * L] = sum[e];
-    }
+    if (!open) flush_row<kDwF32, kVec>(a, ko, c, sum);
+    else publish(sum);
   }
   // the run that was open before the piece
-  if (part == 0 && open_key[0][0] != a.V) {
-    float sum[8];
+  const uint32_t kb = open_key[0][0];
+  if (kb == a.V) return;
+  int n_through = 0;
+  while (n_through < parts && through[n_through]) ++n_through;
+  float own[8];
+  if (part == 0) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) sum[e] = open_sum[0][e * L + l];
-    for (int q = 1; q < parts && through[q - 1]; ++q) {
+    for (int e = 0; e < 8; ++e) own[e] = open_sum[0][e * L + l];
+    for (int q = 1; q <= n_through && q < parts; ++q) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) sum[e] = __fadd_rn(sum[e], open_sum[0][q * 8 * L + e * L + l]);
+      for (int e = 0; e < 8; ++e) own[e] = __fadd_rn(own[e], open_sum[0][q * 8 * L + e * L + l]);
     }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) partial[e * L] = sum[e];
+    if (n_through == parts) publish(own);
   }
-}
-
-// Runs that cross pieces.  A CTA takes one piece and one slice; if a run starts in the piece and is still
-// open at its end, its groups add the partial sums of the pieces it covers, group i those of every parts-th piece
-// from the i-th, and the groups' sums are added in order.
-template <bool kDwF32, bool kVec>
-__global__ void __launch_bounds__(kRedThreads)
-embedding_join_kernel(RedArgs a, int64_t pieces) {
-  __shared__ float sums[kRedThreads * 8];
-  __shared__ int64_t s_last;
-  pdl_trigger();
-  const int L = a.L, l = threadIdx.x & (L - 1), part = threadIdx.x / L, parts = kRedThreads / L;
-  const int64_t piece = blockIdx.x / a.slices;
-  const int slice = (int)(blockIdx.x - piece * a.slices), c = first_col<kVec>(slice * 8 * L, l);
-  const int64_t len = (int64_t)parts * a.per_part, p0 = piece * len, p1 = p0 + len;
-  pdl_wait();
-  if (p1 >= a.T) return;
-  const uint32_t k = __ldcg(&a.list[p1 - 1].x), k1 = __ldcg(&a.list[p1].x), kp = p0 > 0 ? __ldcg(&a.list[p0 - 1].x) : a.V;
-  if (k >= a.V || k1 != k || kp == k) return;      // no open run, or one that starts in an earlier piece
-  if (threadIdx.x < 32) {      // last piece of the run: pieces start with k up to there
-    int64_t last = piece;
-    for (int64_t q0 = piece + 1; q0 < pieces; q0 += 32) {
-      const int64_t q = q0 + threadIdx.x;
-      const bool same = q < pieces && __ldcg(&a.list[q * len].x) == k;
+  if (n_through == parts) return;
+  // It ends here.  First piece: going back, pieces before which the list holds the same id.
+  if (threadIdx.x < 32) {
+    uint32_t first = piece - 1;
+    for (int64_t q0 = first;; q0 -= 32) {
+      const int64_t q = q0 - threadIdx.x;
+      const bool same = q > 0 && __ldcg(&a.list[q * len - 1].x) == kb;
       const uint32_t m = __ballot_sync(0xFFFFFFFFu, same);
-      last += __popc(m);
-      if (m != 0xFFFFFFFFu) break;
+      const uint32_t run = m == 0xFFFFFFFFu ? 32u : (uint32_t)__ffs(~m) - 1u;
+      first -= run;
+      if (run < 32u) break;
     }
-    if (threadIdx.x == 0) s_last = last;
+    if (threadIdx.x == 0) s_first = first;
   }
   __syncthreads();
-  const int64_t count = s_last - piece;      // pieces piece + 1 .. s_last
-  const int64_t slot = (int64_t)a.slices * 8 * L;
-  const float *base = a.partial + (int64_t)slice * 8 * L + l;
+  const uint32_t first = s_first;
+  bool ok = true;
+  for (uint32_t q = first + threadIdx.x; q < piece; q += kRedThreads) {
+    uint32_t seen = 0;
+    for (uint32_t i = 0; i < kWaitPolls && !seen; ++i)
+      asm volatile("ld.acquire.gpu.global.u32 %0, [%1];"
+                   : "=r"(seen)
+                   : "l"(a.flags + (int64_t)q * a.slices + slice)
+                   : "memory");
+    ok = ok && seen;
+  }
+  if (!__syncthreads_and(ok)) {
+    if (!ok) atomicOr(a.status, ANC_DEV_TIMEOUT_DEP);
+    return;
+  }
+  // group i adds the sums of every parts-th piece from the i-th, group 0 then the groups' sums
   float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-  for (int64_t q = piece + 1 + part; q <= s_last; q += parts) {
-    const float *p = base + q * 2 * slot;
+  for (uint32_t q = first + part; q < piece; q += parts) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) acc[e] = __fadd_rn(acc[e], __ldcg(p + e * L));
+    for (int e = 0; e < 8; ++e) acc[e] = __fadd_rn(acc[e], __ldcg(partial + q * pitch + e * L));
   }
+  float *sums = open_sum[1];
 #pragma unroll
   for (int e = 0; e < 8; ++e) sums[part * 8 * L + e * L + l] = acc[e];
   __syncthreads();
   if (part != 0) return;
-  const float *first = base + (piece * 2 + 1) * slot;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) acc[e] = __ldcg(first + e * L);
-  for (int w = 0; w < parts && w < count; ++w)
+  for (int w = 1; w < parts && (uint32_t)w < piece - first; ++w) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) acc[e] = __fadd_rn(acc[e], sums[w * 8 * L + e * L + l]);
-  flush_row<kDwF32, kVec>(a, k, c, acc);
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) acc[e] = __fadd_rn(acc[e], own[e]);
+  flush_row<kDwF32, kVec>(a, kb, c, acc);
 }
 
 // ------------------------------------------------------------------ few tokens
@@ -645,6 +747,10 @@ embedding_small_kernel(RedArgs a, const void *__restrict__ ids, int ids64, int64
 
 // ------------------------------------------------------------------ host side
 constexpr int kMaxPart = 32, kMinPart = 4;
+constexpr int kSortTarget = 4;               // rounds of 32 keys per warp the sort aims at
+constexpr int64_t kZeroBytes = 128 << 10;    // zeros per block
+constexpr int64_t kSideBytes = 64 << 20;     // zeros beside the sort
+constexpr uint64_t kAheadBytes = 64 << 20;   // of dy into L2 beside the sort
 constexpr int64_t kFullGrid = 888;       // CTAs the reduction should have at least
 
 struct Shape {
@@ -671,10 +777,11 @@ Shape shape_of(int64_t T, int64_t D) {
 }
 
 struct Workspace {
-  size_t list[2], partial, total;
+  size_t list[2], clear, partial, total;
+  uint32_t n_flags, n_named;       // words at `clear`
 };
 
-Workspace workspace_of(int64_t T, int64_t D) {
+Workspace workspace_of(int64_t T, int64_t V, int64_t D) {
   const Shape s = shape_of(T, D);
   auto up = [](size_t x) { return (x + 255) / 256 * 256; };
   Workspace w;
@@ -683,9 +790,13 @@ Workspace workspace_of(int64_t T, int64_t D) {
     w.list[i] = at;
     at += up((size_t)T * sizeof(uint2));
   }
+  w.n_flags = (uint32_t)(s.max_pieces * s.slices);
+  w.n_named = (uint32_t)((V + 31) / 32);
+  w.clear = at;
+  at += up(((size_t)w.n_flags + w.n_named) * 4);
   w.partial = at;
-  at += up((size_t)s.max_pieces * 2 * s.slices * 8 * s.L * 4);
-  w.total = at ? at : 256;
+  at += up((size_t)s.max_pieces * s.slices * 8 * s.L * 4);
+  w.total = at;
   return w;
 }
 
@@ -703,16 +814,41 @@ int check_dtype(int d, const char *what) {
   return ANC_OK;
 }
 
-// Raises the sort's shared-memory limit once per device.
-cudaError_t sort_kernel_ready(int device) {
+// Largest cluster the sort can use on a device (0: an error is set); asked once per device.
+uint32_t sort_cluster(int device) {
   static std::mutex mu;
-  static bool done[64] = {};
+  static uint32_t most[64] = {};
   std::lock_guard<std::mutex> lock(mu);
-  if (device >= 0 && device < 64 && done[device]) return cudaSuccess;
-  const cudaError_t e =
-      cudaFuncSetAttribute(embedding_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSortSmem);
-  if (e == cudaSuccess && device >= 0 && device < 64) done[device] = true;
-  return e;
+  if (device >= 0 && device < 64 && most[device]) return most[device];
+  cudaError_t e = cudaFuncSetAttribute(embedding_sort_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  if (e == cudaSuccess)
+    e = cudaFuncSetAttribute(embedding_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(SortShared));
+  uint32_t found = 8;                // the portable size
+  for (uint32_t c = kMaxCluster; e == cudaSuccess && c > 8; c /= 2) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(c);
+    cfg.blockDim = dim3(kSortThreads);
+    cfg.dynamicSmemBytes = sizeof(SortShared);
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = c;
+    at[0].val.clusterDim.y = 1;
+    at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    int n = 0;
+    if (cudaOccupancyMaxActiveClusters(&n, embedding_sort_kernel, &cfg) == cudaSuccess && n > 0) {
+      found = c;
+      break;
+    }
+    cudaGetLastError();
+  }
+  if (e != cudaSuccess) {
+    anc_cuda_fail(e, "sort kernel attributes");
+    return 0;
+  }
+  if (device >= 0 && device < 64) most[device] = found;
+  return found;
 }
 
 bool rows_are_vectors(const void *p, int64_t ld, int f32, int64_t D) {
@@ -769,7 +905,7 @@ int anc_embedding_grad_workspace(int64_t T, int64_t V, int64_t D, uint64_t *byte
   ANC_REQUIRE(bytes, "bytes is NULL");
   int rc = check_sizes(T, V, D);
   if (rc) return rc;
-  *bytes = workspace_of(T, D).total;
+  *bytes = workspace_of(T, V, D).total;
   return ANC_OK;
 }
 
@@ -794,7 +930,7 @@ int anc_embedding_grad(anc_ctx *ctx, const void *dy, int dy_dtype, int64_t dy_ld
                 "pointer not aligned to its element size");
     ANC_REQUIRE(((uintptr_t)work & 15) == 0, "workspace not aligned to 16 bytes");
   }
-  const Workspace ws = workspace_of(T, D);
+  const Workspace ws = workspace_of(T, V, D);
   ANC_REQUIRE(T == 0 || work_bytes >= ws.total, "workspace of %llu bytes, %llu are needed",
               (unsigned long long)work_bytes, (unsigned long long)ws.total);
   if (T == 0 && mode == ANC_EMBED_ADD) return ANC_OK;
@@ -810,42 +946,70 @@ int anc_embedding_grad(anc_ctx *ctx, const void *dy, int dy_dtype, int64_t dy_ld
   cudaLaunchAttribute pdl[1];
   pdl[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   pdl[0].val.programmaticStreamSerializationAllowed = 1;
-  auto launch_zero = [&](int n_attrs) {
-    const int64_t items = V * (za.row_bytes / (za.vec ? 16 : 2)), cap = (int64_t)ctx->sm_count * 16;
+  // zeros in the table's first `rows` rows, `ahead` bytes of dy into L2
+  auto launch_side = [&](int64_t rows, uint64_t ahead, int n_attrs) {
+    ZeroArgs z = za;
+    z.V = rows;
+    const uint8_t *from = (const uint8_t *)(((uintptr_t)dy + 15) & ~(uintptr_t)15);
+    const int64_t per_block = za.row_bytes < kZeroBytes ? kZeroBytes / za.row_bytes : 1;
+    int64_t blocks = (rows + per_block - 1) / per_block;
+    const int64_t fetches = (int64_t)((ahead + kPrefetchBytes - 1) / kPrefetchBytes);
+    if (blocks < 1) blocks = fetches < ctx->sm_count * 4 ? fetches : ctx->sm_count * 4;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)((items + 255) / 256 < cap ? (items + 255) / 256 : cap));
-    cfg.blockDim = dim3(256);
+    cfg.gridDim = dim3((unsigned)blocks);
+    cfg.blockDim = dim3(kSideThreads);
     cfg.stream = st;
     cfg.attrs = pdl;
     cfg.numAttrs = n_attrs;
-    return cudaLaunchKernelEx(&cfg, embedding_zero_kernel, za);
+    return cudaLaunchKernelEx(&cfg, embedding_side_kernel, z, per_block, from, ahead);
   };
-  if (write && small) ANC_CUDA(launch_zero(0));
+  if (write && small) ANC_CUDA(launch_side(V, 0, 0));
   if (T == 0) return ANC_OK;
   uint8_t *wp = (uint8_t *)work;
-  SortArgs sa;
-  sa.ids = ids; sa.ids64 = i64; sa.T = T; sa.V = V; sa.padding_idx = padding_idx;
-  for (int i = 0; i < 2; ++i) sa.list[i] = (uint2 *)(wp + ws.list[i]);
-  int bits = 0;
-  while (((uint64_t)V >> bits) != 0) ++bits;
-  sa.passes = (bits + kDigitBits - 1) / kDigitBits;
-  sa.status = ctx->d_status;
   const Shape sh = shape_of(T, D);
-  RedArgs ra;
+  RedArgs ra = {};
   ra.dy = dy; ra.dw = dw; ra.dy_ld = dy_ld; ra.dw_ld = dw_ld; ra.T = T;
-  ra.list = sa.list[(sa.passes - 1) & 1];
   ra.partial = (float *)(wp + ws.partial);
   ra.V = (uint32_t)V; ra.D = (int)D; ra.slices = sh.slices; ra.L = sh.L; ra.per_part = sh.per_part; ra.scale = scale;
   ra.add = !write;
-  const int64_t grid = small ? (T * sh.slices + kRedThreads / sh.L - 1) / (kRedThreads / sh.L) : sh.pieces * sh.slices;
-  ANC_REQUIRE(grid <= 0x7FFFFFFF, "T x D too large");
+  ra.status = ctx->d_status;
+  const int64_t n_red = small ? (T * sh.slices + kRedThreads / sh.L - 1) / (kRedThreads / sh.L) : sh.pieces * sh.slices;
+  ANC_REQUIRE(n_red <= 0x3FFFFFFF, "T x D too large");
+  ra.n_red = (uint32_t)n_red;
+  int n_attrs = write ? 1 : 0;
   if (!small) {
-    ANC_CUDA(sort_kernel_ready(ctx->device));
-    const uint32_t n_ctas = T <= 4096 ? 1 : T <= 8192 ? 2 : T <= 16384 ? 4 : 8;
+    SortArgs sa = {};
+    sa.ids = ids; sa.ids64 = i64; sa.T = (uint32_t)T; sa.V = V; sa.padding_idx = padding_idx;
+    for (int i = 0; i < 2; ++i) sa.list[i] = (uint2 *)(wp + ws.list[i]);
+    int bits = 0;
+    while (((uint64_t)V >> bits) != 0) ++bits;
+    sa.passes = (bits + kDigitBits - 1) / kDigitBits;
+    sa.status = ctx->d_status;
+    // rows the side launch zeroes while the sort runs; the rest is the reduction's, named rows left out
+    const int64_t side_rows = !write ? 0 : za.row_bytes * V <= kSideBytes ? V : kSideBytes / za.row_bytes;
+    sa.clear = (uint32_t *)(wp + ws.clear);
+    ra.flags = sa.clear;
+    sa.n_clear = (uint32_t)(sh.pieces * sh.slices);
+    if (side_rows < V && write) {
+      sa.named = sa.clear + ws.n_flags;
+      sa.n_clear = ws.n_flags + ws.n_named;
+      ra.named = sa.named;
+      ra.z = za;
+      ra.z_first = side_rows;
+      ra.z_per_block = za.row_bytes < kZeroBytes ? kZeroBytes / za.row_bytes : 1;
+      const int64_t n_zero = (V - side_rows + ra.z_per_block - 1) / ra.z_per_block;
+      ANC_REQUIRE(n_zero <= 0x3FFFFFFF, "table too large");
+      ra.n_zero = (uint32_t)n_zero;
+    }
+    ra.list = sa.list[(sa.passes - 1) & 1];
+    const uint32_t most = sort_cluster(ctx->device);
+    if (!most) return ANC_E_CUDA;
+    uint32_t n_ctas = 1;
+    while (n_ctas < most && (int64_t)n_ctas * kSortThreads * kSortTarget < T) n_ctas *= 2;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(n_ctas);
     cfg.blockDim = dim3(kSortThreads);
-    cfg.dynamicSmemBytes = kSortSmem;
+    cfg.dynamicSmemBytes = sizeof(SortShared);
     cfg.stream = st;
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeClusterDimension;
@@ -855,24 +1019,26 @@ int anc_embedding_grad(anc_ctx *ctx, const void *dy, int dy_dtype, int64_t dy_ld
     cfg.attrs = at;
     cfg.numAttrs = 1;
     ANC_CUDA(cudaLaunchKernelEx(&cfg, embedding_sort_kernel, sa, n_ctas));
-    if (write) ANC_CUDA(launch_zero(1));
+    // with "add", as much of dy as the sort's time can bring in and L2 can hold
+    const uint64_t dy_bytes = ((uint64_t)(T - 1) * dy_ld + D) * (yf ? 4 : 2) / 16 * 16;
+    const uint64_t ahead = write || dy_bytes < 64 ? 0 : dy_bytes - 16 < kAheadBytes ? dy_bytes - 16 : kAheadBytes;
+    if (side_rows || ahead) ANC_CUDA(launch_side(side_rows, ahead, 1));
+    n_attrs = 1;
   }
-  // the following launches start while their predecessor drains and wait for it on the device
+  // these launches start while their predecessor drains and wait for it on the device
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)grid);
+  cfg.gridDim = dim3(ra.n_red + ra.n_zero);
   cfg.blockDim = dim3(kRedThreads);
   cfg.stream = st;
   cfg.attrs = pdl;
-  cfg.numAttrs = small && !write ? 0 : 1;
+  cfg.numAttrs = n_attrs;
   const bool vec = rows_are_vectors(dy, dy_ld, yf, D) && rows_are_vectors(dw, dw_ld, wf, D);
 #define ANC_REDUCE(Y, W, VEC)                                                                        \
   do {                                                                                               \
-    if (small) {                                                                                     \
+    if (small)                                                                                       \
       ANC_CUDA(cudaLaunchKernelEx(&cfg, embedding_small_kernel<Y, W, VEC>, ra, ids, i64, padding_idx, ctx->d_status)); \
-    } else {                                                                                         \
+    else                                                                                             \
       ANC_CUDA(cudaLaunchKernelEx(&cfg, embedding_reduce_kernel<Y, W, VEC>, ra));                    \
-      if (sh.pieces > 1) ANC_CUDA(cudaLaunchKernelEx(&cfg, embedding_join_kernel<W, VEC>, ra, sh.pieces)); \
-    }                                                                                                \
   } while (0)
 #define ANC_REDUCE_V(Y, W)                \
   do {                                    \
