@@ -12,7 +12,9 @@
 // tokens keep their order), the sorted list is cut into equal pieces, each piece sums its runs of equal
 // ids, and runs that cross a piece's border are joined from the pieces' partial sums in order.  The work is balanced
 // however often one token occurs.
+#include <algorithm>
 #include <cuda_bf16.h>
+#include <initializer_list>
 #include <mutex>
 #include "anc_internal.h"
 #include "philox.cuh"
@@ -21,67 +23,56 @@
 namespace {
 
 // ------------------------------------------------------------------ rows in registers
-// A lane holds eight columns of a row: eight neighbouring ones where rows are 16-byte aligned vectors of
-// eight (kVec), else every L-th of a group of L lanes.
-template <bool kVec>
-__device__ __forceinline__ int first_col(int c0, int l) {
-  return kVec ? c0 + l * 8 : c0 + l;
-}
-
-// the eight elements as they lie in memory
+// Eight columns of a row as they lie in memory: eight neighbouring ones, in one access, where rows are vectors
+// of eight aligned to their size (kVec: 16 bytes of bf16, 32 of f32), else every L-th column.
 template <bool kF32, bool kVec>
-struct Row8 {
+struct Oct {
   uint32_t w[(kF32 || !kVec) ? 8 : 4];
 };
 
+// p: address of the first column; cols: columns from there to the row's end
 template <bool kF32, bool kVec>
-__device__ __forceinline__ void load_row(Row8<kF32, kVec> &r, const void *row, int c, int L, int D, bool on) {
+__device__ __forceinline__ void load_oct(Oct<kF32, kVec> &r, const uint8_t *p, int cols, int L, bool on) {
   if constexpr (kVec) {
-    const uint8_t *q = (const uint8_t *)row + (int64_t)c * (kF32 ? 4 : 2);
-    on = on && c < D;
-    ld_v4(r.w[0], r.w[1], r.w[2], r.w[3], q, on);
-    if constexpr (kF32) ld_v4(r.w[4], r.w[5], r.w[6], r.w[7], q + 16, on);
+    on = on && cols > 0;
+    if constexpr (kF32) ld_v8(r.w, p, on);
+    else ld_v4(r.w[0], r.w[1], r.w[2], r.w[3], p, on);
   } else {
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-      const int ck = c + k * L;
-      if constexpr (kF32) ld_1(r.w[k], (const float *)row + ck, on && ck < D);
-      else ld_h(r.w[k], (const uint16_t *)row + ck, on && ck < D);
+      if constexpr (kF32) ld_1(r.w[k], (const float *)p + k * L, on && k * L < cols);
+      else ld_h(r.w[k], (const uint16_t *)p + k * L, on && k * L < cols);
     }
   }
 }
 
 template <bool kF32, bool kVec>
-__device__ __forceinline__ float elem(const Row8<kF32, kVec> &r, int k) {
+__device__ __forceinline__ float elem(const Oct<kF32, kVec> &r, int k) {
   if constexpr (kF32) return __uint_as_float(r.w[k]);
   else if constexpr (!kVec) return __uint_as_float(r.w[k] << 16);
   else return __uint_as_float((k & 1) ? (r.w[k >> 1] & 0xFFFF0000u) : (r.w[k >> 1] << 16));
 }
 
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t *>(&h);
+}
+
 template <bool kF32, bool kVec>
-__device__ __forceinline__ void store_row(void *row, int c, int L, int D, const float x[8]) {
+__device__ __forceinline__ void store_oct(uint8_t *p, int cols, int L, const float (&x)[8]) {
   if constexpr (kVec) {
-    if (c >= D) return;
-    if constexpr (kF32) {
-      float4 *d = reinterpret_cast<float4 *>((float *)row + c);
-      d[0] = make_float4(x[0], x[1], x[2], x[3]);
-      d[1] = make_float4(x[4], x[5], x[6], x[7]);
-    } else {
-      uint32_t h[8];
-#pragma unroll
-      for (int k = 0; k < 8; ++k) h[k] = bf16_rne(x[k]);
-      *reinterpret_cast<uint4 *>((uint16_t *)row + c) =
-          make_uint4(h[0] | (h[1] << 16), h[2] | (h[3] << 16), h[4] | (h[5] << 16), h[6] | (h[7] << 16));
-    }
+    if (cols <= 0) return;
+    if constexpr (kF32) st_v8(p, x);
+    else
+      *reinterpret_cast<uint4 *>(p) =
+          make_uint4(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7]));
   } else {
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const int ck = c + k * L;
-      if (ck < D) {
-        if constexpr (kF32) ((float *)row)[ck] = x[k];
-        else ((uint16_t *)row)[ck] = (uint16_t)bf16_rne(x[k]);
+    for (int k = 0; k < 8; ++k)
+      if (k * L < cols) {
+        if constexpr (kF32) ((float *)p)[k * L] = x[k];
+        else ((uint16_t *)p)[k * L] = (uint16_t)bf16_rne(x[k]);
       }
-    }
   }
 }
 
@@ -131,13 +122,13 @@ embedding_lookup_kernel(const void *__restrict__ table, int64_t table_ld, const 
 #pragma unroll
       for (int u = 0; u < U; ++u) id[u] = ((const int32_t *)ids)[t[u]];
     }
-    Row8<kTabF32, kVec> x[U];      // !kVec: only the first element
+    Oct<kTabF32, kVec> x[U];      // !kVec: only the first element
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const bool live = id[u] >= 0 && id[u] < V && c[u] >= 0;
       const void *row = row_ptr<kTabF32>(table, live ? id[u] : 0, table_ld);
-      x[u] = Row8<kTabF32, kVec>{};
-      if constexpr (kVec) load_row<kTabF32, true>(x[u], row, c[u], 0, D, live);
+      x[u] = Oct<kTabF32, kVec>{};
+      if constexpr (kVec) load_oct<kTabF32, true>(x[u], (const uint8_t *)row + c[u] * (kTabF32 ? 4 : 2), 8, 0, live);
       else if constexpr (kTabF32) ld_1(x[u].w[0], (const float *)row + c[u], live);
       else ld_h(x[u].w[0], (const uint16_t *)row + c[u], live);
     }
@@ -152,7 +143,7 @@ embedding_lookup_kernel(const void *__restrict__ table, int64_t table_ld, const 
         float f[8];
 #pragma unroll
         for (int k = 0; k < 8; ++k) f[k] = __fmul_rn(elem(x[u], k), scale);
-        store_row<kOutF32, true>(row, c[u], 0, D, f);
+        store_oct<kOutF32, true>((uint8_t *)row + c[u] * (kOutF32 ? 4 : 2), 8, 0, f);
       } else {
         const float f = __fmul_rn(elem(x[u], 0), scale);
         if constexpr (kOutF32) ((float *)row)[c[u]] = f;
@@ -443,15 +434,16 @@ embedding_side_kernel(ZeroArgs z, int64_t rows_per_block, const uint8_t *ahead, 
 
 // ------------------------------------------------------------------ sums of runs
 constexpr int kRedThreads = 256;
-constexpr int kMaxPiece = 1024;      // sorted places per CTA
+constexpr int kMaxPiece = 512;       // sorted places per block
 constexpr uint32_t kWaitPolls = 1u << 20;
 
 struct RedArgs {
-  const void *dy;
-  void *dw;
-  int64_t dy_ld, dw_ld, T;
+  const uint8_t *dy;
+  uint8_t *dw;
+  uint32_t dy_pitch, dw_pitch;   // bytes from row to row
+  int64_t T;
   const uint2 *list;             // sorted (id, token)
-  float *partial;                // [piece][open at its start, open at its end][slices * 8 * L], register layout
+  float *partial;                // [piece][slices * columns of a slice], register layout
   uint32_t V;
   int D, slices;
   int L;                         // lanes that share a row's slice: a power of two up to 32
@@ -466,27 +458,100 @@ struct RedArgs {
   const uint32_t *named;
 };
 
-template <bool kDwF32, bool kVec>
-__device__ __forceinline__ void finish_row(const RedArgs &a, void *row, int c, const float acc[8],
-                                           const Row8<kDwF32, kVec> &old) {
-  float x[8];
-#pragma unroll
-  for (int k = 0; k < 8; ++k) {
-    x[k] = __fmul_rn(a.scale, acc[k]);
-    if (a.add) x[k] = __fadd_rn(elem(old, k), x[k]);
+// A lane's columns of a slice: sixteen in two octets, all lanes' first octets before their second ones, or
+// eight where rows are not vectors.  Sums are pairs of floats (one instruction adds two).
+template <bool kVec>
+struct Cols {
+  static constexpr int kOcts = kVec ? 2 : 1, kEach = 8 * kOcts;
+};
+template <bool kVec>
+struct Sum {
+  uint64_t p[Cols<kVec>::kEach / 2];
+  __device__ __forceinline__ float get(int k) const {
+    return __uint_as_float((uint32_t)((k & 1) ? p[k >> 1] >> 32 : p[k >> 1]));
   }
-  store_row<kDwF32, kVec>(row, c, a.L, a.D, x);
-}
+  __device__ __forceinline__ void add_pair(int i, float lo, float hi) {
+    asm("{\n\t.reg .b64 t;\n\tmov.b64 t, {%1, %2};\n\tadd.rn.f32x2 %0, %0, t;\n\t}" : "+l"(p[i]) : "f"(lo), "f"(hi));
+  }
+  __device__ __forceinline__ void set_pair(int i, float lo, float hi) {
+    asm("mov.b64 %0, {%1, %2};" : "=l"(p[i]) : "f"(lo), "f"(hi));
+  }
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < Cols<kVec>::kEach / 2; ++i) p[i] = 0ull;
+  }
+  // as kEach floats `pitch` apart
+  __device__ __forceinline__ void put(float *d, int pitch) const {
+#pragma unroll
+    for (int k = 0; k < Cols<kVec>::kEach; ++k) d[k * pitch] = get(k);
+  }
+  __device__ __forceinline__ void set(const float *d, int pitch) {
+#pragma unroll
+    for (int i = 0; i < Cols<kVec>::kEach / 2; ++i) set_pair(i, d[2 * i * pitch], d[(2 * i + 1) * pitch]);
+  }
+  __device__ __forceinline__ void add(const float *d, int pitch) {
+#pragma unroll
+    for (int i = 0; i < Cols<kVec>::kEach / 2; ++i) add_pair(i, d[2 * i * pitch], d[(2 * i + 1) * pitch]);
+  }
+};
 
-template <bool kDwF32, bool kVec>
-__device__ __forceinline__ void flush_row(const RedArgs &a, uint32_t v, int c, const float acc[8]) {
-  void *row = row_ptr<kDwF32>(a.dw, v, a.dw_ld);
-  Row8<kDwF32, kVec> old = {};
-  load_row<kDwF32, kVec>(old, row, c, a.L, a.D, a.add);
-  finish_row<kDwF32, kVec>(a, row, c, acc, old);
-}
+template <bool kF32, bool kVec>
+struct Row {
+  Oct<kF32, kVec> o[Cols<kVec>::kOcts];
+  __device__ __forceinline__ void load(const uint8_t *p, int cols, int L, bool on) {
+#pragma unroll
+    for (int q = 0; q < Cols<kVec>::kOcts; ++q)
+      load_oct<kF32, kVec>(o[q], p + q * 8 * L * (kF32 ? 4 : 2), cols - q * 8 * L, L, on);
+  }
+  __device__ __forceinline__ void add_to(Sum<kVec> &s) const {
+#pragma unroll
+    for (int q = 0; q < Cols<kVec>::kOcts; ++q)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s.add_pair(q * 4 + i, elem(o[q], 2 * i), elem(o[q], 2 * i + 1));
+  }
+};
 
-// A block takes one piece of the sorted list and one slice of 8 * L columns; each of its groups of L lanes
+// One lane's view of the rows: its first column, and the columns from there to the row's end.
+template <bool kDyF32, bool kDwF32, bool kVec>
+struct Lane {
+  const uint8_t *dy;
+  uint8_t *dw;
+  int cols;
+  __device__ __forceinline__ Lane(const RedArgs &a, int slice, int l) {
+    const int c = slice * Cols<kVec>::kEach * a.L + (kVec ? l * 8 : l);
+    cols = a.D - c;
+    dy = a.dy + (int64_t)c * (kDyF32 ? 4 : 2);
+    dw = a.dw + (int64_t)c * (kDwF32 ? 4 : 2);
+  }
+  __device__ __forceinline__ const uint8_t *dy_row(const RedArgs &a, uint32_t t) const {
+    return dy + (uint64_t)t * a.dy_pitch;
+  }
+  __device__ __forceinline__ uint8_t *dw_row(const RedArgs &a, uint32_t v) const {
+    return dw + (uint64_t)v * a.dw_pitch;
+  }
+  // the finished sum of row v into the table
+  __device__ __forceinline__ void finish(const RedArgs &a, uint32_t v, const Sum<kVec> &s,
+                                         const Row<kDwF32, kVec> &old) const {
+    uint8_t *p = dw_row(a, v);
+#pragma unroll
+    for (int q = 0; q < Cols<kVec>::kOcts; ++q) {
+      float x[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        x[k] = __fmul_rn(a.scale, s.get(q * 8 + k));
+        if (a.add) x[k] = __fadd_rn(elem(old.o[q], k), x[k]);
+      }
+      store_oct<kDwF32, kVec>(p + q * 8 * a.L * (kDwF32 ? 4 : 2), cols - q * 8 * a.L, a.L, x);
+    }
+  }
+  __device__ __forceinline__ void flush(const RedArgs &a, uint32_t v, const Sum<kVec> &s) const {
+    Row<kDwF32, kVec> old = {};
+    old.load(dw_row(a, v), cols, a.L, a.add);
+    finish(a, v, s, old);
+  }
+};
+
+// A block takes one piece of the sorted list and one slice of columns; each of its groups of L lanes
 // takes per_part places of the piece.  A run inside a part goes straight to the table.  The sums of runs
 // that are open at a part's start or end are left in shared memory and joined in order by the group in whose
 // part the run starts.  A run that is open at the piece's end leaves its sum in `partial`, raises the
@@ -502,11 +567,13 @@ __device__ __forceinline__ void flush_row(const RedArgs &a, uint32_t v, int c, c
 template <bool kDyF32, bool kDwF32, bool kVec>
 __global__ void __launch_bounds__(kRedThreads, 2)
 embedding_reduce_kernel(RedArgs a) {
-  __shared__ float open_sum[2][kRedThreads * 8];      // [slot][part][8 * L]
+  constexpr int kEach = Cols<kVec>::kEach, kStep = 4;
+  constexpr int kAhead = (kDyF32 && kVec) ? 2 : 4, kOldAhead = (kDwF32 && kVec) ? 2 : 4;
+  constexpr uint32_t kEnds = 0x80000000u;             // in a token number: the run ends here
+  __shared__ float open_sum[2][kRedThreads * kEach];  // [slot][part][kEach * L]
   __shared__ uint32_t open_key[2][kRedThreads];       // V: nothing open
   __shared__ uint8_t through[kRedThreads];            // the part is one run, open at both ends (slot 0)
-  __shared__ uint2 list[kMaxPiece + 2];               // the piece's places and one on either side
-  constexpr int kAhead = (kDyF32 || !kVec) ? 4 : 8, kOldAhead = 4;
+  __shared__ uint2 list[kMaxPiece + 1];               // the place before the piece, the piece's places
   __shared__ uint32_t s_first;
   uint32_t block = blockIdx.x;
   if (a.n_zero) {
@@ -520,21 +587,26 @@ embedding_reduce_kernel(RedArgs a) {
       return;
     }
   }
-  const int L = a.L, l = threadIdx.x & (L - 1), part = threadIdx.x / L, parts = kRedThreads / L;
+  const int L = a.L, l = threadIdx.x & (L - 1), part = threadIdx.x / L, parts = kRedThreads / L, span = kEach * L;
   const uint32_t piece = block / a.slices;
-  const int slice = (int)(block - piece * a.slices), c = first_col<kVec>(slice * 8 * L, l);
+  const int slice = (int)(block - piece * a.slices);
+  const Lane<kDyF32, kDwF32, kVec> lane(a, slice, l);
   const int len = parts * a.per_part;
   const int64_t p0 = (int64_t)piece * len;
   for (int i = threadIdx.x; i < 2 * parts; i += kRedThreads) open_key[i & 1][i >> 1] = a.V;
   if (l == 0) through[part] = 0;
   pdl_wait();
   int live = 0;      // the padding lies behind the last run
-  for (int i0 = 0; i0 < len + 2; i0 += kRedThreads) {
+  for (int i0 = 0; i0 < len + 1; i0 += kRedThreads) {
     const int i = i0 + threadIdx.x;
     const int64_t g = p0 + i - 1;
     uint2 e = make_uint2(a.V, 0u);
-    if (i < len + 2 && g >= 0 && g < a.T) e = __ldcg(a.list + g);
-    if (i < len + 2) list[i] = e;
+    if (i < len + 1 && g >= 0 && g < a.T) {
+      e = __ldcg(a.list + g);
+      const uint32_t next = g + 1 < a.T ? __ldcg(&a.list[g + 1].x) : a.V;
+      if (next != e.x) e.y |= kEnds;
+    }
+    if (i < len + 1) list[i] = e;
     live += __syncthreads_count(i >= 1 && i <= len && e.x < a.V);
   }
   const uint2 *mine = list + 1 + part * a.per_part;
@@ -542,58 +614,58 @@ embedding_reduce_kernel(RedArgs a) {
   n = n < 0 ? 0 : n > a.per_part ? a.per_part : n;
   if (n > 0) {
     const uint32_t prev = mine[-1].x;
-    Row8<kDyF32, kVec> x[kAhead] = {};
-    Row8<kDwF32, kVec> old[kOldAhead] = {};
-    auto fetch = [&](Row8<kDyF32, kVec> &r, int j) {
-      load_row<kDyF32, kVec>(r, row_ptr<kDyF32>(a.dy, mine[j < n ? j : 0].y, a.dy_ld), c, L, a.D, j < n);
+    uint2 ent[kStep];
+    Row<kDyF32, kVec> x[kAhead] = {};
+    Row<kDwF32, kVec> old[kOldAhead] = {};
+    auto fetch = [&](Row<kDyF32, kVec> &r, uint2 e, int j) {
+      r.load(lane.dy_row(a, e.y & ~kEnds), lane.cols, L, j < n);
     };
-    auto fetch_old = [&](Row8<kDwF32, kVec> &r, int j) {
-      const int i = j < n ? j : 0;
-      const uint32_t k = mine[i].x;
-      load_row<kDwF32, kVec>(r, row_ptr<kDwF32>(a.dw, k, a.dw_ld), c, L, a.D,
-                             a.add && j < n && mine[i + 1].x != k && k != prev);
+    auto fetch_old = [&](Row<kDwF32, kVec> &r, uint2 e, int j) {
+      r.load(lane.dw_row(a, e.x), lane.cols, L, j < n && (e.y & kEnds) && e.x != prev);
     };
 #pragma unroll
-    for (int b = 0; b < kAhead; ++b) fetch(x[b], b);
+    for (int b = 0; b < kStep; ++b) ent[b] = mine[b < n ? b : 0];
 #pragma unroll
-    for (int b = 0; b < kOldAhead; ++b) fetch_old(old[b], b);
-    float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    for (int j0 = 0; j0 < n; j0 += kAhead) {
+    for (int b = 0; b < kAhead; ++b) fetch(x[b], ent[b], b);
+    if (a.add) {
 #pragma unroll
-      for (int b = 0; b < kAhead; ++b) {
+      for (int b = 0; b < kOldAhead; ++b) fetch_old(old[b], ent[b], b);
+    }
+    Sum<kVec> acc;
+    acc.clear();
+    for (int j0 = 0; j0 < n; j0 += kStep) {
+#pragma unroll
+      for (int b = 0; b < kStep; ++b) {
         const int j = j0 + b;
         if (j >= n) break;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) acc[e] = __fadd_rn(acc[e], elem(x[b], e));
-        fetch(x[b], j + kAhead);
-        const uint32_t k = mine[j].x;
-        const bool ends = mine[j + 1].x != k;
+        x[b % kAhead].add_to(acc);
+        const uint2 e = ent[b];
+        ent[b] = mine[j + kStep < n ? j + kStep : 0];
+        fetch(x[b % kAhead], ent[(b + kAhead) % kStep], j + kAhead);
+        const bool ends = (e.y & kEnds) != 0u;
         if (ends || j + 1 == n) {
-          if (ends && k != prev) {
-            finish_row<kDwF32, kVec>(a, row_ptr<kDwF32>(a.dw, k, a.dw_ld), c, acc, old[b % kOldAhead]);
+          if (ends && e.x != prev) {
+            lane.finish(a, e.x, acc, old[b % kOldAhead]);
           } else {
-            const int s = k == prev ? 0 : 1;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) open_sum[s][part * 8 * L + e * L + l] = acc[e];
+            const int s = e.x == prev ? 0 : 1;
+            acc.put(open_sum[s] + part * span + l, L);
             if (l == 0) {
-              open_key[s][part] = k;
+              open_key[s][part] = e.x;
               if (s == 0 && !ends) through[part] = 1;
             }
           }
-#pragma unroll
-          for (int e = 0; e < 8; ++e) acc[e] = 0.f;
+          acc.clear();
         }
-        fetch_old(old[b % kOldAhead], j + kOldAhead);
+        if (a.add) fetch_old(old[b % kOldAhead], ent[(b + kOldAhead) % kStep], j + kOldAhead);
       }
     }
   }
   __syncthreads();
-  // [piece][slice][8 * L]: the sum of the run that is open at the piece's end, over this piece
-  float *partial = a.partial + slice * (8 * L) + l;
-  const int64_t pitch = (int64_t)a.slices * 8 * L;
-  auto publish = [&](const float (&sum)[8]) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) partial[piece * pitch + e * L] = sum[e];
+  // [piece][slice][span]: the sum of the run that is open at the piece's end, over this piece
+  float *partial = a.partial + (int64_t)slice * span + l;
+  const int64_t pitch = (int64_t)a.slices * span;
+  auto publish = [&](const Sum<kVec> &sum) {
+    sum.put(partial + piece * pitch, L);
     __syncwarp(L == 32 ? 0xFFFFFFFFu : ((1u << L) - 1u) << (threadIdx.x & 31 & ~(L - 1)));
     if (l == 0) {
       __threadfence();
@@ -604,16 +676,14 @@ embedding_reduce_kernel(RedArgs a) {
   // the run this part starts and leaves open
   const uint32_t ko = open_key[1][part];
   if (ko != a.V) {
-    float sum[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) sum[e] = open_sum[1][part * 8 * L + e * L + l];
+    Sum<kVec> sum;
+    sum.set(open_sum[1] + part * span + l, L);
     bool open = true;
     for (int q = part + 1; q < parts && open; ++q) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) sum[e] = __fadd_rn(sum[e], open_sum[0][q * 8 * L + e * L + l]);
+      sum.add(open_sum[0] + q * span + l, L);
       open = through[q];
     }
-    if (!open) flush_row<kDwF32, kVec>(a, ko, c, sum);
+    if (!open) lane.flush(a, ko, sum);
     else publish(sum);
   }
   // the run that was open before the piece
@@ -621,14 +691,10 @@ embedding_reduce_kernel(RedArgs a) {
   if (kb == a.V) return;
   int n_through = 0;
   while (n_through < parts && through[n_through]) ++n_through;
-  float own[8];
+  Sum<kVec> own;
   if (part == 0) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) own[e] = open_sum[0][e * L + l];
-    for (int q = 1; q <= n_through && q < parts; ++q) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) own[e] = __fadd_rn(own[e], open_sum[0][q * 8 * L + e * L + l]);
-    }
+    own.set(open_sum[0] + l, L);
+    for (int q = 1; q <= n_through && q < parts; ++q) own.add(open_sum[0] + q * span + l, L);
     if (n_through == parts) publish(own);
   }
   if (n_through == parts) return;
@@ -662,24 +728,22 @@ embedding_reduce_kernel(RedArgs a) {
     return;
   }
   // group i adds the sums of every parts-th piece from the i-th, group 0 then the groups' sums
-  float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
+  Sum<kVec> acc;
+  acc.clear();
   for (uint32_t q = first + part; q < piece; q += parts) {
+    float t[kEach];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) acc[e] = __fadd_rn(acc[e], __ldcg(partial + q * pitch + e * L));
+    for (int k = 0; k < kEach; ++k) t[k] = __ldcg(partial + q * pitch + k * L);
+#pragma unroll
+    for (int i = 0; i < kEach / 2; ++i) acc.add_pair(i, t[2 * i], t[2 * i + 1]);
   }
-  float *sums = open_sum[1];
-#pragma unroll
-  for (int e = 0; e < 8; ++e) sums[part * 8 * L + e * L + l] = acc[e];
+  acc.put(open_sum[1] + part * span + l, L);
   __syncthreads();
   if (part != 0) return;
-  for (int w = 1; w < parts && (uint32_t)w < piece - first; ++w) {
+  for (int w = 1; w < parts && (uint32_t)w < piece - first; ++w) acc.add(open_sum[1] + w * span + l, L);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) acc[e] = __fadd_rn(acc[e], sums[w * 8 * L + e * L + l]);
-  }
-#pragma unroll
-  for (int e = 0; e < 8; ++e) acc[e] = __fadd_rn(acc[e], own[e]);
-  flush_row<kDwF32, kVec>(a, kb, c, acc);
+  for (int i = 0; i < kEach / 2; ++i) acc.add_pair(i, own.get(2 * i), own.get(2 * i + 1));
+  lane.flush(a, kb, acc);
 }
 
 // ------------------------------------------------------------------ few tokens
@@ -719,17 +783,17 @@ embedding_small_kernel(RedArgs a, const void *__restrict__ ids, int ids64, int64
   const int64_t u = (int64_t)blockIdx.x * (kRedThreads / L) + threadIdx.x / L;
   const int64_t t0 = u / a.slices;
   if (t0 >= T || !head[t0]) return;
-  const int c = first_col<kVec>((int)(u - t0 * a.slices) * 8 * L, l);
-  void *row = row_ptr<kDwF32>(a.dw, key[t0], a.dw_ld);
-  Row8<kDwF32, kVec> old = {};
-  load_row<kDwF32, kVec>(old, row, c, L, a.D, a.add);
-  float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  const Lane<kDyF32, kDwF32, kVec> lane(a, (int)(u - t0 * a.slices), l);
+  Row<kDwF32, kVec> old = {};
+  old.load(lane.dw_row(a, key[t0]), lane.cols, L, a.add);
+  Sum<kVec> acc;
+  acc.clear();
   for (int t = (int)t0; t >= 0;) {
-    Row8<kDyF32, kVec> x[kBatch] = {};
+    Row<kDyF32, kVec> x[kBatch] = {};
     int m = 0;
 #pragma unroll
     for (int b = 0; b < kBatch; ++b) {
-      load_row<kDyF32, kVec>(x[b], row_ptr<kDyF32>(a.dy, t < 0 ? 0 : t, a.dy_ld), c, L, a.D, t >= 0);
+      x[b].load(lane.dy_row(a, t < 0 ? 0 : t), lane.cols, L, t >= 0);
       if (t >= 0) {
         t = link[t];
         m = b + 1;
@@ -737,12 +801,9 @@ embedding_small_kernel(RedArgs a, const void *__restrict__ ids, int ids64, int64
     }
 #pragma unroll
     for (int b = 0; b < kBatch; ++b)
-      if (b < m) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) acc[e] = __fadd_rn(acc[e], elem(x[b], e));
-      }
+      if (b < m) x[b].add_to(acc);
   }
-  finish_row<kDwF32, kVec>(a, row, c, acc, old);
+  lane.finish(a, key[t0], acc, old);
 }
 
 // ------------------------------------------------------------------ host side
@@ -754,23 +815,26 @@ constexpr uint64_t kAheadBytes = 64 << 20;   // of dy into L2 beside the sort
 constexpr int64_t kFullGrid = 888;       // CTAs the reduction should have at least
 
 struct Shape {
-  int L, slices, per_part;
+  int L, slices, per_part, span;      // span: columns of a slice
   int64_t pieces, max_pieces;
 };
 
-Shape shape_of(int64_t T, int64_t D) {
+Shape shape_of(int64_t T, int64_t D, bool vec) {
+  const int each = vec ? Cols<true>::kEach : Cols<false>::kEach;
   Shape s;
   s.L = 1;
-  while (s.L < 32 && s.L * 8 < D) s.L *= 2;
-  s.slices = (int)((D + s.L * 8 - 1) / (s.L * 8));
+  while (s.L < 32 && s.L * each < D) s.L *= 2;
+  s.span = s.L * each;
+  s.slices = (int)((D + s.span - 1) / s.span);
   // parts as long as leaves enough of them to fill the GPU
   const int64_t parts_per_cta = kRedThreads / s.L;
   s.per_part = kMaxPiece / parts_per_cta < kMaxPart ? (int)(kMaxPiece / parts_per_cta) : kMaxPart;
-  while (s.per_part > kMinPart && (T / (parts_per_cta * s.per_part)) * s.slices < kFullGrid) s.per_part /= 2;
+  const int least = s.per_part < kMinPart ? s.per_part : kMinPart;
+  while (s.per_part > least && (T / (parts_per_cta * s.per_part)) * s.slices < kFullGrid) s.per_part /= 2;
   s.pieces = (T + parts_per_cta * s.per_part - 1) / (parts_per_cta * s.per_part);
   // most pieces any smaller T has: the workspace for T serves every smaller T
   const int64_t most = 2 * (kFullGrid / s.slices) + 4;
-  const int64_t finest = (T + parts_per_cta * kMinPart - 1) / (parts_per_cta * kMinPart);
+  const int64_t finest = (T + parts_per_cta * least - 1) / (parts_per_cta * least);
   const int64_t bound = most < finest ? most : finest;
   s.max_pieces = s.pieces > bound ? s.pieces : bound;
   return s;
@@ -782,24 +846,30 @@ struct Workspace {
 };
 
 Workspace workspace_of(int64_t T, int64_t V, int64_t D) {
-  const Shape s = shape_of(T, D);
   auto up = [](size_t x) { return (x + 255) / 256 * 256; };
+  size_t flags = 0, partial = 0;       // whether rows are vectors is not known yet
+  for (bool vec : {false, true}) {
+    const Shape s = shape_of(T, D, vec);
+    flags = std::max(flags, (size_t)s.max_pieces * s.slices);
+    partial = std::max(partial, (size_t)s.max_pieces * s.slices * s.span * sizeof(float));
+  }
   Workspace w;
   size_t at = 0;
   for (int i = 0; i < 2; ++i) {
     w.list[i] = at;
     at += up((size_t)T * sizeof(uint2));
   }
-  w.n_flags = (uint32_t)(s.max_pieces * s.slices);
+  w.n_flags = (uint32_t)flags;
   w.n_named = (uint32_t)((V + 31) / 32);
   w.clear = at;
   at += up(((size_t)w.n_flags + w.n_named) * 4);
   w.partial = at;
-  at += up((size_t)s.max_pieces * s.slices * 8 * s.L * 4);
+  at += up(partial);
   w.total = at;
   return w;
 }
 
+constexpr int64_t kMaxLd = 1 << 29;          // row strides in bytes stay below 2^32
 constexpr int64_t kMaxT = 0x7FFFFFFF - 1024, kMaxV = 0x7FFFFFFE, kMaxD = 1 << 24;
 
 int check_sizes(int64_t T, int64_t V, int64_t D) {
@@ -852,7 +922,8 @@ uint32_t sort_cluster(int device) {
 }
 
 bool rows_are_vectors(const void *p, int64_t ld, int f32, int64_t D) {
-  return ((uintptr_t)p & 15) == 0 && D % 8 == 0 && (ld * (f32 ? 4 : 2)) % 16 == 0;
+  const int64_t align = f32 ? 32 : 16;       // of eight elements
+  return (uintptr_t)p % align == 0 && D % 8 == 0 && ld % 8 == 0;
 }
 
 }  // namespace
@@ -872,7 +943,8 @@ int anc_embedding_lookup(anc_ctx *ctx, const void *table, int table_dtype, int64
   ANC_REQUIRE(table && ids && out, "NULL argument");
   if (table_ld == 0) table_ld = D;
   if (out_ld == 0) out_ld = D;
-  ANC_REQUIRE(table_ld >= D && out_ld >= D, "row strides must be at least the row length");
+  ANC_REQUIRE(table_ld >= D && out_ld >= D && table_ld <= kMaxLd && out_ld <= kMaxLd,
+              "row strides must be at least the row length and at most 2^29");
   const int tf = table_dtype == ANC_GRAD_F32, of = out_dtype == ANC_GRAD_F32, i64 = ids_dtype == ANC_IDS_I64;
   ANC_REQUIRE(((uintptr_t)table & (tf ? 3 : 1)) == 0 && ((uintptr_t)out & (of ? 3 : 1)) == 0 &&
                   ((uintptr_t)ids & (i64 ? 7 : 3)) == 0,
@@ -921,7 +993,8 @@ int anc_embedding_grad(anc_ctx *ctx, const void *dy, int dy_dtype, int64_t dy_ld
   ANC_REQUIRE(mode == ANC_EMBED_WRITE || mode == ANC_EMBED_ADD, "bad mode %d", mode);
   if (dy_ld == 0) dy_ld = D;
   if (dw_ld == 0) dw_ld = D;
-  ANC_REQUIRE(dy_ld >= D && dw_ld >= D, "row strides must be at least the row length");
+  ANC_REQUIRE(dy_ld >= D && dw_ld >= D && dy_ld <= kMaxLd && dw_ld <= kMaxLd,
+              "row strides must be at least the row length and at most 2^29");
   const int yf = dy_dtype == ANC_GRAD_F32, wf = dw_dtype == ANC_GRAD_F32, i64 = ids_dtype == ANC_IDS_I64;
   ANC_REQUIRE(((uintptr_t)dw & (wf ? 3 : 1)) == 0, "dw not aligned to its element size");
   if (T > 0) {
@@ -966,9 +1039,11 @@ int anc_embedding_grad(anc_ctx *ctx, const void *dy, int dy_dtype, int64_t dy_ld
   if (write && small) ANC_CUDA(launch_side(V, 0, 0));
   if (T == 0) return ANC_OK;
   uint8_t *wp = (uint8_t *)work;
-  const Shape sh = shape_of(T, D);
+  const bool vec = rows_are_vectors(dy, dy_ld, yf, D) && rows_are_vectors(dw, dw_ld, wf, D);
+  const Shape sh = shape_of(T, D, vec);
   RedArgs ra = {};
-  ra.dy = dy; ra.dw = dw; ra.dy_ld = dy_ld; ra.dw_ld = dw_ld; ra.T = T;
+  ra.dy = (const uint8_t *)dy; ra.dw = (uint8_t *)dw; ra.T = T;
+  ra.dy_pitch = (uint32_t)(dy_ld * (yf ? 4 : 2)); ra.dw_pitch = (uint32_t)(dw_ld * (wf ? 4 : 2));
   ra.partial = (float *)(wp + ws.partial);
   ra.V = (uint32_t)V; ra.D = (int)D; ra.slices = sh.slices; ra.L = sh.L; ra.per_part = sh.per_part; ra.scale = scale;
   ra.add = !write;
@@ -1032,7 +1107,6 @@ int anc_embedding_grad(anc_ctx *ctx, const void *dy, int dy_dtype, int64_t dy_ld
   cfg.stream = st;
   cfg.attrs = pdl;
   cfg.numAttrs = n_attrs;
-  const bool vec = rows_are_vectors(dy, dy_ld, yf, D) && rows_are_vectors(dw, dw_ld, wf, D);
 #define ANC_REDUCE(Y, W, VEC)                                                                        \
   do {                                                                                               \
     if (small)                                                                                       \
