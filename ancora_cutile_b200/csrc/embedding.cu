@@ -15,6 +15,7 @@
 #include <algorithm>
 #include <cuda_bf16.h>
 #include <initializer_list>
+#include <type_traits>
 #include <mutex>
 #include "anc_internal.h"
 #include "philox.cuh"
@@ -194,9 +195,8 @@ struct SortArgs {
   int64_t V, padding_idx;
   uint2 *list[2];                // (id, token)
   int passes;
-  uint32_t *clear;               // words to clear: flags of the reduction, then the bitmap of named rows
+  uint32_t *clear;               // words to clear: flags of the sums
   uint32_t n_clear;
-  uint32_t *named;               // bitmap of the rows some token names (nullptr: not wanted)
   uint32_t *status;
 };
 
@@ -286,11 +286,6 @@ embedding_sort_kernel(SortArgs a, uint32_t n_ctas) {
       if (on) {
         if (single && !last) sh.list[dst] = e;
         else out[dst] = e;
-      }
-      if (last && a.named) {
-        const uint32_t before = __shfl_up_sync(0xFFFFFFFFu, e.x, 1);
-        if (on && e.x < (uint32_t)a.V && (lane == 0 || before != e.x))
-          atomicOr(a.named + (e.x >> 5), 1u << (e.x & 31));
       }
     };
     for (uint32_t d = lane * 4; d < kDigits; d += 128) *reinterpret_cast<uint4 *>(mine + d) = make_uint4(0u, 0u, 0u, 0u);
@@ -394,18 +389,21 @@ struct ZeroArgs {
   int vec;                       // rows are 16-byte aligned vectors
 };
 
-// zeros in rows [first, last) but those of the bitmap, by the threads of one block
-__device__ __forceinline__ void zero_rows(const ZeroArgs &z, int64_t first, int64_t last, const uint32_t *named) {
+// zeros in rows [first, last) by the threads of one block
+__device__ __forceinline__ void zero_rows(const ZeroArgs &z, int64_t first, int64_t last) {
   const uint32_t per = (uint32_t)(z.vec ? z.row_bytes / 16 : z.row_bytes / 2);
   const int64_t n = (last - first) * per;
+  if (z.vec && z.pitch == z.row_bytes) {
+    uint4 *p = reinterpret_cast<uint4 *>(z.dw + first * z.pitch);
+    for (int64_t i = threadIdx.x; i < n; i += blockDim.x) p[i] = make_uint4(0u, 0u, 0u, 0u);
+    return;
+  }
   for (int64_t i0 = 0; i0 < n; i0 += (int64_t)1 << 30) {      // 32-bit division inside
     const int64_t row0 = first + i0 / per;
     const uint32_t rem = (uint32_t)(i0 % per), m = (uint32_t)(n - i0 < ((int64_t)1 << 30) ? n - i0 : (int64_t)1 << 30);
     for (uint32_t i = threadIdx.x; i < m; i += blockDim.x) {
       const uint32_t r = (rem + i) / per, c = rem + i - r * per;
-      const int64_t row = row0 + r;
-      if (named && ((named[row >> 5] >> (row & 31)) & 1u)) continue;
-      uint8_t *p = z.dw + row * z.pitch;
+      uint8_t *p = z.dw + (row0 + r) * z.pitch;
       if (z.vec) *reinterpret_cast<uint4 *>(p + (int64_t)c * 16) = make_uint4(0u, 0u, 0u, 0u);
       else *reinterpret_cast<uint16_t *>(p + (int64_t)c * 2) = 0;
     }
@@ -415,14 +413,14 @@ __device__ __forceinline__ void zero_rows(const ZeroArgs &z, int64_t first, int6
 constexpr int kSideThreads = 256;
 constexpr uint32_t kPrefetchBytes = 8192;      // per instruction
 
-// What the SMs that do not sort do meanwhile: zeros in the first rows of the table (write), or the first
-// rows of dy into L2 (add).  Launched behind the sort without waiting for it; it waits for the sort only
+// What the SMs that do not sort do meanwhile: zeros in the table when all of it is written, and the first
+// rows of dy into L2.  Launched behind the sort without waiting for it; it waits for the sort only
 // before it ends, so that whoever waits for this kernel has the sorted list too.
 __global__ void __launch_bounds__(kSideThreads)
 embedding_side_kernel(ZeroArgs z, int64_t rows_per_block, const uint8_t *ahead, uint64_t ahead_bytes) {
   pdl_trigger();
   const int64_t first = blockIdx.x * rows_per_block, last = first + rows_per_block < z.V ? first + rows_per_block : z.V;
-  if (first < last) zero_rows(z, first, last, nullptr);
+  if (first < last) zero_rows(z, first, last);
   const uint64_t step = (uint64_t)gridDim.x * kPrefetchBytes;
   if (threadIdx.x == 0)
     for (uint64_t o = (uint64_t)blockIdx.x * kPrefetchBytes; o < ahead_bytes; o += step) {
@@ -450,12 +448,8 @@ struct RedArgs {
   int per_part;                  // sorted places per group of L lanes
   float scale;
   int add;
-  uint32_t n_red, n_zero;        // blocks that add up runs, blocks that write zeros
   uint32_t *flags;               // [piece][slice]: the partial sum of the run open at the piece's end is there
   uint32_t *status;
-  ZeroArgs z;                    // zeros in rows from z_first on that `named` does not hold
-  int64_t z_first, z_per_block;
-  const uint32_t *named;
 };
 
 // A lane's columns of a slice: sixteen in two octets, all lanes' first octets before their second ones, or
@@ -559,37 +553,44 @@ struct Lane {
 // before it (blocks start in index order, and a block raises its flag before it waits for anything; the
 // wait is bounded) and adds their sums in order.
 //
-// Bound by memory latency unless enough rows are in flight: a group always has the rows of the next kAhead
-// places on the way and, with "add", the old table rows of the runs that end among the next kOldAhead.
-//
-// When the whole table is written, blocks that write zeros into the rows no token names are dealt evenly
-// among the others, so that the two kinds of traffic overlap.
-template <bool kDyF32, bool kDwF32, bool kVec>
+// Bound by memory latency unless enough rows are in flight.  Rows that are vectors go through a ring in
+// shared memory: every warp has asynchronous copies of the rows of the next kDepth places on the way and,
+// with "add", of the old table rows of the runs that end there (12 KB per warp, 192 KB per SM).  Loads ahead into
+// registers did not get there: they share six scoreboards, so waiting for one row waited for the newest
+// one too (accumulating 65536 rows of 1024: REDNOTE).
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, bool on) {
+  asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.u32 q, %2, 0;\n\t@q cp.async.cg.shared.global [%0], [%1], 16;\n\t}" ::"r"(dst),
+               "l"(src), "r"((uint32_t)on)
+               : "memory");
+}
+
+template <bool kDyF32, bool kDwF32, bool kVec, bool kAdd>
+struct Stage {
+  static constexpr int kCols = 32 * Cols<true>::kEach;                  // columns a warp holds
+  static constexpr int kDy = kCols * (kDyF32 ? 4 : 2), kOld = kAdd ? kCols * (kDwF32 ? 4 : 2) : 0;
+  static constexpr int kDepth = 12288 / (kDy + kOld) < 8 ? 12288 / (kDy + kOld) : 8;
+  static constexpr uint32_t kWarp = kDepth * (kDy + kOld);
+  // afterwards the same memory holds the open sums of all parts
+  static constexpr uint32_t kRing = kRedThreads / 32 * kWarp, kOpen = 2 * kRedThreads * Cols<kVec>::kEach * 4;
+  static constexpr uint32_t kBytes = kVec && kRing > kOpen ? kRing : kOpen;
+};
+
+template <bool kDyF32, bool kDwF32, bool kVec, bool kAdd>
 __global__ void __launch_bounds__(kRedThreads, 2)
 embedding_reduce_kernel(RedArgs a) {
-  constexpr int kEach = Cols<kVec>::kEach, kStep = 4;
-  constexpr int kAhead = (kDyF32 && kVec) ? 2 : 4, kOldAhead = (kDwF32 && kVec) ? 2 : 4;
+  using St = Stage<kDyF32, kDwF32, kVec, kAdd>;
+  constexpr int kEach = Cols<kVec>::kEach;
   constexpr uint32_t kEnds = 0x80000000u;             // in a token number: the run ends here
-  __shared__ float open_sum[2][kRedThreads * kEach];  // [slot][part][kEach * L]
+  extern __shared__ __align__(128) uint8_t stage_smem[];
   __shared__ uint32_t open_key[2][kRedThreads];       // V: nothing open
   __shared__ uint8_t through[kRedThreads];            // the part is one run, open at both ends (slot 0)
   __shared__ uint2 list[kMaxPiece + 1];               // the place before the piece, the piece's places
   __shared__ uint32_t s_first;
-  uint32_t block = blockIdx.x;
-  if (a.n_zero) {
-    const uint64_t total = (uint64_t)a.n_red + a.n_zero;
-    block = (uint32_t)((uint64_t)blockIdx.x * a.n_red / total);
-    if ((uint32_t)((blockIdx.x + 1ull) * a.n_red / total) == block) {
-      pdl_wait();
-      const int64_t first = a.z_first + (int64_t)(blockIdx.x - block) * a.z_per_block;
-      const int64_t last = first + a.z_per_block < a.z.V ? first + a.z_per_block : a.z.V;
-      if (first < last) zero_rows(a.z, first, last, a.named);
-      return;
-    }
-  }
   const int L = a.L, l = threadIdx.x & (L - 1), part = threadIdx.x / L, parts = kRedThreads / L, span = kEach * L;
-  const uint32_t piece = block / a.slices;
-  const int slice = (int)(block - piece * a.slices);
+  float *const open_head = reinterpret_cast<float *>(stage_smem);      // [part][span], after the loop: the run open at
+  float *const open_tail = open_head + kRedThreads * kEach;            // the part's start, and at its end only
+  const uint32_t piece = blockIdx.x / a.slices;
+  const int slice = (int)(blockIdx.x - piece * a.slices);
   const Lane<kDyF32, kDwF32, kVec> lane(a, slice, l);
   const int len = parts * a.per_part;
   const int64_t p0 = (int64_t)piece * len;
@@ -612,52 +613,122 @@ embedding_reduce_kernel(RedArgs a) {
   const uint2 *mine = list + 1 + part * a.per_part;
   int n = live - part * a.per_part;
   n = n < 0 ? 0 : n > a.per_part ? a.per_part : n;
-  if (n > 0) {
-    const uint32_t prev = mine[-1].x;
-    uint2 ent[kStep];
-    Row<kDyF32, kVec> x[kAhead] = {};
-    Row<kDwF32, kVec> old[kOldAhead] = {};
-    auto fetch = [&](Row<kDyF32, kVec> &r, uint2 e, int j) {
-      r.load(lane.dy_row(a, e.y & ~kEnds), lane.cols, L, j < n);
-    };
-    auto fetch_old = [&](Row<kDwF32, kVec> &r, uint2 e, int j) {
-      r.load(lane.dw_row(a, e.x), lane.cols, L, j < n && (e.y & kEnds) && e.x != prev);
-    };
-#pragma unroll
-    for (int b = 0; b < kStep; ++b) ent[b] = mine[b < n ? b : 0];
-#pragma unroll
-    for (int b = 0; b < kAhead; ++b) fetch(x[b], ent[b], b);
-    if (a.add) {
-#pragma unroll
-      for (int b = 0; b < kOldAhead; ++b) fetch_old(old[b], ent[b], b);
+  const uint32_t prev = mine[-1].x;
+  Sum<kVec> acc, own;        // the run so far; the run from before the part (later: the piece), where it ends here
+  acc.clear();
+  own.clear();
+  bool has_own = false, open = false;
+  // the end of place e in its run, with acc holding the run's sum
+  auto end_run = [&](uint2 e, const Row<kDwF32, kVec> &old) {
+    if (e.x != prev) {
+      lane.finish(a, e.x, acc, old);
+    } else {
+      own = acc;
+      has_own = true;
     }
-    Sum<kVec> acc;
     acc.clear();
-    for (int j0 = 0; j0 < n; j0 += kStep) {
+    open = false;
+  };
+  if constexpr (kVec) {
+    constexpr int kYB = kDyF32 ? 4 : 2, kWB = kDwF32 ? 4 : 2, kYChunks = kEach * kYB / 16, kWChunks = kEach * kWB / 16;
+    const int c0 = slice * span, group = (threadIdx.x & 31) / L;
+    const uint32_t ring = (uint32_t)__cvta_generic_to_shared(stage_smem) + (threadIdx.x >> 5) * St::kWarp;
+    const uint8_t *ring_ptr = stage_smem + (threadIdx.x >> 5) * St::kWarp;
+    const uint8_t *dy = a.dy + (int64_t)c0 * kYB, *dw = a.dw + (int64_t)c0 * kWB;
+    const int y_bytes = (a.D - c0) * kYB, w_bytes = (a.D - c0) * kWB;
+    // chunk q of a row: 16 bytes per lane, the group's lanes side by side
+    auto fetch = [&](uint32_t slot, int j) {
+      const bool on = j < n;
+      const uint2 e = mine[on ? j : 0];
+      const uint8_t *src = dy + (uint64_t)(e.y & ~kEnds) * a.dy_pitch;
+      const uint32_t dst = ring + slot * (St::kDy + St::kOld) + group * (span * kYB);
 #pragma unroll
-      for (int b = 0; b < kStep; ++b) {
-        const int j = j0 + b;
-        if (j >= n) break;
-        x[b % kAhead].add_to(acc);
-        const uint2 e = ent[b];
-        ent[b] = mine[j + kStep < n ? j + kStep : 0];
-        fetch(x[b % kAhead], ent[(b + kAhead) % kStep], j + kAhead);
-        const bool ends = (e.y & kEnds) != 0u;
-        if (ends || j + 1 == n) {
-          if (ends && e.x != prev) {
-            lane.finish(a, e.x, acc, old[b % kOldAhead]);
-          } else {
-            const int s = e.x == prev ? 0 : 1;
-            acc.put(open_sum[s] + part * span + l, L);
-            if (l == 0) {
-              open_key[s][part] = e.x;
-              if (s == 0 && !ends) through[part] = 1;
-            }
-          }
-          acc.clear();
-        }
-        if (a.add) fetch_old(old[b % kOldAhead], ent[(b + kOldAhead) % kStep], j + kOldAhead);
+      for (int q = 0; q < kYChunks; ++q) {
+        const int o = (q * L + l) * 16;
+        cp_async16(dst + o, src + o, on && o < y_bytes);
       }
+      if constexpr (kAdd) {
+        const bool want = on && (e.y & kEnds) && e.x != prev;
+        const uint8_t *old = dw + (uint64_t)e.x * a.dw_pitch;
+        const uint32_t od = ring + slot * (St::kDy + St::kOld) + St::kDy + group * (span * kWB);
+#pragma unroll
+        for (int q = 0; q < kWChunks; ++q) {
+          const int o = (q * L + l) * 16;
+          cp_async16(od + o, old + o, want && o < w_bytes);
+        }
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    auto take = [&](auto &row, const uint8_t *p, auto f32) {      // this lane's octets of a staged row
+#pragma unroll
+      for (int q = 0; q < Cols<true>::kOcts; ++q) {
+        const uint4 *v = reinterpret_cast<const uint4 *>(p + (q * 8 * L + l * 8) * (f32.value ? 4 : 2));
+        const uint4 w = v[0];
+        row.o[q].w[0] = w.x; row.o[q].w[1] = w.y; row.o[q].w[2] = w.z; row.o[q].w[3] = w.w;
+        if constexpr (f32.value) {
+          const uint4 u = v[1];
+          row.o[q].w[4] = u.x; row.o[q].w[5] = u.y; row.o[q].w[6] = u.z; row.o[q].w[7] = u.w;
+        }
+      }
+    };
+    // all groups of a warp go round together, the longest sets the count
+    int rounds = n;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) rounds = max(rounds, __shfl_xor_sync(0xFFFFFFFFu, rounds, o));
+#pragma unroll
+    for (int d = 0; d < St::kDepth; ++d) fetch(d, d);
+    uint32_t slot = 0;
+    for (int j = 0; j < rounds; ++j) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(St::kDepth - 1) : "memory");
+      __syncwarp();
+      if (j < n) {
+        const uint8_t *st = ring_ptr + slot * (St::kDy + St::kOld);
+        const uint2 e = mine[j];
+        Row<kDyF32, kVec> x;
+        take(x, st + group * (span * kYB), std::integral_constant<bool, kDyF32>());
+        x.add_to(acc);
+        open = true;
+        if (e.y & kEnds) {
+          Row<kDwF32, kVec> old = {};
+          if (kAdd && e.x != prev) take(old, st + St::kDy + group * (span * kWB), std::integral_constant<bool, kDwF32>());
+          end_run(e, old);
+        }
+      }
+      __syncwarp();
+      fetch(slot, j + St::kDepth);
+      if (++slot == St::kDepth) slot = 0;
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+  } else {
+    constexpr int kAhead = 4;
+    for (int j0 = 0; j0 < n; j0 += kAhead) {
+      Row<kDyF32, kVec> x[kAhead] = {};
+      Row<kDwF32, kVec> old[kAhead] = {};
+#pragma unroll
+      for (int b = 0; b < kAhead; ++b) {
+        const uint2 e = mine[j0 + b < n ? j0 + b : 0];
+        x[b].load(lane.dy_row(a, e.y & ~kEnds), lane.cols, L, j0 + b < n);
+        if (kAdd) old[b].load(lane.dw_row(a, e.x), lane.cols, L, j0 + b < n && (e.y & kEnds) && e.x != prev);
+      }
+#pragma unroll
+      for (int b = 0; b < kAhead; ++b) {
+        if (j0 + b >= n) break;
+        const uint2 e = mine[j0 + b];
+        x[b].add_to(acc);
+        open = true;
+        if (e.y & kEnds) end_run(e, old[b]);
+      }
+    }
+  }
+  __syncthreads();
+  if (has_own) own.put(open_head + part * span + l, L);
+  if (open) acc.put((mine[n - 1].x == prev ? open_head : open_tail) + part * span + l, L);
+  if (l == 0) {
+    if (has_own) open_key[0][part] = prev;
+    if (open) {
+      const uint32_t k = mine[n - 1].x;
+      open_key[k == prev ? 0 : 1][part] = k;
+      if (k == prev) through[part] = 1;
     }
   }
   __syncthreads();
@@ -677,10 +748,10 @@ embedding_reduce_kernel(RedArgs a) {
   const uint32_t ko = open_key[1][part];
   if (ko != a.V) {
     Sum<kVec> sum;
-    sum.set(open_sum[1] + part * span + l, L);
+    sum.set(open_tail + part * span + l, L);
     bool open = true;
     for (int q = part + 1; q < parts && open; ++q) {
-      sum.add(open_sum[0] + q * span + l, L);
+      sum.add(open_head + q * span + l, L);
       open = through[q];
     }
     if (!open) lane.flush(a, ko, sum);
@@ -691,10 +762,9 @@ embedding_reduce_kernel(RedArgs a) {
   if (kb == a.V) return;
   int n_through = 0;
   while (n_through < parts && through[n_through]) ++n_through;
-  Sum<kVec> own;
   if (part == 0) {
-    own.set(open_sum[0] + l, L);
-    for (int q = 1; q <= n_through && q < parts; ++q) own.add(open_sum[0] + q * span + l, L);
+    own.set(open_head + l, L);
+    for (int q = 1; q <= n_through && q < parts; ++q) own.add(open_head + q * span + l, L);
     if (n_through == parts) publish(own);
   }
   if (n_through == parts) return;
@@ -728,7 +798,6 @@ embedding_reduce_kernel(RedArgs a) {
     return;
   }
   // group i adds the sums of every parts-th piece from the i-th, group 0 then the groups' sums
-  Sum<kVec> acc;
   acc.clear();
   for (uint32_t q = first + part; q < piece; q += parts) {
     float t[kEach];
@@ -737,10 +806,10 @@ embedding_reduce_kernel(RedArgs a) {
 #pragma unroll
     for (int i = 0; i < kEach / 2; ++i) acc.add_pair(i, t[2 * i], t[2 * i + 1]);
   }
-  acc.put(open_sum[1] + part * span + l, L);
+  acc.put(open_tail + part * span + l, L);
   __syncthreads();
   if (part != 0) return;
-  for (int w = 1; w < parts && (uint32_t)w < piece - first; ++w) acc.add(open_sum[1] + w * span + l, L);
+  for (int w = 1; w < parts && (uint32_t)w < piece - first; ++w) acc.add(open_tail + w * span + l, L);
 #pragma unroll
   for (int i = 0; i < kEach / 2; ++i) acc.add_pair(i, own.get(2 * i), own.get(2 * i + 1));
   lane.flush(a, kb, acc);
@@ -807,12 +876,11 @@ embedding_small_kernel(RedArgs a, const void *__restrict__ ids, int ids64, int64
 }
 
 // ------------------------------------------------------------------ host side
-constexpr int kMaxPart = 32, kMinPart = 4;
+constexpr int kMaxPart = 64, kMinPart = 4;
 constexpr int kSortTarget = 4;               // rounds of 32 keys per warp the sort aims at
 constexpr int64_t kZeroBytes = 128 << 10;    // zeros per block
-constexpr int64_t kSideBytes = 64 << 20;     // zeros beside the sort
 constexpr uint64_t kAheadBytes = 64 << 20;   // of dy into L2 beside the sort
-constexpr int64_t kFullGrid = 888;       // CTAs the reduction should have at least
+constexpr int64_t kFullGrid = 200;       // blocks the sums should have at least
 
 struct Shape {
   int L, slices, per_part, span;      // span: columns of a slice
@@ -842,10 +910,10 @@ Shape shape_of(int64_t T, int64_t D, bool vec) {
 
 struct Workspace {
   size_t list[2], clear, partial, total;
-  uint32_t n_flags, n_named;       // words at `clear`
+  uint32_t n_flags;                // words at `clear`
 };
 
-Workspace workspace_of(int64_t T, int64_t V, int64_t D) {
+Workspace workspace_of(int64_t T, int64_t D) {
   auto up = [](size_t x) { return (x + 255) / 256 * 256; };
   size_t flags = 0, partial = 0;       // whether rows are vectors is not known yet
   for (bool vec : {false, true}) {
@@ -860,12 +928,11 @@ Workspace workspace_of(int64_t T, int64_t V, int64_t D) {
     at += up((size_t)T * sizeof(uint2));
   }
   w.n_flags = (uint32_t)flags;
-  w.n_named = (uint32_t)((V + 31) / 32);
   w.clear = at;
-  at += up(((size_t)w.n_flags + w.n_named) * 4);
+  at += up((size_t)w.n_flags * 4);
   w.partial = at;
   at += up(partial);
-  w.total = at;
+  w.total = at ? at : 256;
   return w;
 }
 
@@ -884,7 +951,8 @@ int check_dtype(int d, const char *what) {
   return ANC_OK;
 }
 
-// Largest cluster the sort can use on a device (0: an error is set); asked once per device.
+// Largest cluster the sort can use on a device (0: an error is set), and the kernels' shared-memory limits;
+// once per device.
 uint32_t sort_cluster(int device) {
   static std::mutex mu;
   static uint32_t most[64] = {};
@@ -893,6 +961,19 @@ uint32_t sort_cluster(int device) {
   cudaError_t e = cudaFuncSetAttribute(embedding_sort_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
   if (e == cudaSuccess)
     e = cudaFuncSetAttribute(embedding_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(SortShared));
+#define ANC_REDUCE_SMEM(Y, W, ADD)                                                                         \
+  if (e == cudaSuccess)                                                                                    \
+  e = cudaFuncSetAttribute(embedding_reduce_kernel<Y, W, true, ADD>, cudaFuncAttributeMaxDynamicSharedMemorySize, \
+                           (int)Stage<Y, W, true, ADD>::kBytes)
+  ANC_REDUCE_SMEM(false, false, false);
+  ANC_REDUCE_SMEM(false, false, true);
+  ANC_REDUCE_SMEM(false, true, false);
+  ANC_REDUCE_SMEM(false, true, true);
+  ANC_REDUCE_SMEM(true, false, false);
+  ANC_REDUCE_SMEM(true, false, true);
+  ANC_REDUCE_SMEM(true, true, false);
+  ANC_REDUCE_SMEM(true, true, true);
+#undef ANC_REDUCE_SMEM
   uint32_t found = 8;                // the portable size
   for (uint32_t c = kMaxCluster; e == cudaSuccess && c > 8; c /= 2) {
     cudaLaunchConfig_t cfg = {};
@@ -914,7 +995,7 @@ uint32_t sort_cluster(int device) {
     cudaGetLastError();
   }
   if (e != cudaSuccess) {
-    anc_cuda_fail(e, "sort kernel attributes");
+    anc_cuda_fail(e, "embedding kernel attributes");
     return 0;
   }
   if (device >= 0 && device < 64) most[device] = found;
@@ -977,7 +1058,7 @@ int anc_embedding_grad_workspace(int64_t T, int64_t V, int64_t D, uint64_t *byte
   ANC_REQUIRE(bytes, "bytes is NULL");
   int rc = check_sizes(T, V, D);
   if (rc) return rc;
-  *bytes = workspace_of(T, V, D).total;
+  *bytes = workspace_of(T, D).total;
   return ANC_OK;
 }
 
@@ -1003,7 +1084,7 @@ int anc_embedding_grad(anc_ctx *ctx, const void *dy, int dy_dtype, int64_t dy_ld
                 "pointer not aligned to its element size");
     ANC_REQUIRE(((uintptr_t)work & 15) == 0, "workspace not aligned to 16 bytes");
   }
-  const Workspace ws = workspace_of(T, V, D);
+  const Workspace ws = workspace_of(T, D);
   ANC_REQUIRE(T == 0 || work_bytes >= ws.total, "workspace of %llu bytes, %llu are needed",
               (unsigned long long)work_bytes, (unsigned long long)ws.total);
   if (T == 0 && mode == ANC_EMBED_ADD) return ANC_OK;
@@ -1048,9 +1129,9 @@ int anc_embedding_grad(anc_ctx *ctx, const void *dy, int dy_dtype, int64_t dy_ld
   ra.V = (uint32_t)V; ra.D = (int)D; ra.slices = sh.slices; ra.L = sh.L; ra.per_part = sh.per_part; ra.scale = scale;
   ra.add = !write;
   ra.status = ctx->d_status;
-  const int64_t n_red = small ? (T * sh.slices + kRedThreads / sh.L - 1) / (kRedThreads / sh.L) : sh.pieces * sh.slices;
-  ANC_REQUIRE(n_red <= 0x3FFFFFFF, "T x D too large");
-  ra.n_red = (uint32_t)n_red;
+  const int64_t blocks =
+      small ? (T * sh.slices + kRedThreads / sh.L - 1) / (kRedThreads / sh.L) : sh.pieces * sh.slices;
+  ANC_REQUIRE(blocks <= 0x7FFFFFFF, "T x D too large");
   int n_attrs = write ? 1 : 0;
   if (!small) {
     SortArgs sa = {};
@@ -1060,22 +1141,9 @@ int anc_embedding_grad(anc_ctx *ctx, const void *dy, int dy_dtype, int64_t dy_ld
     while (((uint64_t)V >> bits) != 0) ++bits;
     sa.passes = (bits + kDigitBits - 1) / kDigitBits;
     sa.status = ctx->d_status;
-    // rows the side launch zeroes while the sort runs; the rest is the reduction's, named rows left out
-    const int64_t side_rows = !write ? 0 : za.row_bytes * V <= kSideBytes ? V : kSideBytes / za.row_bytes;
     sa.clear = (uint32_t *)(wp + ws.clear);
+    sa.n_clear = (uint32_t)blocks;
     ra.flags = sa.clear;
-    sa.n_clear = (uint32_t)(sh.pieces * sh.slices);
-    if (side_rows < V && write) {
-      sa.named = sa.clear + ws.n_flags;
-      sa.n_clear = ws.n_flags + ws.n_named;
-      ra.named = sa.named;
-      ra.z = za;
-      ra.z_first = side_rows;
-      ra.z_per_block = za.row_bytes < kZeroBytes ? kZeroBytes / za.row_bytes : 1;
-      const int64_t n_zero = (V - side_rows + ra.z_per_block - 1) / ra.z_per_block;
-      ANC_REQUIRE(n_zero <= 0x3FFFFFFF, "table too large");
-      ra.n_zero = (uint32_t)n_zero;
-    }
     ra.list = sa.list[(sa.passes - 1) & 1];
     const uint32_t most = sort_cluster(ctx->device);
     if (!most) return ANC_E_CUDA;
@@ -1094,25 +1162,31 @@ int anc_embedding_grad(anc_ctx *ctx, const void *dy, int dy_dtype, int64_t dy_ld
     cfg.attrs = at;
     cfg.numAttrs = 1;
     ANC_CUDA(cudaLaunchKernelEx(&cfg, embedding_sort_kernel, sa, n_ctas));
-    // with "add", as much of dy as the sort's time can bring in and L2 can hold
     const uint64_t dy_bytes = ((uint64_t)(T - 1) * dy_ld + D) * (yf ? 4 : 2) / 16 * 16;
-    const uint64_t ahead = write || dy_bytes < 64 ? 0 : dy_bytes - 16 < kAheadBytes ? dy_bytes - 16 : kAheadBytes;
-    if (side_rows || ahead) ANC_CUDA(launch_side(side_rows, ahead, 1));
+    const uint64_t ahead = dy_bytes < 64 ? 0 : dy_bytes - 16 < kAheadBytes ? dy_bytes - 16 : kAheadBytes;
+    if (write || ahead) ANC_CUDA(launch_side(write ? V : 0, ahead, 1));
     n_attrs = 1;
   }
   // these launches start while their predecessor drains and wait for it on the device
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(ra.n_red + ra.n_zero);
+  cfg.gridDim = dim3((unsigned)blocks);
   cfg.blockDim = dim3(kRedThreads);
   cfg.stream = st;
   cfg.attrs = pdl;
   cfg.numAttrs = n_attrs;
+#define ANC_REDUCE_A(Y, W, VEC, ADD)                                                                 \
+  do {                                                                                               \
+    cfg.dynamicSmemBytes = Stage<Y, W, VEC, ADD>::kBytes;                                            \
+    ANC_CUDA(cudaLaunchKernelEx(&cfg, embedding_reduce_kernel<Y, W, VEC, ADD>, ra));                 \
+  } while (0)
 #define ANC_REDUCE(Y, W, VEC)                                                                        \
   do {                                                                                               \
     if (small)                                                                                       \
       ANC_CUDA(cudaLaunchKernelEx(&cfg, embedding_small_kernel<Y, W, VEC>, ra, ids, i64, padding_idx, ctx->d_status)); \
+    else if (write)                                                                                  \
+      ANC_REDUCE_A(Y, W, VEC, false);                                                                \
     else                                                                                             \
-      ANC_CUDA(cudaLaunchKernelEx(&cfg, embedding_reduce_kernel<Y, W, VEC>, ra));                    \
+      ANC_REDUCE_A(Y, W, VEC, true);                                                                 \
   } while (0)
 #define ANC_REDUCE_V(Y, W)                \
   do {                                    \
@@ -1125,6 +1199,7 @@ int anc_embedding_grad(anc_ctx *ctx, const void *dy, int dy_dtype, int64_t dy_ld
   else ANC_REDUCE_V(false, false);
 #undef ANC_REDUCE_V
 #undef ANC_REDUCE
+#undef ANC_REDUCE_A
   ANC_CUDA(cudaGetLastError());
   return ANC_OK;
 }
