@@ -161,7 +161,8 @@ embedding_lookup_kernel(const void *__restrict__ table, int64_t table_ld, const 
 // writes its stretch to the places the counts give.  Padding sorts behind the last row of the table as id V.
 // The passes are bound by latency, not by bytes: hence many CTAs with short stretches, all loads of a stretch
 // before their first use, and the ranks of a stretch of up to eight rounds kept in registers from the
-// counting to the writing.  (Lanes of equal digit: a word per digit in shared memory; a round took SORTNOTE.)
+// counting to the writing.  Lanes of equal digit find each other by a word per digit in shared memory (nine
+// ballots or the match instruction took two to four times as long).  65536 tokens: 18.5 us, 2048: 8.9 us.
 constexpr int kDigitBits = 9;
 constexpr int kDigits = 1 << kDigitBits;
 constexpr int kSortThreads = kDigits;              // a thread per digit
@@ -413,8 +414,8 @@ __device__ __forceinline__ void zero_rows(const ZeroArgs &z, int64_t first, int6
 constexpr int kSideThreads = 256;
 constexpr uint32_t kPrefetchBytes = 8192;      // per instruction
 
-// What the SMs that do not sort do meanwhile: zeros in the table when all of it is written, and the first
-// rows of dy into L2.  Launched behind the sort without waiting for it; it waits for the sort only
+// What the SMs that do not sort do meanwhile: zeros in the table (write; the first rows of dy into L2 as well
+// cost more than they gave, 75 against 66 us for 16384 tokens), or the first rows of dy into L2 (add).  Launched behind the sort without waiting for it; it waits for the sort only
 // before it ends, so that whoever waits for this kernel has the sorted list too.
 __global__ void __launch_bounds__(kSideThreads)
 embedding_side_kernel(ZeroArgs z, int64_t rows_per_block, const uint8_t *ahead, uint64_t ahead_bytes) {
@@ -447,7 +448,6 @@ struct RedArgs {
   int L;                         // lanes that share a row's slice: a power of two up to 32
   int per_part;                  // sorted places per group of L lanes
   float scale;
-  int add;
   uint32_t *flags;               // [piece][slice]: the partial sum of the run open at the piece's end is there
   uint32_t *status;
 };
@@ -506,14 +506,15 @@ struct Row {
 };
 
 // One lane's view of the rows: its first column, and the columns from there to the row's end.
-template <bool kDyF32, bool kDwF32, bool kVec>
+template <bool kDyF32, bool kDwF32, bool kVec, bool kAdd, bool kWide>
 struct Lane {
   const uint8_t *dy;
   uint8_t *dw;
-  int cols;
+  int cols, L;
   __device__ __forceinline__ Lane(const RedArgs &a, int slice, int l) {
-    const int c = slice * Cols<kVec>::kEach * a.L + (kVec ? l * 8 : l);
-    cols = a.D - c;
+    L = kWide ? 32 : a.L;
+    const int c = slice * Cols<kVec>::kEach * L + (kVec ? l * 8 : l);
+    cols = kWide ? Cols<kVec>::kEach * 32 : a.D - c;
     dy = a.dy + (int64_t)c * (kDyF32 ? 4 : 2);
     dw = a.dw + (int64_t)c * (kDwF32 ? 4 : 2);
   }
@@ -533,14 +534,14 @@ struct Lane {
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
         x[k] = __fmul_rn(a.scale, s.get(q * 8 + k));
-        if (a.add) x[k] = __fadd_rn(elem(old.o[q], k), x[k]);
+        if (kAdd) x[k] = __fadd_rn(elem(old.o[q], k), x[k]);
       }
-      store_oct<kDwF32, kVec>(p + q * 8 * a.L * (kDwF32 ? 4 : 2), cols - q * 8 * a.L, a.L, x);
+      store_oct<kDwF32, kVec>(p + q * 8 * L * (kDwF32 ? 4 : 2), cols - q * 8 * L, L, x);
     }
   }
   __device__ __forceinline__ void flush(const RedArgs &a, uint32_t v, const Sum<kVec> &s) const {
     Row<kDwF32, kVec> old = {};
-    old.load(dw_row(a, v), cols, a.L, a.add);
+    old.load(dw_row(a, v), cols, L, kAdd);
     finish(a, v, s, old);
   }
 };
@@ -557,11 +558,12 @@ struct Lane {
 // shared memory: every warp has asynchronous copies of the rows of the next kDepth places on the way and,
 // with "add", of the old table rows of the runs that end there (12 KB per warp, 192 KB per SM).  Loads ahead into
 // registers did not get there: they share six scoreboards, so waiting for one row waited for the newest
-// one too (accumulating 65536 rows of 1024: REDNOTE).
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, bool on) {
-  asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.u32 q, %2, 0;\n\t@q cp.async.cg.shared.global [%0], [%1], 16;\n\t}" ::"r"(dst),
-               "l"(src), "r"((uint32_t)on)
-               : "memory");
+// one too (accumulating 65536 rows of 1024: 63 us that way, 51 us by the ring, 5.8 TB/s).
+//
+// kWide: 32 lanes per row and whole slices, so that nothing about columns is left to compute in the loop (198
+// instructions per place and warp without it, 140 with it).
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 
 template <bool kDyF32, bool kDwF32, bool kVec, bool kAdd>
@@ -575,7 +577,7 @@ struct Stage {
   static constexpr uint32_t kBytes = kVec && kRing > kOpen ? kRing : kOpen;
 };
 
-template <bool kDyF32, bool kDwF32, bool kVec, bool kAdd>
+template <bool kDyF32, bool kDwF32, bool kVec, bool kAdd, bool kWide>
 __global__ void __launch_bounds__(kRedThreads, 2)
 embedding_reduce_kernel(RedArgs a) {
   using St = Stage<kDyF32, kDwF32, kVec, kAdd>;
@@ -586,12 +588,13 @@ embedding_reduce_kernel(RedArgs a) {
   __shared__ uint8_t through[kRedThreads];            // the part is one run, open at both ends (slot 0)
   __shared__ uint2 list[kMaxPiece + 1];               // the place before the piece, the piece's places
   __shared__ uint32_t s_first;
-  const int L = a.L, l = threadIdx.x & (L - 1), part = threadIdx.x / L, parts = kRedThreads / L, span = kEach * L;
+  const int L = kWide ? 32 : a.L, l = threadIdx.x & (L - 1), part = threadIdx.x / L, parts = kRedThreads / L;
+  const int span = kEach * L;
   float *const open_head = reinterpret_cast<float *>(stage_smem);      // [part][span], after the loop: the run open at
   float *const open_tail = open_head + kRedThreads * kEach;            // the part's start, and at its end only
   const uint32_t piece = blockIdx.x / a.slices;
   const int slice = (int)(blockIdx.x - piece * a.slices);
-  const Lane<kDyF32, kDwF32, kVec> lane(a, slice, l);
+  const Lane<kDyF32, kDwF32, kVec, kAdd, kWide> lane(a, slice, l);
   const int len = parts * a.per_part;
   const int64_t p0 = (int64_t)piece * len;
   for (int i = threadIdx.x; i < 2 * parts; i += kRedThreads) open_key[i & 1][i >> 1] = a.V;
@@ -638,23 +641,19 @@ embedding_reduce_kernel(RedArgs a) {
     const int y_bytes = (a.D - c0) * kYB, w_bytes = (a.D - c0) * kWB;
     // chunk q of a row: 16 bytes per lane, the group's lanes side by side
     auto fetch = [&](uint32_t slot, int j) {
-      const bool on = j < n;
-      const uint2 e = mine[on ? j : 0];
-      const uint8_t *src = dy + (uint64_t)(e.y & ~kEnds) * a.dy_pitch;
-      const uint32_t dst = ring + slot * (St::kDy + St::kOld) + group * (span * kYB);
+      if (j < n) {
+        const uint2 e = mine[j];
+        const uint8_t *src = dy + (uint64_t)(e.y & ~kEnds) * a.dy_pitch + l * 16;
+        const uint32_t dst = ring + slot * (St::kDy + St::kOld) + group * (span * kYB) + l * 16;
 #pragma unroll
-      for (int q = 0; q < kYChunks; ++q) {
-        const int o = (q * L + l) * 16;
-        cp_async16(dst + o, src + o, on && o < y_bytes);
-      }
-      if constexpr (kAdd) {
-        const bool want = on && (e.y & kEnds) && e.x != prev;
-        const uint8_t *old = dw + (uint64_t)e.x * a.dw_pitch;
-        const uint32_t od = ring + slot * (St::kDy + St::kOld) + St::kDy + group * (span * kWB);
+        for (int q = 0; q < kYChunks; ++q)
+          if (kWide || (q * L + l) * 16 < y_bytes) cp_async16(dst + q * L * 16, src + q * L * 16);
+        if (kAdd && (e.y & kEnds) && e.x != prev) {
+          const uint8_t *old = dw + (uint64_t)e.x * a.dw_pitch + l * 16;
+          const uint32_t od = ring + slot * (St::kDy + St::kOld) + St::kDy + group * (span * kWB) + l * 16;
 #pragma unroll
-        for (int q = 0; q < kWChunks; ++q) {
-          const int o = (q * L + l) * 16;
-          cp_async16(od + o, old + o, want && o < w_bytes);
+          for (int q = 0; q < kWChunks; ++q)
+            if (kWide || (q * L + l) * 16 < w_bytes) cp_async16(od + q * L * 16, old + q * L * 16);
         }
       }
       asm volatile("cp.async.commit_group;" ::: "memory");
@@ -820,7 +819,7 @@ embedding_reduce_kernel(RedArgs a) {
 // the group of lanes of each id's first token adds the rows along the links.  One launch.
 constexpr int kSmallT = 128;
 
-template <bool kDyF32, bool kDwF32, bool kVec>
+template <bool kDyF32, bool kDwF32, bool kVec, bool kAdd>
 __global__ void __launch_bounds__(kRedThreads)
 embedding_small_kernel(RedArgs a, const void *__restrict__ ids, int ids64, int64_t padding_idx, uint32_t *status) {
   __shared__ uint32_t key[kSmallT];
@@ -852,9 +851,9 @@ embedding_small_kernel(RedArgs a, const void *__restrict__ ids, int ids64, int64
   const int64_t u = (int64_t)blockIdx.x * (kRedThreads / L) + threadIdx.x / L;
   const int64_t t0 = u / a.slices;
   if (t0 >= T || !head[t0]) return;
-  const Lane<kDyF32, kDwF32, kVec> lane(a, (int)(u - t0 * a.slices), l);
+  const Lane<kDyF32, kDwF32, kVec, kAdd, false> lane(a, (int)(u - t0 * a.slices), l);
   Row<kDwF32, kVec> old = {};
-  old.load(lane.dw_row(a, key[t0]), lane.cols, L, a.add);
+  old.load(lane.dw_row(a, key[t0]), lane.cols, L, kAdd);
   Sum<kVec> acc;
   acc.clear();
   for (int t = (int)t0; t >= 0;) {
@@ -876,12 +875,11 @@ embedding_small_kernel(RedArgs a, const void *__restrict__ ids, int ids64, int64
 }
 
 // ------------------------------------------------------------------ host side
-constexpr int kMaxPart = 64, kMinPart = 4;
+constexpr int kMinPart = 4;                  // places per part at least
+constexpr int64_t kResident = 296;           // blocks of the sums that are resident at once, two per SM
 constexpr int kSortTarget = 4;               // rounds of 32 keys per warp the sort aims at
 constexpr int64_t kZeroBytes = 128 << 10;    // zeros per block
 constexpr uint64_t kAheadBytes = 64 << 20;   // of dy into L2 beside the sort
-constexpr int64_t kFullGrid = 200;       // blocks the sums should have at least
-
 struct Shape {
   int L, slices, per_part, span;      // span: columns of a slice
   int64_t pieces, max_pieces;
@@ -894,17 +892,18 @@ Shape shape_of(int64_t T, int64_t D, bool vec) {
   while (s.L < 32 && s.L * each < D) s.L *= 2;
   s.span = s.L * each;
   s.slices = (int)((D + s.span - 1) / s.span);
-  // parts as long as leaves enough of them to fill the GPU
-  const int64_t parts_per_cta = kRedThreads / s.L;
-  s.per_part = kMaxPiece / parts_per_cta < kMaxPart ? (int)(kMaxPiece / parts_per_cta) : kMaxPart;
-  const int least = s.per_part < kMinPart ? s.per_part : kMinPart;
-  while (s.per_part > least && (T / (parts_per_cta * s.per_part)) * s.slices < kFullGrid) s.per_part /= 2;
+  // As many places per part as fill the GPU's resident blocks evenly, in as few waves as the list of a piece
+  // allows: a block has a start and an end without rows in flight (accumulating 65536 rows of 1024,
+  // sort included: 294 blocks 72.5 us, 1024 blocks 79 us).
+  const int64_t parts_per_cta = kRedThreads / s.L, longest = kMaxPiece / parts_per_cta;
+  const int64_t wave = std::max<int64_t>(1, kResident / s.slices);
+  const int64_t waves = (T + wave * kMaxPiece - 1) / (wave * kMaxPiece);
+  int64_t places = waves > 0 ? (T + waves * wave * parts_per_cta - 1) / (waves * wave * parts_per_cta) : 1;
+  const int64_t least = std::min<int64_t>(longest, kMinPart);
+  s.per_part = (int)std::max(least, std::min(longest, places));
   s.pieces = (T + parts_per_cta * s.per_part - 1) / (parts_per_cta * s.per_part);
-  // most pieces any smaller T has: the workspace for T serves every smaller T
-  const int64_t most = 2 * (kFullGrid / s.slices) + 4;
-  const int64_t finest = (T + parts_per_cta * least - 1) / (parts_per_cta * least);
-  const int64_t bound = most < finest ? most : finest;
-  s.max_pieces = s.pieces > bound ? s.pieces : bound;
+  // at least the pieces of any smaller T, so that the workspace for T serves every smaller one
+  s.max_pieces = std::max((waves + 1) * wave, s.pieces);
   return s;
 }
 
@@ -962,9 +961,9 @@ uint32_t sort_cluster(int device) {
   if (e == cudaSuccess)
     e = cudaFuncSetAttribute(embedding_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(SortShared));
 #define ANC_REDUCE_SMEM(Y, W, ADD)                                                                         \
-  if (e == cudaSuccess)                                                                                    \
-  e = cudaFuncSetAttribute(embedding_reduce_kernel<Y, W, true, ADD>, cudaFuncAttributeMaxDynamicSharedMemorySize, \
-                           (int)Stage<Y, W, true, ADD>::kBytes)
+  for (auto k : {embedding_reduce_kernel<Y, W, true, ADD, false>, embedding_reduce_kernel<Y, W, true, ADD, true>}) \
+    if (e == cudaSuccess)                                                                                  \
+      e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Stage<Y, W, true, ADD>::kBytes)
   ANC_REDUCE_SMEM(false, false, false);
   ANC_REDUCE_SMEM(false, false, true);
   ANC_REDUCE_SMEM(false, true, false);
@@ -1127,7 +1126,6 @@ int anc_embedding_grad(anc_ctx *ctx, const void *dy, int dy_dtype, int64_t dy_ld
   ra.dy_pitch = (uint32_t)(dy_ld * (yf ? 4 : 2)); ra.dw_pitch = (uint32_t)(dw_ld * (wf ? 4 : 2));
   ra.partial = (float *)(wp + ws.partial);
   ra.V = (uint32_t)V; ra.D = (int)D; ra.slices = sh.slices; ra.L = sh.L; ra.per_part = sh.per_part; ra.scale = scale;
-  ra.add = !write;
   ra.status = ctx->d_status;
   const int64_t blocks =
       small ? (T * sh.slices + kRedThreads / sh.L - 1) / (kRedThreads / sh.L) : sh.pieces * sh.slices;
@@ -1163,7 +1161,7 @@ int anc_embedding_grad(anc_ctx *ctx, const void *dy, int dy_dtype, int64_t dy_ld
     cfg.numAttrs = 1;
     ANC_CUDA(cudaLaunchKernelEx(&cfg, embedding_sort_kernel, sa, n_ctas));
     const uint64_t dy_bytes = ((uint64_t)(T - 1) * dy_ld + D) * (yf ? 4 : 2) / 16 * 16;
-    const uint64_t ahead = dy_bytes < 64 ? 0 : dy_bytes - 16 < kAheadBytes ? dy_bytes - 16 : kAheadBytes;
+    const uint64_t ahead = write || dy_bytes < 64 ? 0 : dy_bytes - 16 < kAheadBytes ? dy_bytes - 16 : kAheadBytes;
     if (write || ahead) ANC_CUDA(launch_side(write ? V : 0, ahead, 1));
     n_attrs = 1;
   }
@@ -1174,19 +1172,25 @@ int anc_embedding_grad(anc_ctx *ctx, const void *dy, int dy_dtype, int64_t dy_ld
   cfg.stream = st;
   cfg.attrs = pdl;
   cfg.numAttrs = n_attrs;
-#define ANC_REDUCE_A(Y, W, VEC, ADD)                                                                 \
+#define ANC_REDUCE_W(Y, W, VEC, ADD, WIDE)                                                           \
   do {                                                                                               \
     cfg.dynamicSmemBytes = Stage<Y, W, VEC, ADD>::kBytes;                                            \
-    ANC_CUDA(cudaLaunchKernelEx(&cfg, embedding_reduce_kernel<Y, W, VEC, ADD>, ra));                 \
+    ANC_CUDA(cudaLaunchKernelEx(&cfg, embedding_reduce_kernel<Y, W, VEC, ADD, WIDE>, ra));           \
   } while (0)
-#define ANC_REDUCE(Y, W, VEC)                                                                        \
+#define ANC_REDUCE_A(Y, W, VEC, ADD)                                                                 \
   do {                                                                                               \
     if (small)                                                                                       \
-      ANC_CUDA(cudaLaunchKernelEx(&cfg, embedding_small_kernel<Y, W, VEC>, ra, ids, i64, padding_idx, ctx->d_status)); \
-    else if (write)                                                                                  \
-      ANC_REDUCE_A(Y, W, VEC, false);                                                                \
+      ANC_CUDA(cudaLaunchKernelEx(&cfg, embedding_small_kernel<Y, W, VEC, ADD>, ra, ids, i64, padding_idx, \
+                                  ctx->d_status));                                                   \
+    else if (VEC && sh.L == 32 && D % sh.span == 0)                                                  \
+      ANC_REDUCE_W(Y, W, VEC, ADD, VEC);                                                             \
     else                                                                                             \
-      ANC_REDUCE_A(Y, W, VEC, true);                                                                 \
+      ANC_REDUCE_W(Y, W, VEC, ADD, false);                                                           \
+  } while (0)
+#define ANC_REDUCE(Y, W, VEC)                    \
+  do {                                           \
+    if (write) ANC_REDUCE_A(Y, W, VEC, false);   \
+    else ANC_REDUCE_A(Y, W, VEC, true);          \
   } while (0)
 #define ANC_REDUCE_V(Y, W)                \
   do {                                    \
@@ -1200,6 +1204,7 @@ int anc_embedding_grad(anc_ctx *ctx, const void *dy, int dy_dtype, int64_t dy_ld
 #undef ANC_REDUCE_V
 #undef ANC_REDUCE
 #undef ANC_REDUCE_A
+#undef ANC_REDUCE_W
   ANC_CUDA(cudaGetLastError());
   return ANC_OK;
 }
