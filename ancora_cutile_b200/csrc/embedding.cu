@@ -85,7 +85,7 @@ __device__ __forceinline__ int64_t load_id(const void *ids, int ids64, int64_t t
 // Bound by memory once two latencies (id, then row) are covered.  A warp takes 32 / L rows side by side, L lanes
 // a row, and every lane four octets: kOcts of a row, of 4 / kOcts rows.  The ids of the next rows are read
 // before the current rows are.  131072 rows of 1024 bf16: 62 us, 32768: 17.8 us; rows of 1001 f32 to bf16, which
-// are not vectors, at ODDNOTE.
+// are not vectors, 93 us for 100000.
 constexpr int kLookupThreads = 128;
 
 struct LookupArgs {
@@ -309,10 +309,13 @@ embedding_sort_kernel(SortArgs a, uint32_t n_ctas) {
       sh.cnt[w][tid] = run;
       run += c[w];
     }
-    sh.tot[tid] = run;
-    if (single) __syncthreads();
-    else cluster_sync();
-    {
+    if (!single) {
+      sh.tot[tid] = run;
+      cluster_sync();
+    }
+    if (single) {
+      all = run;
+    } else {
       // a quarter of the threads per quarter of the cluster, four digits each
       const uint32_t quad = tid & 127, quarter = tid >> 7;
       const uint32_t slot = (uint32_t)__cvta_generic_to_shared(sh.tot + quad * 4);
@@ -333,12 +336,12 @@ embedding_sort_kernel(SortArgs a, uint32_t n_ctas) {
       }
       *reinterpret_cast<uint4 *>(&sh.share[0][quarter][quad * 4]) = sum_all;
       *reinterpret_cast<uint4 *>(&sh.share[1][quarter][quad * 4]) = sum_before;
-    }
-    __syncthreads();
+      __syncthreads();
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      all += sh.share[0][q][tid];
-      before += sh.share[1][q][tid];
+      for (int q = 0; q < 4; ++q) {
+        all += sh.share[0][q][tid];
+        before += sh.share[1][q][tid];
+      }
     }
     uint32_t sum = all;      // exclusive scan of the digit totals
 #pragma unroll
@@ -411,9 +414,10 @@ __device__ __forceinline__ void zero_rows(const ZeroArgs &z, int64_t first, int6
 constexpr int kSideThreads = 256;
 constexpr uint32_t kPrefetchBytes = 8192;      // per instruction
 
-// What the SMs that do not sort do meanwhile: zeros in the table (write; the first rows of dy into L2 as well
-// cost more than they gave, 75 against 66 us for 16384 tokens), or the first rows of dy into L2 (add).  Launched behind the sort without waiting for it; it waits for the sort only
-// before it ends, so that whoever waits for this kernel has the sorted list too.
+// What the SMs that do not sort do meanwhile: zeros in the table (write), or the first rows of dy into L2 (add;
+// 76 us without it for 65536 rows of 1024, 73 with it.  Beside the zeros it cost more than it gave, 75 against
+// 66 us for 16384 tokens).  Launched behind the sort without waiting for it; it waits for the sort only before it
+// ends, so that whoever waits for this kernel has the sorted list too.
 __global__ void __launch_bounds__(kSideThreads)
 embedding_side_kernel(ZeroArgs z, int64_t rows_per_block, const uint8_t *ahead, uint64_t ahead_bytes) {
   pdl_trigger();
@@ -999,6 +1003,15 @@ uint32_t sort_cluster(int device) {
   return found;
 }
 
+// bytes from the first to the last element of an array of rows
+int64_t row_span(int64_t rows, int64_t ld, int bytes, int64_t D) { return ((rows - 1) * ld + D) * bytes; }
+
+// whether an array of rows and `n` bytes at b share a byte
+bool overlap(const void *a, int64_t rows, int64_t ld, int bytes, int64_t D, const void *b, int64_t n) {
+  const uintptr_t a0 = (uintptr_t)a, b0 = (uintptr_t)b;
+  return a0 < b0 + (uintptr_t)n && b0 < a0 + (uintptr_t)row_span(rows, ld, bytes, D);
+}
+
 bool rows_are_vectors(const void *p, int64_t ld, int f32, int64_t D) {
   const int64_t align = f32 ? 32 : 16;       // of eight elements
   return (uintptr_t)p % align == 0 && D % 8 == 0 && ld % 8 == 0;
@@ -1027,6 +1040,9 @@ int anc_embedding_lookup(anc_ctx *ctx, const void *table, int table_dtype, int64
   ANC_REQUIRE(((uintptr_t)table & (tf ? 3 : 1)) == 0 && ((uintptr_t)out & (of ? 3 : 1)) == 0 &&
                   ((uintptr_t)ids & (i64 ? 7 : 3)) == 0,
               "pointer not aligned to its element size");
+  ANC_REQUIRE(!overlap(table, V, table_ld, tf ? 4 : 2, D, out, row_span(T, out_ld, of ? 4 : 2, D)) &&
+                  !overlap(out, T, out_ld, of ? 4 : 2, D, ids, T * (i64 ? 8 : 4)),
+              "the output overlaps an input");
   anc_device_guard guard(ctx->device);
   cudaStream_t st = anc_pick_stream(ctx, stream);
   const bool vec = rows_are_vectors(table, table_ld, tf, D) && rows_are_vectors(out, out_ld, of, D);
@@ -1096,6 +1112,11 @@ int anc_embedding_grad(anc_ctx *ctx, const void *dy, int dy_dtype, int64_t dy_ld
     ANC_REQUIRE(((uintptr_t)dy & (yf ? 3 : 1)) == 0 && ((uintptr_t)ids & (i64 ? 7 : 3)) == 0,
                 "pointer not aligned to its element size");
     ANC_REQUIRE(((uintptr_t)work & 15) == 0, "workspace not aligned to 16 bytes");
+    ANC_REQUIRE(!overlap(dw, V, dw_ld, wf ? 4 : 2, D, dy, row_span(T, dy_ld, yf ? 4 : 2, D)) &&
+                    !overlap(dw, V, dw_ld, wf ? 4 : 2, D, ids, T * (i64 ? 8 : 4)) &&
+                    !overlap(dw, V, dw_ld, wf ? 4 : 2, D, work, (int64_t)workspace_of(T, D).total) &&
+                    !overlap(dy, T, dy_ld, yf ? 4 : 2, D, work, (int64_t)workspace_of(T, D).total),
+                "dw overlaps an input");
   }
   const Workspace ws = workspace_of(T, D);
   ANC_REQUIRE(T == 0 || work_bytes >= ws.total, "workspace of %llu bytes, %llu are needed",

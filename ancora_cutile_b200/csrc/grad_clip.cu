@@ -39,8 +39,8 @@ constexpr int kChunkVec = kThreads * kVecPerThread;           // vectors per chu
 constexpr int kChunkElems = kChunkVec * 8;
 constexpr uint32_t kWaitPolls = 1u << 22;                     // of the one-launch clip; about a second
 
-// One tensor.  The norm reads elements [head, head + 8 * nvec) as 16-byte aligned vectors and the up to 7 on
-// either side one by one.  The scaling sweep wants input and output aligned together: from shead on, snvec
+// One tensor.  The norm reads elements [head, head + 8 * nvec) as vectors of eight aligned to their size (16
+// bytes of bf16, 32 of f32), and the up to 7 on either side one by one.  The scaling sweep wants input and output aligned together: from shead on, snvec
 // vectors; without a common alignment snvec is 0 and all its elements go one by one.
 struct Entry {
   const void *g;
@@ -67,8 +67,8 @@ struct Raw {
 template <bool kF32>
 __device__ __forceinline__ void load_raw(Raw<kF32> &r, const void *p, uint64_t i, bool on) {
   const uint8_t *q = (const uint8_t *)p + i * (kF32 ? 4 : 2);
-  ld_v4(r.w[0], r.w[1], r.w[2], r.w[3], q, on);
-  if constexpr (kF32) ld_v4(r.w[4], r.w[5], r.w[6], r.w[7], q + 16, on);
+  if constexpr (kF32) ld_v8(r.w, q, on);
+  else ld_v4(r.w[0], r.w[1], r.w[2], r.w[3], q, on);
 }
 template <bool kF32>
 __device__ __forceinline__ void widen(const Raw<kF32> &r, float x[8]) {
@@ -281,9 +281,7 @@ struct Chunk {
 #pragma unroll
       for (int j = 0; j < 8; ++j) x[j] = __fmul_rn(x[j], f);
       if constexpr (kOutF32) {
-        float4 *d = reinterpret_cast<float4 *>((float *)e.out + i);
-        d[0] = make_float4(x[0], x[1], x[2], x[3]);
-        d[1] = make_float4(x[4], x[5], x[6], x[7]);
+        st_v8((float *)e.out + i, x);
       } else {
         uint32_t h[8];
 #pragma unroll
@@ -322,7 +320,7 @@ grad_scale_kernel(const Entry *__restrict__ tab, uint32_t n_tab, const float *__
 
 // Norm and scaling in one launch: a block per chunk, all resident at once (a cooperative launch), the
 // chunk in registers while the blocks wait for one another's sums.  The wait is bounded: when it runs out,
-// status bit 0x10 is set and nothing is written.
+// status bit 0x10 is set, norm and factor are NaN and no gradient is written.
 template <bool kF32, bool kOutF32>
 __global__ void __launch_bounds__(kThreads)
 grad_clip_fused_kernel(const Entry *__restrict__ tab, uint32_t n_tab, double *partial, uint32_t *ticket, NormOut o,
@@ -346,7 +344,10 @@ grad_clip_fused_kernel(const Entry *__restrict__ tab, uint32_t n_tab, double *pa
       ticket[0] = 0u;
       ticket[1] = 0u;
     }
-    if (!ok) atomicOr(status, ANC_DEV_TIMEOUT_DEP);
+    if (!ok) {
+      atomicOr(status, ANC_DEV_TIMEOUT_DEP);
+      o.result[0] = o.result[1] = __int_as_float(0x7FFFFFFF);
+    }
   }
   __syncthreads();
   if (!ok) return;
@@ -477,13 +478,13 @@ int anc_clip_plan_create(anc_ctx *ctx, const anc_clip_tensor *tensors, int n_ten
       e.numel = t.numel;
       e.vec0 = vecs;
       e.chunk0 = (uint32_t)chunks;
-      e.head = (uint16_t)(((16 - ((uintptr_t)e.g & 15)) & 15) / gs);
+      e.head = (uint16_t)((8 * gs - (uintptr_t)e.g % (8 * gs)) % (8 * gs) / gs);
       e.nvec = t.numel >= e.head + 8u ? (t.numel - e.head) / 8 : 0;
       if (!e.nvec) e.head = 0;
       e.shead = 0;
       e.snvec = 0;
       for (uint32_t h = 0; h < 8; ++h) {
-        if ((((uintptr_t)e.g + h * gs) & 15) || (((uintptr_t)e.out + h * os) & 15)) continue;
+        if (((uintptr_t)e.g + h * gs) % (8 * gs) || ((uintptr_t)e.out + h * os) % (8 * os)) continue;
         if (t.numel >= h + 8) {
           e.shead = (uint16_t)h;
           e.snvec = (t.numel - h) / 8;

@@ -46,11 +46,15 @@ class GradClip:
 
     def norm(self, max_norm=float("inf"), scale=1.0, eps=1e-6, stream=None):
         """{norm, factor} of the gradients as they are now."""
-        L.check(L.lib().anc_grad_norm(self.handle, scale, max_norm, eps, stream or None))
+        rc = L.lib().anc_grad_norm(self.handle, scale, max_norm, eps, stream or None)
+        if rc:
+            L.check(rc)
 
     def clip(self, max_norm, scale=1.0, eps=1e-6, stream=None):
         """``norm``, then out = round(g * factor) for every tensor."""
-        L.check(L.lib().anc_grad_clip(self.handle, scale, max_norm, eps, stream or None))
+        rc = L.lib().anc_grad_clip(self.handle, scale, max_norm, eps, stream or None)
+        if rc:
+            L.check(rc)
 
     def sumsq(self, stream=None):
         """This rank's sum of squares alone (``sumsq_ptr``); add the ranks' sums, then ``finish``."""

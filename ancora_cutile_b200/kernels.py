@@ -70,7 +70,21 @@ def grad_accumulate(acc, src=None, g16=None, numel=None, src_dtype="f32", elem_o
 
 
 _IDS = {"i32": L.IDS_I32, "i64": L.IDS_I64}
+_SIZE = {"bf16": 2, "f32": 4, "i32": 4, "i64": 8}
+
+
+def _buf(obj, rows, ld, D, dtype, what):
+    """Address of ``obj``; a buffer that knows its size must hold the rows it is said to."""
+    if type(obj) is int:
+        return obj
+    n = getattr(obj, "nbytes", None)
+    if n is not None and rows > 0 and n < ((rows - 1) * (ld or D) + D) * _SIZE[dtype]:
+        raise ValueError(f"{what} holds {n} bytes: too few for {rows} rows of {D} {dtype}")
+    return dev_ptr(obj)
+
+
 _EMBED = {"write": L.EMBED_WRITE, "add": L.EMBED_ADD}
+_VOUCHED = 2 ** 64 - 1
 
 
 def embedding_lookup(table, ids, out, T, V, D, scale=1.0, table_dtype="bf16", out_dtype="bf16", ids_dtype="i64",
@@ -78,9 +92,12 @@ def embedding_lookup(table, ids, out, T, V, D, scale=1.0, table_dtype="bf16", ou
     """out[t] = round(scale * table[ids[t]]) for T tokens over a (V, D) table; rows ``*_ld`` elements apart
     (0: D).  A negative id gives a zero row; an id >= V too, and sets status bit 0x8."""
     ctx = ctx or get_context()
-    L.check(L.lib().anc_embedding_lookup(ctx.handle, dev_ptr(table), _GRAD[table_dtype], table_ld, dev_ptr(ids),
-                                         _IDS[ids_dtype], dev_ptr(out), _GRAD[out_dtype], out_ld, T, V, D,
-                                         scale, stream or None))
+    rc = L.lib().anc_embedding_lookup(ctx.handle, _buf(table, V, table_ld, D, table_dtype, "table"),
+                                      _GRAD[table_dtype], table_ld, _buf(ids, 1, T, T, ids_dtype, "ids"),
+                                      _IDS[ids_dtype], _buf(out, T, out_ld, D, out_dtype, "out"), _GRAD[out_dtype],
+                                      out_ld, T, V, D, scale, stream or None)
+    if rc:
+        L.check(rc)
 
 
 def embedding_grad_workspace(T, V, D):
@@ -96,13 +113,15 @@ def embedding_grad(dy, ids, dw, T, V, D, work, scale=1.0, dy_dtype="bf16", dw_dt
     dw[v] = round(dw[v] + scale * S_v) on the rows some token names (mode "add"), with S_v the float32 sum of
     dy[t] over the tokens with ids[t] == v, in an order the ids alone fix.  Negative ids and ``padding_idx``
     contribute nothing.  ``work``: a device buffer of ``embedding_grad_workspace(T, V, D)`` bytes that no
-    other call in flight uses; ``work_bytes`` defaults to its ``nbytes`` and, for a bare address, to the need."""
+    other call in flight uses; ``work_bytes`` defaults to its ``nbytes``; a bare address is taken to be enough."""
     ctx = ctx or get_context()
     if work_bytes is None:
-        work_bytes = getattr(work, "nbytes", None)
-        if work_bytes is None:
-            work_bytes = embedding_grad_workspace(T, V, D)
-    L.check(L.lib().anc_embedding_grad(ctx.handle, dev_ptr(dy), _GRAD[dy_dtype], dy_ld, dev_ptr(ids),
-                                       _IDS[ids_dtype], dev_ptr(dw), _GRAD[dw_dtype], dw_ld, T, V, D, scale,
-                                       _EMBED[mode], -1 if padding_idx is None else padding_idx, dev_ptr(work),
-                                       work_bytes, stream or None))
+        work_bytes = getattr(work, "nbytes", _VOUCHED)
+    rc = L.lib().anc_embedding_grad(ctx.handle, _buf(dy, T, dy_ld, D, dy_dtype, "dy"), _GRAD[dy_dtype], dy_ld,
+                                    _buf(ids, 1, T, T, ids_dtype, "ids"), _IDS[ids_dtype],
+                                    _buf(dw, V, dw_ld, D, dw_dtype, "dw"), _GRAD[dw_dtype], dw_ld, T, V, D, scale,
+                                    _EMBED[mode],
+                                    -1 if padding_idx is None else padding_idx, dev_ptr(work), work_bytes,
+                                    stream or None)
+    if rc:
+        L.check(rc)

@@ -62,12 +62,13 @@ def test_clip_scalars_refused(scale, max_norm, eps):
         assert f(FAKE, scale, max_norm, eps, None) == L.E_INVALID
 
 
-def _lookup(ctx=FAKE, table=4096, td=0, tld=0, ids=4096, idt=L.IDS_I64, out=4096, od=0, old=0, T=4, V=10, D=8,
+def _lookup(ctx=FAKE, table=4096, td=0, tld=0, ids=1 << 20, idt=L.IDS_I64, out=1 << 21, od=0, old=0, T=4, V=10, D=8,
             scale=1.0):
     return L.lib().anc_embedding_lookup(ctx, table, td, tld, ids, idt, out, od, old, T, V, D, scale, None)
 
 
 @pytest.mark.parametrize("kw", [
+    dict(out=4096), dict(out=4098), dict(out=1 << 21, ids=(1 << 21) + 8),
     dict(ctx=None), dict(table=None), dict(ids=None), dict(out=None), dict(td=3), dict(od=-1), dict(idt=2),
     dict(table=4097), dict(out=4098, od=1), dict(ids=4100), dict(ids=4098, idt=L.IDS_I32), dict(tld=7), dict(old=7),
     dict(T=-1), dict(T=1 << 31), dict(V=0), dict(V=(1 << 31) - 1), dict(D=0), dict(D=(1 << 24) + 1)])
@@ -79,18 +80,41 @@ def test_lookup_of_no_tokens_is_nothing():
     assert _lookup(T=0, table=None, ids=None, out=None) == 0
 
 
-def _grad(ctx=FAKE, dy=4096, yd=0, yld=0, ids=4096, idt=L.IDS_I64, dw=4096, wd=0, wld=0, T=4, V=10, D=8, scale=1.0,
-          mode=L.EMBED_ADD, pad=-1, work=4096, wb=1 << 30):
+def _grad(ctx=FAKE, dy=4096, yd=0, yld=0, ids=1 << 21, idt=L.IDS_I64, dw=1 << 20, wd=0, wld=0, T=4, V=10, D=8, scale=1.0,
+          mode=L.EMBED_ADD, pad=-1, work=1 << 24, wb=1 << 30):
     return L.lib().anc_embedding_grad(ctx, dy, yd, yld, ids, idt, dw, wd, wld, T, V, D, scale, mode, pad, work, wb, None)
 
 
 @pytest.mark.parametrize("kw", [
-    dict(ctx=None), dict(dy=None), dict(ids=None), dict(dw=None), dict(work=None), dict(work=4104), dict(yd=3),
+    dict(dw=4096), dict(dw=8192, dy=8240), dict(dw=8192, ids=8248), dict(dw=1 << 20, work=(1 << 20) - 256),
+    dict(dy=1 << 20, work=(1 << 20) - 256),
+    dict(ctx=None), dict(dy=None), dict(ids=None), dict(dw=None), dict(work=None), dict(work=(1 << 24) + 8), dict(yd=3),
     dict(wd=-1), dict(idt=2), dict(mode=2), dict(dy=4097), dict(dw=4098, wd=1), dict(ids=4100), dict(yld=7),
     dict(wld=7), dict(T=-1), dict(T=1 << 31), dict(V=0), dict(V=(1 << 31) - 1), dict(D=0), dict(D=(1 << 24) + 1),
     dict(wb=16)])
 def test_embedding_grad_refusals(kw):
     assert _grad(**kw) == L.E_INVALID
+
+
+def test_buffers_that_know_their_size_are_held_to_it():
+    class Buf:
+        def __init__(self, nbytes):
+            self.ptr, self.nbytes = 4096, nbytes
+
+    class Ctx:
+        handle = FAKE
+    ok = dict(table=Buf(10 * 16), ids=Buf(32), out=Buf(64), T=4, V=10, D=8, ctx=Ctx)
+    for k, n in (("table", 159), ("ids", 31), ("out", 63)):
+        with pytest.raises(ValueError, match=k):
+            kernels.embedding_lookup(**dict(ok, **{k: Buf(n)}))
+    with pytest.raises(ValueError, match="ids"):               # 32-bit ids taken for 64-bit ones
+        kernels.embedding_lookup(**dict(ok, ids=Buf(16)))
+    ok = dict(dy=Buf(64), ids=Buf(32), dw=Buf(160), work=4096, T=4, V=10, D=8, ctx=Ctx)
+    for k, n in (("dy", 63), ("ids", 31), ("dw", 159)):
+        with pytest.raises(ValueError, match=k):
+            kernels.embedding_grad(**dict(ok, **{k: Buf(n)}))
+    with pytest.raises(ValueError, match="dw"):
+        kernels.embedding_grad(**dict(ok, dw_ld=9))
 
 
 def test_adding_no_tokens_is_nothing():
