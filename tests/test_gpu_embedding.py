@@ -184,7 +184,8 @@ def test_gradient(ctx, case, dy_dtype, dw_dtype, mode):
 
 
 @pytest.mark.parametrize("T,V,D,kind", [(5000, 37, 130, "zipf"), (40000, 3, 264, "zipf"), (66000, 70000, 24, "padded"),
-                                        (300, 20, 2048, "zipf")])
+                                        (300, 20, 2048, "zipf"), (30000, 5, 1024, "zipf"), (9000, 2000, 512, "padded"),
+                                        (20000, 9, 1536, "one row"), (200000, 100, 8, "zipf"), (129, 3, 512, "one row")])
 def test_integer_gradients_are_exact(ctx, T, V, D, kind):
     rng = np.random.default_rng(T)
     ids = _ids(rng, T, V, kind)
@@ -306,3 +307,56 @@ def test_captured_and_replayed_with_new_tokens(ctx):
     for b in [d_dy, d_ids] + works + dws:
         b.free()
     assert ctx.status() == 0
+
+
+def test_offsets_past_32_bits(ctx):
+    """Rows whose byte and element offsets pass 2^31 and 2^32, in the table, the gradient table and dy."""
+    V, D, T = 300_000, 8192, 290_000
+    rng = np.random.default_rng(2)
+    table = anc.DBuf.zeros((V, D), np.uint16, ctx)                 # 4.9 GB
+    rows = np.array([0, 1, 131071, 131072, 262143, 262144, 262145, V - 2, V - 1])
+    vals = obf.rne_bits(rng.standard_normal((len(rows), D)))
+    for r, v in zip(rows, vals):
+        table.slice_elems(int(r) * D, D).upload(v)
+    out, di = anc.DBuf.zeros((len(rows), D), np.uint16, ctx), anc.DBuf(rows, ctx)
+    kernels.embedding_lookup(table, di, out, len(rows), V, D, ctx=ctx)
+    ctx.sync()
+    assert np.array_equal(out.to_numpy(), vals)
+    # dy: the same memory as T rows, zero but for those; every token of the nonzero rows names a far row
+    ids = np.full(T, -1, np.int64)
+    ids[::2] = 7
+    ids[rows[:-2]] = V - 1 - np.arange(len(rows) - 2) // 2
+    dw, d_ids = anc.DBuf.zeros((V, D), np.float32, ctx), anc.DBuf(ids, ctx)      # 9.8 GB
+    work = anc.DBuf.empty((kernels.embedding_grad_workspace(T, V, D),), np.uint8, ctx)
+    kernels.embedding_grad(table, d_ids, dw, T, V, D, work, dw_dtype="f32", mode="add", ctx=ctx)
+    ctx.sync()
+    want = np.zeros((8, D))
+    for k, v in enumerate(vals[:-2]):
+        want[k // 2] += obf.bits_f32(v)
+    for k in range(8):
+        got = dw.slice_elems((V - 1 - k) * D, D).to_numpy()
+        assert np.abs(got - want[k]).max() <= 4 * U * 8, k                       # sums of at most two terms below 8
+    assert not dw.slice_elems(7 * D, D).to_numpy().any()
+    assert ctx.status() == 0
+    for b in (table, out, di, dw, d_ids, work):
+        b.free()
+
+
+def test_table_of_many_short_rows(ctx):
+    """Four sort passes (ids of 28 bits)."""
+    V, D, T = 150_000_001, 1, 5000
+    rng = np.random.default_rng(4)
+    ids = rng.integers(0, V, T)
+    ids[:1000] = ids[1000:2000]
+    ids[2000:2500] = V - 1
+    dy = rng.integers(-8, 9, (T, D)).astype(np.float32)
+    dw, d_ids, d_dy = anc.DBuf.zeros((V,), np.float32, ctx), anc.DBuf(ids, ctx), anc.DBuf(dy, ctx)
+    work = anc.DBuf.empty((kernels.embedding_grad_workspace(T, V, D),), np.uint8, ctx)
+    kernels.embedding_grad(d_dy, d_ids, dw, T, V, D, work, dy_dtype="f32", dw_dtype="f32", mode="add", ctx=ctx)
+    ctx.sync()
+    got = dw.to_numpy()
+    want = np.zeros(V, np.float32)
+    np.add.at(want, ids, dy[:, 0])
+    assert np.array_equal(got, want)
+    for b in (dw, d_ids, d_dy, work):
+        b.free()
