@@ -383,7 +383,7 @@ embedding_sort_kernel(SortArgs a, uint32_t n_ctas) {
   }
 }
 
-// ------------------------------------------------------------------ zeros, and reading ahead
+// ------------------------------------------------------------------ zeros
 struct ZeroArgs {
   uint8_t *dw;
   int64_t row_bytes, pitch, V;
@@ -411,24 +411,17 @@ __device__ __forceinline__ void zero_rows(const ZeroArgs &z, int64_t first, int6
   }
 }
 
-constexpr int kSideThreads = 256;
-constexpr uint32_t kPrefetchBytes = 8192;      // per instruction
+constexpr int kZeroThreads = 256;
 
-// What the SMs that do not sort do meanwhile: zeros in the table (write), or the first rows of dy into L2 (add;
-// 76 us without it for 65536 rows of 1024, 73 with it.  Beside the zeros it cost more than it gave, 75 against
-// 66 us for 16384 tokens).  Launched behind the sort without waiting for it; it waits for the sort only before it
-// ends, so that whoever waits for this kernel has the sorted list too.
-__global__ void __launch_bounds__(kSideThreads)
-embedding_side_kernel(ZeroArgs z, int64_t rows_per_block, const uint8_t *ahead, uint64_t ahead_bytes) {
+// When the whole table is written, what the SMs that do not sort do meanwhile.  Launched behind the sort without
+// waiting for it; it waits for the sort only before it ends, so that whoever waits for this kernel has the
+// sorted list too.  (Reading the first rows of dy into L2 at that time gave 3 us of 75 for 65536 rows of 1024
+// bf16 added to f32, cost 5 of 149 for 30000 rows of 4096 f32 and 9 of 66 beside the zeros.)
+__global__ void __launch_bounds__(kZeroThreads)
+embedding_zero_kernel(ZeroArgs z, int64_t rows_per_block) {
   pdl_trigger();
   const int64_t first = blockIdx.x * rows_per_block, last = first + rows_per_block < z.V ? first + rows_per_block : z.V;
-  if (first < last) zero_rows(z, first, last);
-  const uint64_t step = (uint64_t)gridDim.x * kPrefetchBytes;
-  if (threadIdx.x == 0)
-    for (uint64_t o = (uint64_t)blockIdx.x * kPrefetchBytes; o < ahead_bytes; o += step) {
-      const uint32_t n = (uint32_t)(ahead_bytes - o < kPrefetchBytes ? ahead_bytes - o : kPrefetchBytes);
-      asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(ahead + o), "r"(n) : "memory");
-    }
+  zero_rows(z, first, last);
   pdl_wait();
 }
 
@@ -881,7 +874,6 @@ constexpr int kMinPart = 4;                  // places per part at least
 constexpr int64_t kResident = 296;           // blocks of the sums that are resident at once, two per SM
 constexpr int kSortTarget = 4;               // rounds of 32 keys per warp the sort aims at
 constexpr int64_t kZeroBytes = 128 << 10;    // zeros per block
-constexpr uint64_t kAheadBytes = 64 << 20;   // of dy into L2 beside the sort
 struct Shape {
   int L, slices, per_part, span;      // span: columns of a slice
   int64_t pieces, max_pieces;
@@ -1134,24 +1126,17 @@ int anc_embedding_grad(anc_ctx *ctx, const void *dy, int dy_dtype, int64_t dy_ld
   cudaLaunchAttribute pdl[1];
   pdl[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   pdl[0].val.programmaticStreamSerializationAllowed = 1;
-  // zeros in the table's first `rows` rows, `ahead` bytes of dy into L2
-  auto launch_side = [&](int64_t rows, uint64_t ahead, int n_attrs) {
-    ZeroArgs z = za;
-    z.V = rows;
-    const uint8_t *from = (const uint8_t *)(((uintptr_t)dy + 15) & ~(uintptr_t)15);
+  auto launch_zero = [&](int n_attrs) {
     const int64_t per_block = za.row_bytes < kZeroBytes ? kZeroBytes / za.row_bytes : 1;
-    int64_t blocks = (rows + per_block - 1) / per_block;
-    const int64_t fetches = (int64_t)((ahead + kPrefetchBytes - 1) / kPrefetchBytes);
-    if (blocks < 1) blocks = fetches < ctx->sm_count * 4 ? fetches : ctx->sm_count * 4;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)blocks);
-    cfg.blockDim = dim3(kSideThreads);
+    cfg.gridDim = dim3((unsigned)((V + per_block - 1) / per_block));
+    cfg.blockDim = dim3(kZeroThreads);
     cfg.stream = st;
     cfg.attrs = pdl;
     cfg.numAttrs = n_attrs;
-    return cudaLaunchKernelEx(&cfg, embedding_side_kernel, z, per_block, from, ahead);
+    return cudaLaunchKernelEx(&cfg, embedding_zero_kernel, za, per_block);
   };
-  if (write && small) ANC_CUDA(launch_side(V, 0, 0));
+  if (write && small) ANC_CUDA(launch_zero(0));
   if (T == 0) return ANC_OK;
   uint8_t *wp = (uint8_t *)work;
   const bool vec = rows_are_vectors(dy, dy_ld, yf, D) && rows_are_vectors(dw, dw_ld, wf, D);
@@ -1195,9 +1180,7 @@ int anc_embedding_grad(anc_ctx *ctx, const void *dy, int dy_dtype, int64_t dy_ld
     cfg.attrs = at;
     cfg.numAttrs = 1;
     ANC_CUDA(cudaLaunchKernelEx(&cfg, embedding_sort_kernel, sa, n_ctas));
-    const uint64_t dy_bytes = ((uint64_t)(T - 1) * dy_ld + D) * (yf ? 4 : 2) / 16 * 16;
-    const uint64_t ahead = write || dy_bytes < 64 ? 0 : dy_bytes - 16 < kAheadBytes ? dy_bytes - 16 : kAheadBytes;
-    if (write || ahead) ANC_CUDA(launch_side(write ? V : 0, ahead, 1));
+    if (write) ANC_CUDA(launch_zero(1));
     n_attrs = 1;
   }
   // these launches start while their predecessor drains and wait for it on the device
