@@ -83,9 +83,9 @@ __device__ __forceinline__ int64_t load_id(const void *ids, int ids64, int64_t t
 
 // ------------------------------------------------------------------ lookup
 // Bound by memory once two latencies (id, then row) are covered.  A warp takes 32 / L rows side by side, L lanes
-// a row, and every lane four octets: kOcts of a row, of 4 / kOcts rows.  The ids of the next rows are read
-// before the current rows are.  131072 rows of 1024 bf16: 62 us, 32768: 17.8 us; rows of 1001 f32 to bf16, which
-// are not vectors, 93 us for 100000.
+// a row, and every lane four octets: kOcts of a row, of 4 / kOcts rows.  Warps do one unit and leave: resident
+// ones that went on to further rows, with the next ids read ahead, were slower (131072 rows of 1024 bf16: 70
+// against 59 us; 32768: 20.4 against 18.7).
 constexpr int kLookupThreads = 128;
 
 struct LookupArgs {
@@ -93,61 +93,50 @@ struct LookupArgs {
   const void *ids;
   uint8_t *out;
   uint32_t table_pitch, out_pitch;      // bytes from row to row
-  int64_t T, V, units;
-  int ids64, D, L, slices;
+  uint32_t T, V, units;
+  int ids64, D, L;
   float scale;
   uint32_t *status;
 };
 
+// A warp per unit: unit u is rows [u, u + 1) * kRows * 32 / L; blockIdx.y: slice of 8 * kOcts * L columns.
 template <bool kTabF32, bool kOutF32, bool kVec, int kOcts>
 __global__ void __launch_bounds__(kLookupThreads)
 embedding_lookup_kernel(LookupArgs a) {
   constexpr int kRows = 4 / kOcts, kTB = kTabF32 ? 4 : 2, kOB = kOutF32 ? 4 : 2;
-  const int L = a.L, lane = threadIdx.x & 31, l = lane & (L - 1), group = lane / L, groups = 32 / L;
-  const int64_t stride = (int64_t)gridDim.x * (kLookupThreads / 32);
-  int64_t u = (int64_t)blockIdx.x * (kLookupThreads / 32) + (threadIdx.x >> 5);
-  // row r of this lane's group in unit u
-  auto row_of = [&](int64_t unit, int r) { return (unit / a.slices * kRows + r) * groups + group; };
-  auto read_ids = [&](int64_t unit, int64_t (&id)[kRows]) {
+  const int L = a.L, lane = threadIdx.x & 31, l = lane & (L - 1);
+  const uint32_t u = blockIdx.x * (kLookupThreads / 32) + (threadIdx.x >> 5);
+  if (u >= a.units) return;
+  const int c0 = (int)blockIdx.y * (8 * kOcts) * L + (kVec ? l * 8 : l);
+  const int cols = a.D - c0;            // from this lane's first column to the row's end
+  const uint32_t t0 = u * kRows * (32 / L) + lane / L, t_step = 32 / L;
+  Oct<kTabF32, kVec> x[kRows][kOcts] = {};
+  int64_t id[kRows];
 #pragma unroll
-    for (int r = 0; r < kRows; ++r) {
-      const int64_t t = row_of(unit < a.units ? unit : 0, r);
-      id[r] = load_id(a.ids, a.ids64, t < a.T ? t : a.T - 1);
+  for (int r = 0; r < kRows; ++r) {
+    const uint32_t t = t0 + r * t_step;
+    id[r] = load_id(a.ids, a.ids64, t < a.T ? t : a.T - 1);
+  }
+#pragma unroll
+  for (int r = 0; r < kRows; ++r) {
+    const bool live = id[r] >= 0 && id[r] < a.V;
+    const uint8_t *row = a.table + (int64_t)c0 * kTB + (uint64_t)(live ? (uint32_t)id[r] : 0u) * a.table_pitch;
+#pragma unroll
+    for (int q = 0; q < kOcts; ++q)
+      load_oct<kTabF32, kVec>(x[r][q], row + q * 8 * L * kTB, cols - q * 8 * L, L, live);
+    if (id[r] >= a.V && l == 0 && blockIdx.y == 0) atomicOr(a.status, ANC_DEV_BAD_INDEX);
+  }
+#pragma unroll
+  for (int r = 0; r < kRows; ++r) {
+    const uint32_t t = t0 + r * t_step;
+    uint8_t *row = a.out + (int64_t)c0 * kOB + (uint64_t)t * a.out_pitch;
+#pragma unroll
+    for (int q = 0; q < kOcts; ++q) {
+      float f[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) f[k] = __fmul_rn(elem(x[r][q], k), a.scale);
+      store_oct<kOutF32, kVec>(row + q * 8 * L * kOB, t < a.T ? cols - q * 8 * L : 0, L, f);
     }
-  };
-  int64_t id[kRows], next[kRows];
-  read_ids(u, id);
-  for (; u < a.units; u += stride) {
-    read_ids(u + stride, next);
-    const int c0 = (int)(u % a.slices) * (8 * kOcts) * L + (kVec ? l * 8 : l);
-    Oct<kTabF32, kVec> x[kRows][kOcts] = {};
-#pragma unroll
-    for (int r = 0; r < kRows; ++r) {
-      const bool live = id[r] >= 0 && id[r] < a.V && row_of(u, r) < a.T;
-      const uint8_t *row = a.table + (uint64_t)(uint32_t)(live ? id[r] : 0) * a.table_pitch;
-#pragma unroll
-      for (int q = 0; q < kOcts; ++q) {
-        const int c = c0 + q * 8 * L;
-        load_oct<kTabF32, kVec>(x[r][q], row + (int64_t)c * kTB, a.D - c, L, live);
-      }
-    }
-#pragma unroll
-    for (int r = 0; r < kRows; ++r) {
-      const int64_t t = row_of(u, r);
-      if (t >= a.T) continue;
-      if (id[r] >= a.V && c0 == 0) atomicOr(a.status, ANC_DEV_BAD_INDEX);
-      uint8_t *row = a.out + (uint64_t)t * a.out_pitch;
-#pragma unroll
-      for (int q = 0; q < kOcts; ++q) {
-        const int c = c0 + q * 8 * L;
-        float f[8];
-#pragma unroll
-        for (int k = 0; k < 8; ++k) f[k] = __fmul_rn(elem(x[r][q], k), a.scale);
-        store_oct<kOutF32, kVec>(row + (int64_t)c * kOB, a.D - c, L, f);
-      }
-    }
-#pragma unroll
-    for (int r = 0; r < kRows; ++r) id[r] = next[r];
   }
 }
 
@@ -869,7 +858,6 @@ embedding_small_kernel(RedArgs a, const void *__restrict__ ids, int ids64, int64
 }
 
 // ------------------------------------------------------------------ host side
-constexpr int kLookupBlocks = 8;             // of the lookup per SM
 constexpr int kMinPart = 4;                  // places per part at least
 constexpr int64_t kResident = 296;           // blocks of the sums that are resident at once, two per SM
 constexpr int kSortTarget = 4;               // rounds of 32 keys per warp the sort aims at
@@ -1041,18 +1029,18 @@ int anc_embedding_lookup(anc_ctx *ctx, const void *table, int table_dtype, int64
   LookupArgs a = {};
   a.table = (const uint8_t *)table; a.ids = ids; a.out = (uint8_t *)out;
   a.table_pitch = (uint32_t)(table_ld * (tf ? 4 : 2)); a.out_pitch = (uint32_t)(out_ld * (of ? 4 : 2));
-  a.T = T; a.V = V; a.ids64 = i64; a.D = (int)D; a.scale = scale; a.status = ctx->d_status;
+  a.T = (uint32_t)T; a.V = (uint32_t)V; a.ids64 = i64; a.D = (int)D; a.scale = scale; a.status = ctx->d_status;
   a.L = 1;
   while (a.L < 32 && a.L * 8 < D) a.L *= 2;
   const int64_t per_lane = (D + 8 * a.L - 1) / (8 * a.L);        // octets of a row
   const int octs = per_lane >= 3 ? 4 : (int)per_lane;
-  a.slices = (int)((per_lane + octs - 1) / octs);
+  const int64_t slices = (per_lane + octs - 1) / octs;
+  ANC_REQUIRE(slices <= 65535, "row length %lld out of range", (long long)D);
   const int64_t rows = (int64_t)(32 / a.L) * (4 / octs);         // per unit
-  a.units = (T + rows - 1) / rows * a.slices;
-  const int64_t blocks = std::min<int64_t>((a.units + kLookupThreads / 32 - 1) / (kLookupThreads / 32),
-                                           (int64_t)ctx->sm_count * kLookupBlocks);
+  a.units = (uint32_t)((T + rows - 1) / rows);
+  const dim3 blocks((unsigned)((a.units + kLookupThreads / 32 - 1) / (kLookupThreads / 32)), (unsigned)slices);
 #define ANC_LOOKUP(F, O, VEC, OCTS) \
-  embedding_lookup_kernel<F, O, VEC, OCTS><<<(unsigned)blocks, kLookupThreads, 0, st>>>(a)
+  embedding_lookup_kernel<F, O, VEC, OCTS><<<blocks, kLookupThreads, 0, st>>>(a)
 #define ANC_LOOKUP_O(F, O, VEC)                         \
   do {                                                  \
     if (octs == 4) ANC_LOOKUP(F, O, VEC, 4);            \
@@ -1165,8 +1153,9 @@ int anc_embedding_grad(anc_ctx *ctx, const void *dy, int dy_dtype, int64_t dy_ld
     ra.list = sa.list[(sa.passes - 1) & 1];
     const uint32_t most = sort_cluster(ctx->device);
     if (!most) return ANC_E_CUDA;
+    // one CTA as long as the list stays in its shared memory (4096 tokens: 10.3 us, two CTAs 12.4)
     uint32_t n_ctas = 1;
-    while (n_ctas < most && (int64_t)n_ctas * kSortThreads * kSortTarget < T) n_ctas *= 2;
+    while (T > kSortThreads * kSortRounds && n_ctas < most && (int64_t)n_ctas * kSortThreads * kSortTarget < T) n_ctas *= 2;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(n_ctas);
     cfg.blockDim = dim3(kSortThreads);
