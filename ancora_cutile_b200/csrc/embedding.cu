@@ -82,7 +82,8 @@ __device__ __forceinline__ int64_t load_id(const void *ids, int ids64, int64_t t
 }
 
 // ------------------------------------------------------------------ lookup
-// Bound by memory once two latencies (id, then row) are covered.  A warp takes 32 / L rows side by side, L lanes
+// Bound by memory once two latencies (id, then row) are covered: 32768 rows of 1024 bf16, 91 MB of distinct rows,
+// ids and output, take 15.3 us on the device, 131072 rows 59 us.  A warp takes 32 / L rows side by side, L lanes
 // a row, and every lane four octets: kOcts of a row, of 4 / kOcts rows.  Warps do one unit and leave: resident
 // ones that went on to further rows, with the next ids read ahead, were slower (131072 rows of 1024 bf16: 70
 // against 59 us; 32768: 20.4 against 18.7).
@@ -148,7 +149,7 @@ embedding_lookup_kernel(LookupArgs a) {
 // The passes are bound by latency, not by bytes: hence many CTAs with short stretches, all loads of a stretch
 // before their first use, and the ranks of a stretch of up to eight rounds kept in registers from the
 // counting to the writing.  Lanes of equal digit find each other by a word per digit in shared memory (nine
-// ballots or the match instruction took two to four times as long).  65536 tokens: 18.5 us, 2048: 8.9 us.
+// ballots or the match instruction took two to four times as long).  65536 tokens: 18.5 us, 16384: 14.4, 2048: 8.3.
 constexpr int kDigitBits = 9;
 constexpr int kDigits = 1 << kDigitBits;
 constexpr int kSortThreads = kDigits;              // a thread per digit
@@ -404,8 +405,9 @@ constexpr int kZeroThreads = 256;
 
 // When the whole table is written, what the SMs that do not sort do meanwhile.  Launched behind the sort without
 // waiting for it; it waits for the sort only before it ends, so that whoever waits for this kernel has the
-// sorted list too.  (Reading the first rows of dy into L2 at that time gave 3 us of 75 for 65536 rows of 1024
-// bf16 added to f32, cost 5 of 149 for 30000 rows of 4096 f32 and 9 of 66 beside the zeros.)
+// sorted list too.  311 MB of zeros: 48 us alone, 6.5 TB/s.  (Reading the first rows of dy into L2 at that time
+// gave 3 us of 75 for 65536 rows of 1024 bf16 added to f32, cost 5 of 149 for 30000 rows of 4096 f32 and 9 of 66
+// beside the zeros.)
 __global__ void __launch_bounds__(kZeroThreads)
 embedding_zero_kernel(ZeroArgs z, int64_t rows_per_block) {
   pdl_trigger();
@@ -541,7 +543,7 @@ struct Lane {
 // shared memory: every warp has asynchronous copies of the rows of the next kDepth places on the way and,
 // with "add", of the old table rows of the runs that end there (12 KB per warp, 192 KB per SM).  Loads ahead into
 // registers did not get there: they share six scoreboards, so waiting for one row waited for the newest
-// one too (accumulating 65536 rows of 1024: 63 us that way, 51 us by the ring, 5.8 TB/s).
+// one too (accumulating 65536 rows of 1024, 209 MB read and 44 written: 63 us that way, 50 us by the ring, 5.1 TB/s).
 //
 // kWide: 32 lanes per row and whole slices, so that nothing about columns is left to compute in the loop (198
 // instructions per place and warp without it, 140 with it).
@@ -876,7 +878,7 @@ Shape shape_of(int64_t T, int64_t D, bool vec) {
   s.slices = (int)((D + s.span - 1) / s.span);
   // As many places per part as fill the GPU's resident blocks evenly, in as few waves as the list of a piece
   // allows: a block has a start and an end without rows in flight (accumulating 65536 rows of 1024,
-  // sort included: 294 blocks 72.5 us, 1024 blocks 79 us).
+  // sort included: 293 blocks 72.7 us, 1024 blocks 81 us).
   const int64_t parts_per_cta = kRedThreads / s.L, longest = kMaxPiece / parts_per_cta;
   const int64_t wave = std::max<int64_t>(1, kResident / s.slices);
   const int64_t waves = (T + wave * kMaxPiece - 1) / (wave * kMaxPiece);
