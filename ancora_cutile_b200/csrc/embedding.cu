@@ -192,6 +192,11 @@ __device__ __forceinline__ uint32_t key_of(int64_t id, int64_t V, int64_t paddin
   return (id < 0 || id >= V || id == padding_idx) ? (uint32_t)V : (uint32_t)id;
 }
 
+// The order of the list: the last row of the table first, padding at the end.  Vocabularies have their frequent
+// tokens at the front; the long runs of those are the cheap pieces, and come last (65536 tokens, rows of 1024 bf16
+// added to f32, id = rank in frequency: 75 us against 82 in ascending order).
+__device__ __forceinline__ uint32_t reversed(uint32_t key, uint32_t V) { return key == V ? V : V - 1u - key; }
+
 struct SortShared {
   uint32_t cnt[kSortWarps][kDigits];     // per warp: counts, then places of the warp's first keys
   uint32_t lanes[kSortWarps][kDigits];   // per warp: the lanes that hold a digit, one round at a time
@@ -230,7 +235,7 @@ embedding_sort_kernel(SortArgs a, uint32_t n_ctas) {
       }
 #pragma unroll
       for (int r = 0; r < kSortRounds; ++r) {
-        e[r] = make_uint2(key_of(id[r], a.V, a.padding_idx), i0 + r * 32 + lane);
+        e[r] = make_uint2(reversed(key_of(id[r], a.V, a.padding_idx), (uint32_t)a.V), i0 + r * 32 + lane);
         bad = bad || id[r] >= a.V;
       }
     } else {
@@ -272,6 +277,7 @@ embedding_sort_kernel(SortArgs a, uint32_t n_ctas) {
     const int shift = p * kDigitBits;
     auto put = [&](uint32_t dst, uint2 e, bool on) {
       if (on) {
+        if (last) e.x = reversed(e.x, (uint32_t)a.V);
         if (single && !last) sh.list[dst] = e;
         else out[dst] = e;
       }
