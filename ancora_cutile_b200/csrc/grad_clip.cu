@@ -15,7 +15,7 @@
 // a true infinity or NaN in a gradient makes the norm infinite or NaN.
 //
 // Order.  Thread sums, the shuffle tree, the warps of a block, the blocks: all in an order that depends on
-// the table and the number of SMs alone, never on timing.  The last block to finish (an integer ticket)
+// the table, the number of SMs and the call (norm or clip) alone, never on timing.  The last block to finish (an integer ticket)
 // adds the block sums in index order, so one launch gives the norm.
 //
 // Launches.  The norm is one launch of resident blocks, each with an equal share of all vectors of all tensors.
@@ -37,6 +37,7 @@ constexpr int kThreads = 256;
 constexpr int kVecPerThread = 4;                              // vectors of 8 elements a thread has in flight
 constexpr int kChunkVec = kThreads * kVecPerThread;           // vectors per chunk of the scaling sweep
 constexpr int kChunkElems = kChunkVec * 8;
+constexpr uint64_t kReverseBytes = 400u << 20;                // gradients from which clipping sweeps backwards
 constexpr uint32_t kWaitPolls = 1u << 22;                     // of the one-launch clip; about a second
 
 // One tensor.  The norm reads elements [head, head + 8 * nvec) as vectors of eight aligned to their size (16
@@ -192,8 +193,8 @@ __device__ __forceinline__ void reduce_blocks(double acc, double *partial, uint3
 }
 
 // Bound by the read of the gradients: 1.19 GB of bf16 in 177 us, 0.87 GB of f32 in 135 us, 6.5 to 6.7 TB/s.  A
-// block's share is contiguous, so one search finds its first tensor.  As many blocks as are resident: twice or
-// sixteen times as many gained 2% for 1.19 GB and lost 10 to 25% for 60 to 200 MB.
+// block's share is contiguous, so one search finds its first tensor.  As many blocks as are resident: eight times as
+// many, 185 us.
 template <bool kF32>
 __global__ void __launch_bounds__(kThreads)
 grad_sumsq_kernel(const Entry *__restrict__ tab, uint32_t n_tab, uint64_t n_vec, double *__restrict__ partial,
@@ -311,13 +312,19 @@ grad_sumsq_chunk_kernel(const Entry *__restrict__ tab, uint32_t n_tab, double *p
 
 // A block per chunk, not resident blocks with a loop: blocks that start in address order keep DRAM streaming
 // (1.19 GB of bf16 in and out: 342 us, 7.0 TB/s, against 395-408 with 1184 resident blocks, 366 for a memcpy).
+//
+// Behind a norm over more than the L2 holds the sweep starts at the end of the arena, which the norm read last
+// (`reverse`); for that the norm's blocks have to go through the arena in address order too, eight waves of them.
+// Norm and sweep: 1.19 GB of bf16 538 us against 553, 0.87 GB of f32 to bf16 321 against 330, 0.6 GB 273 against
+// 281; but 0.26 GB 124 against 118.
 template <bool kF32, bool kOutF32>
 __global__ void __launch_bounds__(kThreads)
-grad_scale_kernel(const Entry *__restrict__ tab, uint32_t n_tab, const float *__restrict__ result, int in_place) {
+grad_scale_kernel(const Entry *__restrict__ tab, uint32_t n_tab, const float *__restrict__ result, int in_place,
+                  int reverse) {
   const float f = result[1];
   if (in_place && f == 1.0f) return;     // every element would be written back as it is
   Chunk<kF32, kOutF32> ch;
-  ch.load(tab, n_tab, blockIdx.x);
+  ch.load(tab, n_tab, reverse ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
   ch.store(f);
 }
 
@@ -381,7 +388,7 @@ struct anc_clip_plan {
   int grad_f32, out_f32, in_place;
   uint32_t n_tab;
   uint64_t n_vec, n_chunks;
-  uint32_t grid;             // blocks of the norm
+  uint32_t grid, clip_grid;  // blocks of the norm alone, and in front of the scaling sweep
   int fused;                 // all chunks resident at once: one launch clips
   uint8_t *d_mem;            // one allocation: table, block sums, sum of squares, ticket, result
   Entry *d_tab;
@@ -411,7 +418,7 @@ int check_scalars(float scale, float max_norm, float eps) {
   return ANC_OK;
 }
 
-int launch_sumsq(const anc_clip_plan *pl, const NormOut &o, int finish, cudaStream_t st) {
+int launch_sumsq(const anc_clip_plan *pl, uint32_t grid, const NormOut &o, int finish, cudaStream_t st) {
   if (pl->fused) {
     if (pl->grad_f32)
       grad_sumsq_chunk_kernel<true><<<(unsigned)pl->n_chunks, kThreads, 0, st>>>(pl->d_tab, pl->n_tab, pl->d_partial,
@@ -420,16 +427,16 @@ int launch_sumsq(const anc_clip_plan *pl, const NormOut &o, int finish, cudaStre
       grad_sumsq_chunk_kernel<false><<<(unsigned)pl->n_chunks, kThreads, 0, st>>>(pl->d_tab, pl->n_tab, pl->d_partial,
                                                                                   pl->d_ticket, o, finish);
   } else if (pl->grad_f32)
-    grad_sumsq_kernel<true><<<pl->grid, kThreads, 0, st>>>(pl->d_tab, pl->n_tab, pl->n_vec, pl->d_partial,
-                                                           pl->d_ticket, o, finish);
+    grad_sumsq_kernel<true><<<grid, kThreads, 0, st>>>(pl->d_tab, pl->n_tab, pl->n_vec, pl->d_partial, pl->d_ticket,
+                                                       o, finish);
   else
-    grad_sumsq_kernel<false><<<pl->grid, kThreads, 0, st>>>(pl->d_tab, pl->n_tab, pl->n_vec, pl->d_partial,
-                                                            pl->d_ticket, o, finish);
+    grad_sumsq_kernel<false><<<grid, kThreads, 0, st>>>(pl->d_tab, pl->n_tab, pl->n_vec, pl->d_partial, pl->d_ticket,
+                                                        o, finish);
   ANC_CUDA(cudaGetLastError());
   return ANC_OK;
 }
 
-using ScaleKernel = void (*)(const Entry *, uint32_t, const float *, int);
+using ScaleKernel = void (*)(const Entry *, uint32_t, const float *, int, int);
 using FusedKernel = void (*)(const Entry *, uint32_t, double *, uint32_t *, NormOut, int, uint32_t *);
 
 ScaleKernel scale_kernel(const anc_clip_plan *pl) {
@@ -441,9 +448,10 @@ FusedKernel fused_kernel(const anc_clip_plan *pl) {
   return pl->out_f32 ? grad_clip_fused_kernel<false, true> : grad_clip_fused_kernel<false, false>;
 }
 
-int launch_scale(const anc_clip_plan *pl, cudaStream_t st) {
+int launch_scale(const anc_clip_plan *pl, int reverse, cudaStream_t st) {
   if (pl->n_chunks == 0) return ANC_OK;
-  scale_kernel(pl)<<<(unsigned)pl->n_chunks, kThreads, 0, st>>>(pl->d_tab, pl->n_tab, pl->d_result, pl->in_place);
+  scale_kernel(pl)<<<(unsigned)pl->n_chunks, kThreads, 0, st>>>(pl->d_tab, pl->n_tab, pl->d_result, pl->in_place,
+                                                                reverse);
   ANC_CUDA(cudaGetLastError());
   return ANC_OK;
 }
@@ -542,8 +550,9 @@ int anc_clip_plan_create(anc_ctx *ctx, const anc_clip_tensor *tensors, int n_ten
   const uint64_t cap = (uint64_t)ctx->sm_count * (norm_per_sm > 0 ? norm_per_sm : 1);
   const uint64_t want = (vecs + kChunkVec - 1) / kChunkVec;
   pl->grid = (uint32_t)(want < cap ? (want ? want : 1) : cap);
+  pl->clip_grid = vecs * 8 * gs >= kReverseBytes ? pl->grid * 8 : pl->grid;
   pl->fused = chunks > 0 && chunks <= (uint64_t)fused_per_sm * ctx->sm_count;
-  const uint64_t n_part = pl->fused && chunks > pl->grid ? chunks : pl->grid;
+  const uint64_t n_part = pl->fused && chunks > pl->clip_grid ? chunks : pl->clip_grid;
   const size_t tab_bytes = (tab.size() * sizeof(Entry) + 255) / 256 * 256;
   const size_t part_bytes = ((size_t)n_part * sizeof(double) + 255) / 256 * 256;
   e = cudaMalloc((void **)&pl->d_mem, tab_bytes + part_bytes + 256);
@@ -577,13 +586,13 @@ int anc_grad_norm(anc_clip_plan *plan, float scale, float max_norm, float eps, v
   int rc = check_scalars(scale, max_norm, eps);
   if (rc) return rc;
   anc_device_guard guard(plan->ctx->device);
-  return launch_sumsq(plan, norm_out(plan, scale, max_norm, eps), 1, anc_pick_stream(plan->ctx, stream));
+  return launch_sumsq(plan, plan->grid, norm_out(plan, scale, max_norm, eps), 1, anc_pick_stream(plan->ctx, stream));
 }
 
 int anc_grad_sumsq(anc_clip_plan *plan, void *stream) {
   ANC_REQUIRE(plan, "plan is NULL");
   anc_device_guard guard(plan->ctx->device);
-  return launch_sumsq(plan, norm_out(plan, 1.f, INFINITY, 0.f), 0, anc_pick_stream(plan->ctx, stream));
+  return launch_sumsq(plan, plan->grid, norm_out(plan, 1.f, INFINITY, 0.f), 0, anc_pick_stream(plan->ctx, stream));
 }
 
 int anc_grad_norm_finish(anc_clip_plan *plan, float scale, float max_norm, float eps, void *stream) {
@@ -599,7 +608,7 @@ int anc_grad_norm_finish(anc_clip_plan *plan, float scale, float max_norm, float
 int anc_grad_apply(anc_clip_plan *plan, void *stream) {
   ANC_REQUIRE(plan, "plan is NULL");
   anc_device_guard guard(plan->ctx->device);
-  return launch_scale(plan, anc_pick_stream(plan->ctx, stream));
+  return launch_scale(plan, 0, anc_pick_stream(plan->ctx, stream));
 }
 
 int anc_grad_clip(anc_clip_plan *plan, float scale, float max_norm, float eps, void *stream) {
@@ -610,8 +619,8 @@ int anc_grad_clip(anc_clip_plan *plan, float scale, float max_norm, float eps, v
   cudaStream_t st = anc_pick_stream(plan->ctx, stream);
   const NormOut o = norm_out(plan, scale, max_norm, eps);
   if (!plan->fused) {
-    rc = launch_sumsq(plan, o, 1, st);
-    return rc ? rc : launch_scale(plan, st);
+    rc = launch_sumsq(plan, plan->clip_grid, o, 1, st);
+    return rc ? rc : launch_scale(plan, plan->clip_grid != plan->grid, st);
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)plan->n_chunks);

@@ -231,3 +231,52 @@ def test_caller_owned_result_two_plans_two_streams_and_a_graph(ctx):
     for b in ds + outs + [res]:
         b.free()
     assert ctx.status() == 0
+
+
+def _tile(pattern, start, n):
+    """n values of the endlessly repeated pattern from place ``start``."""
+    i = start % len(pattern)
+    return np.resize(np.concatenate([pattern[i:], pattern[:i]]), n)
+
+
+@pytest.mark.parametrize("g_dtype,in_place", [("bf16", False), ("bf16", True), ("f32", False)])
+def test_gradients_larger_than_the_sweep_backwards_starts_at(ctx, g_dtype, in_place):
+    """From 400 MiB of gradients on the scaling sweep goes backwards and the norm has more blocks: every element
+    scaled once, elements between the tensors untouched, norm and clip agreeing on the result."""
+    it = 2 if g_dtype == "bf16" else 4
+    sizes = [5, 60_000_011, 1, (440 << 20) // it - 60_100_000, 8192, 100_003]
+    offs, at = [], 3
+    for n in sizes:
+        offs.append(at)
+        at += n + 1
+    total = at + 16
+    pattern = (np.random.default_rng(6).standard_normal(999_983) * 1e-3).astype(np.float32)
+    small, vals = _dev(ctx, pattern, g_dtype)
+    bits = small.to_numpy()
+    small.free()
+    d = anc.DBuf(np.resize(bits, total), ctx)
+    out = d if in_place else anc.DBuf.zeros((total,), bits.dtype, ctx)
+    clip = anc.GradClip([dict(g=d.ptr + o * it, numel=n, out=out.ptr + o * it) for o, n in zip(offs, sizes)],
+                        grad_dtype=g_dtype, ctx=ctx)
+    sq = 0.0
+    one = np.square(vals.astype(np.float64))
+    for o, n in zip(offs, sizes):
+        whole, rest = divmod(n, len(vals))
+        sq += whole * math.fsum(one) + math.fsum(_tile(one, o + whole * len(vals), rest))
+    want = math.sqrt(sq)
+    clip.norm(0.25)
+    first = clip.read()
+    clip.clip(0.25)
+    got = clip.read()
+    for norm, factor in (first, got):
+        _check_norm((norm, factor), (want, 0.25 / (want + 1e-6)))
+    scaled = vals * np.float32(got[1])
+    scaled = obf.rne_bits(scaled) if g_dtype == "bf16" else scaled
+    result = out.to_numpy()
+    for o, n in zip(offs, sizes):
+        assert np.array_equal(result[o:o + n], _tile(scaled, o, n)), (o, n)
+        assert result[o - 1] == (bits[(o - 1) % len(bits)] if in_place else 0), o
+    clip.free()
+    if not in_place:
+        out.free()
+    d.free()
