@@ -1103,8 +1103,9 @@ int anc_embedding_grad(anc_ctx *ctx, const void *dy, int dy_dtype, int64_t dy_ld
     ANC_REQUIRE(!overlap(dw, V, dw_ld, wf ? 4 : 2, D, dy, row_span(T, dy_ld, yf ? 4 : 2, D)) &&
                     !overlap(dw, V, dw_ld, wf ? 4 : 2, D, ids, T * (i64 ? 8 : 4)) &&
                     !overlap(dw, V, dw_ld, wf ? 4 : 2, D, work, (int64_t)workspace_of(T, D).total) &&
-                    !overlap(dy, T, dy_ld, yf ? 4 : 2, D, work, (int64_t)workspace_of(T, D).total),
-                "dw overlaps an input");
+                    !overlap(dy, T, dy_ld, yf ? 4 : 2, D, work, (int64_t)workspace_of(T, D).total) &&
+                    !overlap(ids, 1, 0, i64 ? 8 : 4, T, work, (int64_t)workspace_of(T, D).total),
+                "dw or the workspace overlaps another buffer");
   }
   const Workspace ws = workspace_of(T, D);
   ANC_REQUIRE(T == 0 || work_bytes >= ws.total, "workspace of %llu bytes, %llu are needed",

@@ -511,11 +511,12 @@ int anc_clip_plan_create(anc_ctx *ctx, const anc_clip_tensor *tensors, int n_ten
       ANC_REQUIRE(chunks <= 0x7FFFFFFF, "tensors too large for one plan");
       tab.push_back(e);
     }
+    if (result) spans.push_back({(uintptr_t)result, (uintptr_t)result + 2 * sizeof(float), true});
     std::sort(spans.begin(), spans.end(), [](const Span &a, const Span &b) { return a.lo < b.lo; });
     Span reach = {0, 0, false}, written = {0, 0, false};     // furthest-reaching spans so far: any, written
     for (const Span &s : spans) {
       ANC_REQUIRE(!(s.written && s.lo < reach.hi) && s.lo >= written.hi,
-                  "a clipped tensor would overlap another tensor of the plan");
+                  "a clipped tensor or the result would overlap another tensor of the plan");
       if (s.hi > reach.hi) reach = s;
       if (s.written && s.hi > written.hi) written = s;
     }

@@ -360,13 +360,14 @@ ANC_API int anc_grad_accumulate(anc_ctx *ctx, float *acc, const void *src, int s
  *
  * A plan holds the table of gradient tensors (one type for all, any alignment, sizes from 0) and the block
  * sums of the reduction.  `out` NULL clips in place; an output must not overlap another tensor or output of
- * the plan, so a tensor is listed once.
+ * the plan, so a tensor is listed once, and `result` none of them.
  * {norm, factor} are two floats in device memory: `result` when given, else inside the plan.  Squares are summed
  * in float32 by eights and in float64 above, in a fixed order: the same bits every time on one device.  A
  * NaN in a gradient makes norm and factor NaN, an infinity makes norm infinite and factor 0;
  * max_norm = +inf never clips.  anc_grad_clip waits between blocks on the device where the plan is small; should
- * that wait run out (status bit 0x10), norm and factor are NaN and the gradients are as they were.  Calls on one plan must be ordered among themselves (they share its block
- * sums and its result); calls on different plans need not be.  All calls can be captured into a graph. */
+ * that wait run out (status bit 0x10), norm and factor are NaN and the gradients are as they were.  Calls on one
+ * plan must be ordered among themselves (they share its block sums and its result); calls on different plans need
+ * not be.  All calls can be captured into a graph. */
 typedef struct anc_clip_plan anc_clip_plan;
 typedef struct anc_clip_tensor {
   const void *g;   /* gradient, of the plan's grad_dtype                      */
@@ -405,10 +406,10 @@ ANC_API int anc_embedding_lookup(anc_ctx *ctx, const void *table, int table_dtyp
 #define ANC_EMBED_WRITE 0 /* dw[v,:] = round(scale * S_v) for every row, zero where no token names v   */
 #define ANC_EMBED_ADD 1   /* dw[v,:] = round(dw[v,:] + scale * S_v) for the rows named, others untouched */
 /* S_v = sum of dy[t,:] over the tokens t with ids[t] == v and v != padding_idx (< 0: none), in an order that
- * the ids, the sizes and the alignment fix: the same bits every time.  dw may overlap none of the others.
- * Blocks that finish a row wait, with a limit (status bit 0x10), for the blocks that hold its other tokens.  `work`: caller-owned scratch of at least
- * anc_embedding_grad_workspace(T, V, D) bytes, 16-byte aligned, contents unspecified; calls that may overlap on
- * the GPU need one each. */
+ * the ids, the sizes and the alignment fix: the same bits every time.  dw and work may overlap none of the others.
+ * Blocks that finish a row wait, with a limit (status bit 0x10), for the blocks that hold its other tokens.
+ * `work`: caller-owned scratch of at least anc_embedding_grad_workspace(T, V, D) bytes, 16-byte aligned, contents
+ * unspecified; calls that may overlap on the GPU need one each. */
 ANC_API int anc_embedding_grad_workspace(int64_t T, int64_t V, int64_t D, uint64_t *bytes);
 ANC_API int anc_embedding_grad(anc_ctx *ctx, const void *dy, int dy_dtype, int64_t dy_ld, const void *ids,
                                int ids_dtype, void *dw, int dw_dtype, int64_t dw_ld, int64_t T, int64_t V, int64_t D,

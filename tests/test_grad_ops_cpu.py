@@ -33,6 +33,8 @@ def _clip_plan(tensors, grad=L.GRAD_BF16, out=L.GRAD_BF16, result=None, ctx=FAKE
     ([(4096, 8192, 64), (8200, 16384, 64)], {}, b"overlap"),
     ([(4096, 8192, 64), (16384, 8256, 64)], {}, b"overlap"),
     ([(4096, None, 64), (4160, None, 64)], {}, b"overlap"),
+    ([(4096, 8192, 64)], dict(result=8192), b"overlap"),
+    ([(4096, 8192, 64)], dict(result=4220), b"overlap"),
     ([(4096, None, (1 << 63))], {}, b"numel"),
 ])
 def test_clip_plan_refusals(tensors, kw, msg):
@@ -87,7 +89,7 @@ def _grad(ctx=FAKE, dy=4096, yd=0, yld=0, ids=1 << 21, idt=L.IDS_I64, dw=1 << 20
 
 @pytest.mark.parametrize("kw", [
     dict(dw=4096), dict(dw=8192, dy=8240), dict(dw=8192, ids=8248), dict(dw=1 << 20, work=(1 << 20) - 256),
-    dict(dy=1 << 20, work=(1 << 20) - 256),
+    dict(dy=1 << 20, work=(1 << 20) - 256), dict(work=(1 << 21) - 256), dict(work=1 << 21),
     dict(ctx=None), dict(dy=None), dict(ids=None), dict(dw=None), dict(work=None), dict(work=(1 << 24) + 8), dict(yd=3),
     dict(wd=-1), dict(idt=2), dict(mode=2), dict(dy=4097), dict(dw=4098, wd=1), dict(ids=4100), dict(yld=7),
     dict(wld=7), dict(T=-1), dict(T=1 << 31), dict(V=0), dict(V=(1 << 31) - 1), dict(D=0), dict(D=(1 << 24) + 1),
