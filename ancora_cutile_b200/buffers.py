@@ -15,13 +15,12 @@ from . import _lib as L
 
 _contexts = {}
 _default_device = None
-_default_context = None        # what get_context() returned last
 
 
 def set_device(device):
     """Selects the GPU used by contexts created without an explicit device."""
-    global _default_device, _default_context
-    _default_device, _default_context = int(device), None
+    global _default_device
+    _default_device = int(device)
 
 
 def default_device():
@@ -72,14 +71,9 @@ class Context:
 
 def get_context(device=None):
     """Process-wide context per device (the reference is one model per process)."""
-    global _default_context
-    if device is None and _default_context is not None:
-        return _default_context
     d = default_device() if device is None else int(device)
     if d not in _contexts:
         _contexts[d] = Context(d)
-    if device is None:
-        _default_context = _contexts[d]
     return _contexts[d]
 
 

@@ -119,6 +119,18 @@ def test_buffers_that_know_their_size_are_held_to_it():
         kernels.embedding_grad(**dict(ok, dw_ld=9))
 
 
+def test_default_context_follows_the_selected_device(monkeypatch):
+    from ancora_cutile_b200 import buffers
+    monkeypatch.setattr(buffers, "_contexts", {d: f"context {d}" for d in range(3)})
+    monkeypatch.setattr(buffers, "_default_device", None)
+    monkeypatch.delenv("LOCAL_RANK", raising=False)
+    assert buffers.get_context() == "context 0"
+    monkeypatch.setenv("LOCAL_RANK", "2")
+    assert buffers.get_context() == "context 2"
+    buffers.set_device(1)
+    assert buffers.get_context() == "context 1" and buffers.get_context(0) == "context 0"
+
+
 def test_adding_no_tokens_is_nothing():
     assert _grad(T=0, dy=None, ids=None, work=None, wb=0) == 0
 
