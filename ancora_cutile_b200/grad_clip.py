@@ -13,6 +13,15 @@ from . import _lib as L
 from .buffers import dev_ptr, get_context
 
 _GRAD = {"bf16": L.GRAD_BF16, "f32": L.GRAD_F32}
+_SIZE = {"bf16": 2, "f32": 4}
+
+
+def _buf(obj, numel, dtype, what):
+    """Address of ``obj``; a buffer that knows its size must hold ``numel`` elements."""
+    n = getattr(obj, "nbytes", None)
+    if n is not None and n < numel * _SIZE[dtype]:
+        raise ValueError(f"{what} holds {n} bytes: too few for {numel} {dtype}")
+    return dev_ptr(obj)
 
 
 class GradClip:
@@ -30,10 +39,14 @@ class GradClip:
         self.grad_dtype, self.out_dtype = grad_dtype, out_dtype or grad_dtype
         arr = (L.ClipTensor * max(len(tensors), 1))()
         for i, t in enumerate(tensors):
-            arr[i] = L.ClipTensor(dev_ptr(t["g"]), dev_ptr(t.get("out")), int(t["numel"]))
+            n = int(t["numel"])
+            if n < 0:
+                raise ValueError(f"tensor {i}: numel {n}")
+            arr[i] = L.ClipTensor(_buf(t["g"], n, self.grad_dtype, f"tensor {i}: g"),
+                                  _buf(t.get("out"), n, self.out_dtype, f"tensor {i}: out"), n)
         h = C.c_void_p()
         L.check(L.lib().anc_clip_plan_create(self.ctx.handle, arr, len(tensors), _GRAD[self.grad_dtype],
-                                             _GRAD[self.out_dtype], dev_ptr(result), C.byref(h)))
+                                             _GRAD[self.out_dtype], _buf(result, 2, "f32", "result"), C.byref(h)))
         self.handle = h
         r, s = C.c_void_p(), C.c_void_p()
         L.check(L.lib().anc_clip_plan_result(self.handle, C.byref(r), C.byref(s)))

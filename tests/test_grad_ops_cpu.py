@@ -119,6 +119,24 @@ def test_buffers_that_know_their_size_are_held_to_it():
         kernels.embedding_grad(**dict(ok, dw_ld=9))
 
 
+def test_clip_buffers_that_know_their_size_are_held_to_it():
+    class Buf:
+        def __init__(self, nbytes, ptr):
+            self.ptr, self.nbytes = ptr, nbytes
+
+    class Ctx:
+        handle = None                       # refused by the library, after the sizes were looked at
+    from ancora_cutile_b200 import AncoraError, GradClip
+    for g, out, result, what in ((15, 32, 8, "g"), (16, 31, 8, "out"), (16, 32, 7, "result")):
+        with pytest.raises(ValueError, match=what):
+            GradClip([dict(g=Buf(g, 4096), out=Buf(out, 8192), numel=8)], out_dtype="f32", result=Buf(result, 1 << 14),
+                     ctx=Ctx)
+    with pytest.raises(AncoraError):
+        GradClip([dict(g=Buf(16, 4096), out=Buf(32, 8192), numel=8)], out_dtype="f32", result=Buf(8, 1 << 14), ctx=Ctx)
+    with pytest.raises(ValueError, match="numel"):
+        GradClip([dict(g=4096, numel=-1)], ctx=Ctx)
+
+
 def test_default_context_follows_the_selected_device(monkeypatch):
     from ancora_cutile_b200 import buffers
     monkeypatch.setattr(buffers, "_contexts", {d: f"context {d}" for d in range(3)})
