@@ -14,9 +14,9 @@
 // [2^-90, 2^120] is summed again in float64, so that gradients of 1e-25 or 1e25 keep their norm; only
 // a true infinity or NaN in a gradient makes the norm infinite or NaN.
 //
-// Order.  Thread sums, the shuffle tree, the warps of a block, the blocks: all in an order that depends on
-// the table, the number of SMs and the call (norm or clip) alone, never on timing.  The last block to finish (an integer ticket)
-// adds the block sums in index order, so one launch gives the norm.
+// Order.  Thread sums, the shuffle tree, the warps of a block, the blocks: all in an order that depends on the
+// table, the number of SMs and the call (norm or clip) alone, never on timing.  The last block to finish (an
+// integer ticket) adds the block sums in index order, so one launch gives the norm.
 //
 // Launches.  The norm is one launch of resident blocks, each with an equal share of all vectors of all tensors.
 // Clipping reads the gradients twice (the factor is known only after all of them), in two launches; what

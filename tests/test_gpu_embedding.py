@@ -125,6 +125,21 @@ def test_ids_outside_the_table_are_reported_and_touch_nothing(ctx):
     w.free()
 
 
+@pytest.mark.parametrize("T", [500, 5000])
+@pytest.mark.parametrize("mode", ["write", "add"])
+def test_long_lists_with_ids_outside_the_table(ctx, T, mode):
+    V, D = 70, 24
+    rng = np.random.default_rng(T)
+    ids = rng.integers(-3, V, T)
+    ids[[0, 77, T - 1]] = V, 2 ** 40, V + 1
+    dy = rng.integers(-8, 9, (T, D)).astype(np.float32)
+    dy[(ids < 0) | (ids >= V)] = np.nan                    # rows of no id are not read
+    old = rng.integers(-8, 9, (V, D)).astype(np.float32)
+    got, _, _, _ = _run_grad(ctx, dy, ids, V, 1.0, "f32", "f32", mode, old)
+    assert np.array_equal(got, embed_ref.grad(dy, ids, V, 1.0, old if mode == "add" else None)[0].astype(np.float32))
+    assert ctx.status() == 0x8
+
+
 def _run_grad(ctx, dy, ids, V, scale, dy_dtype, dw_dtype, mode, old, padding_idx=None, ids_dtype="i64"):
     T, D = dy.shape
     d_dy, dyv = _dev(ctx, dy, dy_dtype)
@@ -222,6 +237,25 @@ def test_padding_idx_and_special_values(ctx):
     assert np.isnan(got[row, 3]) and got[row, 4] == -np.inf
     got[row, 3:5] = 0
     assert np.isfinite(got).all()
+
+
+@pytest.mark.parametrize("T", [129, 255, 4095, 4096, 4097, 8193])
+@pytest.mark.parametrize("V,D", [(260, 40), (32768, 256), (32769, 256), (300000, 128)])
+def test_list_by_counting_and_by_sorting(ctx, T, V, D):
+    """Sizes on either side of where the list is counted instead of sorted (tokens, and zeros to write): integer
+    sums are exact, every row of a written table is defined,."""
+    rng = np.random.default_rng(T + V)
+    ids = _ids(rng, T, V, "zipf")
+    ids[::7] = V - 1 - ids[::7]
+    ids[5::11] = -1
+    dy = rng.integers(-8, 9, (T, D)).astype(np.float32)
+    old = rng.integers(-100, 101, (V, D)).astype(np.float32)
+    for mode in ("write", "add"):
+        want, _, _ = embed_ref.grad(dy, ids, V, 2.0, old if mode == "add" else None)
+        for ids_dtype in ("i32", "i64"):
+            got, _, _, _ = _run_grad(ctx, dy, ids, V, 2.0, "bf16", "f32", mode, old, ids_dtype=ids_dtype)
+            assert np.array_equal(got, want.astype(np.float32)), (mode, ids_dtype)
+    assert ctx.status() == 0
 
 
 @pytest.mark.parametrize("offset,dy_ld,dw_ld", [(0, 40, 48), (1, 33, 41), (8, 64, 32), (3, 32, 40)])
