@@ -15,6 +15,7 @@
 #include <algorithm>
 #include <cuda_bf16.h>
 #include <initializer_list>
+#include <math.h>
 #include <type_traits>
 #include <mutex>
 #include "anc_internal.h"
@@ -83,10 +84,11 @@ __device__ __forceinline__ int64_t load_id(const void *ids, int ids64, int64_t t
 
 // ------------------------------------------------------------------ lookup
 // Bound by memory once two latencies (id, then row) are covered: 32768 rows of 1024 bf16, 91 MB of distinct rows,
-// ids and output, take 15.3 us on the device, 131072 rows 59 us.  A warp takes 32 / L rows side by side, L lanes
-// a row, and every lane four octets: kOcts of a row, of 4 / kOcts rows.  Warps do one unit and leave: resident
-// ones that went on to further rows, with the next ids read ahead, were slower (131072 rows of 1024 bf16: 70
-// against 59 us; 32768: 20.4 against 18.7).
+// ids and output, take 15.3 us on the device, 131072 rows 59 us.  A warp takes 32 / L rows side by side, L lanes a
+// row, and every lane up to four octets: kOcts of a row, of 4 / kOcts rows; rows longer than four octets a lane
+// are cut into slices as equal as that allows (53579 rows of 1303 bf16: two slices of three octets 62 us, of four
+// and two 76).  Warps do one unit and leave: resident ones that went on to further rows, with the next ids read
+// ahead, were slower (131072 rows of 1024 bf16: 70 against 59 us; 32768: 20.4 against 18.7).
 constexpr int kLookupThreads = 128;
 
 struct LookupArgs {
@@ -383,27 +385,28 @@ embedding_sort_kernel(SortArgs a, uint32_t n_ctas) {
 struct ZeroArgs {
   uint8_t *dw;
   int64_t row_bytes, pitch, V;
-  int vec;                       // rows are 16-byte aligned vectors
+  int64_t rows, bytes;           // of one part: whole rows, or where rows leave no gaps `bytes` of the table
+  uint32_t parts;
 };
 
-// zeros in rows [first, last) by the threads of one block
-__device__ __forceinline__ void zero_rows(const ZeroArgs &z, int64_t first, int64_t last) {
-  const uint32_t per = (uint32_t)(z.vec ? z.row_bytes / 16 : z.row_bytes / 2);
-  const int64_t n = (last - first) * per;
-  if (z.vec && z.pitch == z.row_bytes) {
-    uint4 *p = reinterpret_cast<uint4 *>(z.dw + first * z.pitch);
-    for (int64_t i = threadIdx.x; i < n; i += blockDim.x) p[i] = make_uint4(0u, 0u, 0u, 0u);
-    return;
-  }
-  for (int64_t i0 = 0; i0 < n; i0 += (int64_t)1 << 30) {      // 32-bit division inside
-    const int64_t row0 = first + i0 / per;
-    const uint32_t rem = (uint32_t)(i0 % per), m = (uint32_t)(n - i0 < ((int64_t)1 << 30) ? n - i0 : (int64_t)1 << 30);
-    for (uint32_t i = threadIdx.x; i < m; i += blockDim.x) {
-      const uint32_t r = (rem + i) / per, c = rem + i - r * per;
-      uint8_t *p = z.dw + (row0 + r) * z.pitch;
-      if (z.vec) *reinterpret_cast<uint4 *>(p + (int64_t)c * 16) = make_uint4(0u, 0u, 0u, 0u);
-      else *reinterpret_cast<uint16_t *>(p + (int64_t)c * 2) = 0;
-    }
+// zeros in n bytes at p by the threads of one block, 16 at a time between the first and the last 16-byte boundary
+__device__ __forceinline__ void zero_bytes(uint8_t *p, int64_t n) {
+  const int64_t to_16 = (16 - ((uintptr_t)p & 15)) & 15, head = to_16 < n ? to_16 : n;
+  const int64_t vecs = (n - head) / 16, tail = head + vecs * 16;
+  uint4 *q = reinterpret_cast<uint4 *>(p + head);
+  for (int64_t i = threadIdx.x; i < vecs; i += blockDim.x) q[i] = make_uint4(0u, 0u, 0u, 0u);
+  const int64_t mine = (int64_t)threadIdx.x * 2;
+  if (mine < head) *reinterpret_cast<uint16_t *>(p + mine) = 0;
+  if (tail + mine < n) *reinterpret_cast<uint16_t *>(p + tail + mine) = 0;
+}
+
+__device__ __forceinline__ void zero_part(const ZeroArgs &z, int64_t k) {
+  if (z.pitch == z.row_bytes) {
+    const int64_t lo = k * z.bytes, left = z.V * z.row_bytes - lo;
+    zero_bytes(z.dw + lo, left < z.bytes ? left : z.bytes);
+  } else {
+    const int64_t v1 = (k + 1) * z.rows < z.V ? (k + 1) * z.rows : z.V;
+    for (int64_t v = k * z.rows; v < v1; ++v) zero_bytes(z.dw + v * z.pitch, z.row_bytes);
   }
 }
 
@@ -440,7 +443,7 @@ embedding_rank_kernel(SortArgs a, ZeroArgs z) {
       if (id[k] >= a.V && blockIdx.x == 0) atomicOr(a.status, ANC_DEV_BAD_INDEX);
     }
   }
-  zero_rows(z, z.V * blockIdx.x / gridDim.x, z.V * (blockIdx.x + 1) / gridDim.x);
+  for (int64_t k = blockIdx.x; k < z.parts; k += gridDim.x) zero_part(z, k);
   __syncthreads();
   const uint32_t n_warps = gridDim.x * (kRankThreads / 32);
   for (uint32_t t0 = (blockIdx.x * (kRankThreads / 32) + (tid >> 5)) * kRankTokens; t0 < a.T;
@@ -482,10 +485,9 @@ constexpr int kZeroThreads = 256;
 // gave 3 us of 75 for 65536 rows of 1024 bf16 added to f32, cost 5 of 149 for 30000 rows of 4096 f32 and 9 of 66
 // beside the zeros.)
 __global__ void __launch_bounds__(kZeroThreads)
-embedding_zero_kernel(ZeroArgs z, int64_t rows_per_block) {
+embedding_zero_kernel(ZeroArgs z) {
   pdl_trigger();
-  const int64_t first = blockIdx.x * rows_per_block, last = first + rows_per_block < z.V ? first + rows_per_block : z.V;
-  zero_rows(z, first, last);
+  zero_part(z, blockIdx.x);
   pdl_wait();
 }
 
@@ -933,10 +935,15 @@ embedding_small_kernel(RedArgs a, const void *__restrict__ ids, int ids64, int64
 }
 
 // ------------------------------------------------------------------ host side
+// Lanes per row at least, however short the rows: fewer lanes are more and shorter parts, and joining the runs of a
+// block goes from part to part (rows of 8 f32: 3085 tokens 15.6 us against 26.9 with one lane a row, 131072 43
+// against 64; rows of 56: 41 against 43, with 16 lanes 46).
+constexpr int kMinLanes = 8;
 constexpr int kMinPart = 4;                  // places per part at least
 constexpr int64_t kResident = 296;           // blocks of the sums that are resident at once, two per SM
 constexpr int kSortTarget = 4;               // rounds of 32 keys per warp the sort aims at
-constexpr int64_t kZeroBytes = 128 << 10;    // zeros per block
+constexpr int64_t kZeroBytes = 128 << 10;    // zeros per block at most
+constexpr int64_t kZeroParts = 592;          // blocks a small table's zeros are spread over (0.5 MB: 13 us, in four blocks 17)
 constexpr int64_t kRankZeroBytes = 32 << 20; // zeros the counting kernel writes itself; more hide a sort beside them
 struct Shape {
   int L, slices, per_part, span;      // span: columns of a slice
@@ -946,7 +953,7 @@ struct Shape {
 Shape shape_of(int64_t T, int64_t D, bool vec) {
   const int each = vec ? Cols<true>::kEach : Cols<false>::kEach;
   Shape s;
-  s.L = 1;
+  s.L = kMinLanes;
   while (s.L < 32 && s.L * each < D) s.L *= 2;
   s.span = s.L * each;
   s.slices = (int)((D + s.span - 1) / s.span);
@@ -1086,6 +1093,7 @@ int anc_embedding_lookup(anc_ctx *ctx, const void *table, int table_dtype, int64
   if (!rc) rc = check_dtype(out_dtype, "out_dtype");
   if (rc) return rc;
   ANC_REQUIRE(ids_dtype == ANC_IDS_I32 || ids_dtype == ANC_IDS_I64, "bad ids_dtype %d", ids_dtype);
+  ANC_REQUIRE(isfinite(scale), "scale must be finite");
   if (T == 0) return ANC_OK;
   ANC_REQUIRE(table && ids && out, "NULL argument");
   if (table_ld == 0) table_ld = D;
@@ -1109,8 +1117,8 @@ int anc_embedding_lookup(anc_ctx *ctx, const void *table, int table_dtype, int64
   a.L = 1;
   while (a.L < 32 && a.L * 8 < D) a.L *= 2;
   const int64_t per_lane = (D + 8 * a.L - 1) / (8 * a.L);        // octets of a row
-  const int octs = per_lane >= 3 ? 4 : (int)per_lane;
-  const int64_t slices = (per_lane + octs - 1) / octs;
+  const int64_t slices = (per_lane + 3) / 4;
+  const int octs = (int)((per_lane + slices - 1) / slices);
   ANC_REQUIRE(slices <= 65535, "row length %lld out of range", (long long)D);
   const int64_t rows = (int64_t)(32 / a.L) * (4 / octs);         // per unit
   a.units = (uint32_t)((T + rows - 1) / rows);
@@ -1120,6 +1128,7 @@ int anc_embedding_lookup(anc_ctx *ctx, const void *table, int table_dtype, int64
 #define ANC_LOOKUP_O(F, O, VEC)                         \
   do {                                                  \
     if (octs == 4) ANC_LOOKUP(F, O, VEC, 4);            \
+    else if (octs == 3) ANC_LOOKUP(F, O, VEC, 3);       \
     else if (octs == 2) ANC_LOOKUP(F, O, VEC, 2);       \
     else ANC_LOOKUP(F, O, VEC, 1);                      \
   } while (0)
@@ -1156,6 +1165,7 @@ int anc_embedding_grad(anc_ctx *ctx, const void *dy, int dy_dtype, int64_t dy_ld
   if (!rc) rc = check_dtype(dw_dtype, "dw_dtype");
   if (rc) return rc;
   ANC_REQUIRE(ids_dtype == ANC_IDS_I32 || ids_dtype == ANC_IDS_I64, "bad ids_dtype %d", ids_dtype);
+  ANC_REQUIRE(isfinite(scale), "scale must be finite");
   ANC_REQUIRE(mode == ANC_EMBED_WRITE || mode == ANC_EMBED_ADD, "bad mode %d", mode);
   if (dy_ld == 0) dy_ld = D;
   if (dw_ld == 0) dw_ld = D;
@@ -1186,20 +1196,24 @@ int anc_embedding_grad(anc_ctx *ctx, const void *dy, int dy_dtype, int64_t dy_ld
   za.row_bytes = D * (wf ? 4 : 2);
   za.pitch = dw_ld * (wf ? 4 : 2);
   za.V = V;
-  za.vec = ((uintptr_t)dw & 15) == 0 && za.pitch % 16 == 0 && za.row_bytes % 16 == 0;
+  const int64_t zeros = V * za.row_bytes, even = (zeros + kZeroParts - 1) / kZeroParts;
+  za.bytes = std::min(kZeroBytes, (even + 4095) / 4096 * 4096);
+  za.rows = std::max<int64_t>(1, za.bytes / za.row_bytes);
+  const int64_t parts = za.pitch == za.row_bytes ? (zeros + za.bytes - 1) / za.bytes : (V + za.rows - 1) / za.rows;
+  ANC_REQUIRE(parts <= 0x7FFFFFFF, "V x D too large");
+  za.parts = (uint32_t)parts;
   const bool write = mode == ANC_EMBED_WRITE, small = T <= kSmallT;
   cudaLaunchAttribute pdl[1];
   pdl[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   pdl[0].val.programmaticStreamSerializationAllowed = 1;
   auto launch_zero = [&](int n_attrs) {
-    const int64_t per_block = za.row_bytes < kZeroBytes ? kZeroBytes / za.row_bytes : 1;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)((V + per_block - 1) / per_block));
+    cfg.gridDim = dim3(za.parts);
     cfg.blockDim = dim3(kZeroThreads);
     cfg.stream = st;
     cfg.attrs = pdl;
     cfg.numAttrs = n_attrs;
-    return cudaLaunchKernelEx(&cfg, embedding_zero_kernel, za, per_block);
+    return cudaLaunchKernelEx(&cfg, embedding_zero_kernel, za);
   };
   if (write && small) ANC_CUDA(launch_zero(0));
   if (T == 0) return ANC_OK;
@@ -1233,7 +1247,7 @@ int anc_embedding_grad(anc_ctx *ctx, const void *dy, int dy_dtype, int64_t dy_ld
       ra.list = sa.list[0];
       const int64_t per_cta = kRankThreads / 32 * kRankTokens, want = (T + per_cta - 1) / per_cta;
       const unsigned grid = (unsigned)(write || want > ctx->sm_count ? ctx->sm_count : want);
-      if (!write) za.V = 0;
+      if (!write) za.parts = 0;
       const size_t keys = (T + 127) / 128 * 128 * sizeof(uint32_t);
       embedding_rank_kernel<<<grid, kRankThreads, keys, st>>>(sa, za);
       ANC_CUDA(cudaGetLastError());

@@ -73,7 +73,8 @@ def _lookup(ctx=FAKE, table=4096, td=0, tld=0, ids=1 << 20, idt=L.IDS_I64, out=1
     dict(out=4096), dict(out=4098), dict(out=1 << 21, ids=(1 << 21) + 8),
     dict(ctx=None), dict(table=None), dict(ids=None), dict(out=None), dict(td=3), dict(od=-1), dict(idt=2),
     dict(table=4097), dict(out=4098, od=1), dict(ids=4100), dict(ids=4098, idt=L.IDS_I32), dict(tld=7), dict(old=7),
-    dict(T=-1), dict(T=1 << 31), dict(V=0), dict(V=(1 << 31) - 1), dict(D=0), dict(D=(1 << 24) + 1)])
+    dict(T=-1), dict(T=1 << 31), dict(V=0), dict(V=(1 << 31) - 1), dict(D=0), dict(D=(1 << 24) + 1),
+    dict(scale=math.nan), dict(scale=math.inf)])
 def test_lookup_refusals(kw):
     assert _lookup(**kw) == L.E_INVALID
 
@@ -93,7 +94,7 @@ def _grad(ctx=FAKE, dy=4096, yd=0, yld=0, ids=1 << 21, idt=L.IDS_I64, dw=1 << 20
     dict(ctx=None), dict(dy=None), dict(ids=None), dict(dw=None), dict(work=None), dict(work=(1 << 24) + 8), dict(yd=3),
     dict(wd=-1), dict(idt=2), dict(mode=2), dict(dy=4097), dict(dw=4098, wd=1), dict(ids=4100), dict(yld=7),
     dict(wld=7), dict(T=-1), dict(T=1 << 31), dict(V=0), dict(V=(1 << 31) - 1), dict(D=0), dict(D=(1 << 24) + 1),
-    dict(wb=16)])
+    dict(wb=16), dict(scale=math.nan), dict(scale=-math.inf)])
 def test_embedding_grad_refusals(kw):
     assert _grad(**kw) == L.E_INVALID
 
