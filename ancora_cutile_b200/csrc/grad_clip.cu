@@ -18,7 +18,7 @@
 // table, the number of SMs and the call (norm or clip) alone, never on timing.  The last block to finish (an
 // integer ticket) adds the block sums in index order, so one launch gives the norm.
 //
-// Launches.  The norm is one launch of resident blocks, each with an equal share of all vectors of all tensors.
+// Launches.  The norm is one launch of resident blocks that share the vectors of all tensors piece by piece.
 // Clipping reads the gradients twice (the factor is known only after all of them), in two launches; what
 // fits the registers of the resident blocks is read once, in one launch whose blocks wait for one
 // another between the two halves.
@@ -37,7 +37,8 @@ constexpr int kThreads = 256;
 constexpr int kVecPerThread = 4;                              // vectors of 8 elements a thread has in flight
 constexpr int kChunkVec = kThreads * kVecPerThread;           // vectors per chunk of the scaling sweep
 constexpr int kChunkElems = kChunkVec * 8;
-constexpr uint64_t kReverseBytes = 400u << 20;                // gradients from which clipping sweeps backwards
+constexpr uint64_t kPieceVec = 2 * kChunkVec;                 // vectors per piece of the norm
+constexpr uint64_t kManyBytes = 400u << 20;                   // gradients from which a clip's norm has more blocks
 constexpr uint32_t kWaitPolls = 1u << 22;                     // of the one-launch clip; about a second
 
 // One tensor.  The norm reads elements [head, head + 8 * nvec) as vectors of eight aligned to their size (16
@@ -192,16 +193,16 @@ __device__ __forceinline__ void reduce_blocks(double acc, double *partial, uint3
   }
 }
 
-// Bound by the read of the gradients: 1.19 GB of bf16 in 177 us, 0.87 GB of f32 in 135 us, 6.5 to 6.7 TB/s.  A
-// block's share is contiguous, so one search finds its first tensor.  As many blocks as are resident: eight times as
-// many, 185 us.
+// Bound by the read of the gradients: 1.19 GB of bf16 in 172 us a call, 6.9 TB/s.  Resident blocks go through the arena in
+// pieces, in address order as far as they keep step, which DRAM likes better than one long share per block
+// (150 M bf16: 50.8 us against 52.5, 596 M: 172 against 181; pieces half or twice as long: 186 and 173).
 template <bool kF32>
 __global__ void __launch_bounds__(kThreads)
-grad_sumsq_kernel(const Entry *__restrict__ tab, uint32_t n_tab, uint64_t n_vec, double *__restrict__ partial,
-                  uint32_t *ticket, NormOut o, int finish) {
-  const uint64_t v0 = n_vec * blockIdx.x / gridDim.x, v1 = n_vec * (blockIdx.x + 1ull) / gridDim.x;
+grad_sumsq_kernel(const Entry *__restrict__ tab, uint32_t n_tab, uint64_t n_vec, uint64_t piece,
+                  double *__restrict__ partial, uint32_t *ticket, NormOut o, int finish) {
   double acc = 0.0;
-  if (v0 < v1) {
+  for (uint64_t v0 = blockIdx.x * piece; v0 < n_vec; v0 += gridDim.x * piece) {
+    const uint64_t v1 = v0 + piece < n_vec ? v0 + piece : n_vec;
     uint32_t ti = find_entry(n_tab, v0, [&](uint32_t i) { return tab[i].vec0; });
     for (uint64_t v = v0; v < v1; ++ti) {
       const Entry e = tab[ti];
@@ -298,8 +299,8 @@ struct Chunk {
   }
 };
 
-// The norm of what fits a resident block per chunk: many small tensors are then read side by side, where an
-// equal share of all vectors walks through them one after another (25 tensors, 2.5 M elements: 6.4 against
+// The norm of what fits a resident block per chunk: many small tensors are then read side by side, where
+// the pieces of a block walk through them one after another (25 tensors, 2.5 M elements: 6.4 against
 // 9.3 us).
 template <bool kF32>
 __global__ void __launch_bounds__(kThreads)
@@ -313,10 +314,10 @@ grad_sumsq_chunk_kernel(const Entry *__restrict__ tab, uint32_t n_tab, double *p
 // A block per chunk, not resident blocks with a loop: blocks that start in address order keep DRAM streaming
 // (1.19 GB of bf16 in and out: 342 us, 7.0 TB/s, against 395-408 with 1184 resident blocks, 366 for a memcpy).
 //
-// Behind a norm over more than the L2 holds the sweep starts at the end of the arena, which the norm read last
-// (`reverse`); for that the norm's blocks have to go through the arena in address order too, eight waves of them.
-// Norm and sweep: 1.19 GB of bf16 538 us against 553, 0.87 GB of f32 to bf16 321 against 330, 0.6 GB 273 against
-// 281; but 0.26 GB 124 against 118.
+// Behind a norm the sweep starts at the end of the arena, which the norm read last (`reverse`): 109 M bf16 134 us
+// against 136, 25 M f32 115 against 120.  From 400 MiB on the norm then has eight waves of blocks with a share each,
+// which keep closer to address order: 218 M f32 to bf16 321 us against 329, 0.6 GB 273 against 278; but 0.26 GB 124
+// against 115.
 template <bool kF32, bool kOutF32>
 __global__ void __launch_bounds__(kThreads)
 grad_scale_kernel(const Entry *__restrict__ tab, uint32_t n_tab, const float *__restrict__ result, int in_place,
@@ -418,7 +419,7 @@ int check_scalars(float scale, float max_norm, float eps) {
   return ANC_OK;
 }
 
-int launch_sumsq(const anc_clip_plan *pl, uint32_t grid, const NormOut &o, int finish, cudaStream_t st) {
+int launch_sumsq(const anc_clip_plan *pl, uint32_t grid, uint64_t piece, const NormOut &o, int finish, cudaStream_t st) {
   if (pl->fused) {
     if (pl->grad_f32)
       grad_sumsq_chunk_kernel<true><<<(unsigned)pl->n_chunks, kThreads, 0, st>>>(pl->d_tab, pl->n_tab, pl->d_partial,
@@ -427,11 +428,11 @@ int launch_sumsq(const anc_clip_plan *pl, uint32_t grid, const NormOut &o, int f
       grad_sumsq_chunk_kernel<false><<<(unsigned)pl->n_chunks, kThreads, 0, st>>>(pl->d_tab, pl->n_tab, pl->d_partial,
                                                                                   pl->d_ticket, o, finish);
   } else if (pl->grad_f32)
-    grad_sumsq_kernel<true><<<grid, kThreads, 0, st>>>(pl->d_tab, pl->n_tab, pl->n_vec, pl->d_partial, pl->d_ticket,
-                                                       o, finish);
+    grad_sumsq_kernel<true><<<grid, kThreads, 0, st>>>(pl->d_tab, pl->n_tab, pl->n_vec, piece, pl->d_partial,
+                                                       pl->d_ticket, o, finish);
   else
-    grad_sumsq_kernel<false><<<grid, kThreads, 0, st>>>(pl->d_tab, pl->n_tab, pl->n_vec, pl->d_partial, pl->d_ticket,
-                                                        o, finish);
+    grad_sumsq_kernel<false><<<grid, kThreads, 0, st>>>(pl->d_tab, pl->n_tab, pl->n_vec, piece, pl->d_partial,
+                                                        pl->d_ticket, o, finish);
   ANC_CUDA(cudaGetLastError());
   return ANC_OK;
 }
@@ -551,7 +552,7 @@ int anc_clip_plan_create(anc_ctx *ctx, const anc_clip_tensor *tensors, int n_ten
   const uint64_t cap = (uint64_t)ctx->sm_count * (norm_per_sm > 0 ? norm_per_sm : 1);
   const uint64_t want = (vecs + kChunkVec - 1) / kChunkVec;
   pl->grid = (uint32_t)(want < cap ? (want ? want : 1) : cap);
-  pl->clip_grid = vecs * 8 * gs >= kReverseBytes ? pl->grid * 8 : pl->grid;
+  pl->clip_grid = vecs * 8 * gs >= kManyBytes ? pl->grid * 8 : pl->grid;
   pl->fused = chunks > 0 && chunks <= (uint64_t)fused_per_sm * ctx->sm_count;
   const uint64_t n_part = pl->fused && chunks > pl->clip_grid ? chunks : pl->clip_grid;
   const size_t tab_bytes = (tab.size() * sizeof(Entry) + 255) / 256 * 256;
@@ -587,13 +588,13 @@ int anc_grad_norm(anc_clip_plan *plan, float scale, float max_norm, float eps, v
   int rc = check_scalars(scale, max_norm, eps);
   if (rc) return rc;
   anc_device_guard guard(plan->ctx->device);
-  return launch_sumsq(plan, plan->grid, norm_out(plan, scale, max_norm, eps), 1, anc_pick_stream(plan->ctx, stream));
+  return launch_sumsq(plan, plan->grid, kPieceVec, norm_out(plan, scale, max_norm, eps), 1, anc_pick_stream(plan->ctx, stream));
 }
 
 int anc_grad_sumsq(anc_clip_plan *plan, void *stream) {
   ANC_REQUIRE(plan, "plan is NULL");
   anc_device_guard guard(plan->ctx->device);
-  return launch_sumsq(plan, plan->grid, norm_out(plan, 1.f, INFINITY, 0.f), 0, anc_pick_stream(plan->ctx, stream));
+  return launch_sumsq(plan, plan->grid, kPieceVec, norm_out(plan, 1.f, INFINITY, 0.f), 0, anc_pick_stream(plan->ctx, stream));
 }
 
 int anc_grad_norm_finish(anc_clip_plan *plan, float scale, float max_norm, float eps, void *stream) {
@@ -620,8 +621,9 @@ int anc_grad_clip(anc_clip_plan *plan, float scale, float max_norm, float eps, v
   cudaStream_t st = anc_pick_stream(plan->ctx, stream);
   const NormOut o = norm_out(plan, scale, max_norm, eps);
   if (!plan->fused) {
-    rc = launch_sumsq(plan, plan->clip_grid, o, 1, st);
-    return rc ? rc : launch_scale(plan, plan->clip_grid != plan->grid, st);
+    const uint64_t share = (plan->n_vec + plan->clip_grid - 1) / plan->clip_grid;
+    rc = launch_sumsq(plan, plan->clip_grid, plan->clip_grid == plan->grid ? kPieceVec : share, o, 1, st);
+    return rc ? rc : launch_scale(plan, 1, st);
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)plan->n_chunks);
