@@ -38,6 +38,7 @@ constexpr int kVecPerThread = 4;                              // vectors of 8 el
 constexpr int kChunkVec = kThreads * kVecPerThread;           // vectors per chunk of the scaling sweep
 constexpr int kChunkElems = kChunkVec * 8;
 constexpr uint64_t kPieceVec = 2 * kChunkVec;                 // vectors per piece of the norm
+constexpr uint64_t kMostVec = 1u << 30;                        // a piece fits an int
 constexpr uint64_t kManyBytes = 400u << 20;                   // gradients from which a clip's norm has more blocks
 constexpr uint32_t kWaitPolls = 1u << 22;                     // of the one-launch clip; about a second
 
@@ -200,28 +201,32 @@ template <bool kF32>
 __global__ void __launch_bounds__(kThreads)
 grad_sumsq_kernel(const Entry *__restrict__ tab, uint32_t n_tab, uint64_t n_vec, uint64_t piece,
                   double *__restrict__ partial, uint32_t *ticket, NormOut o, int finish) {
+  constexpr uint32_t kBytes = kF32 ? 32 : 16;                    // of a vector
   double acc = 0.0;
+  Entry e;
+  uint32_t ti = 0;
+  uint64_t end = 0;                                              // of tensor ti, 0: none yet
   for (uint64_t v0 = blockIdx.x * piece; v0 < n_vec; v0 += gridDim.x * piece) {
     const uint64_t v1 = v0 + piece < n_vec ? v0 + piece : n_vec;
-    uint32_t ti = find_entry(n_tab, v0, [&](uint32_t i) { return tab[i].vec0; });
-    for (uint64_t v = v0; v < v1; ++ti) {
-      const Entry e = tab[ti];
-      const uint64_t end = e.vec0 + (e.nvec ? e.nvec : 1);
-      const uint64_t a = v - e.vec0, b = (end < v1 ? end : v1) - e.vec0;
+    for (uint64_t v = v0; v < v1;) {
+      if (v >= end) {
+        ti = v == end && end ? ti + 1 : find_entry(n_tab, v, [&](uint32_t i) { return tab[i].vec0; });
+        e = tab[ti];
+        end = e.vec0 + (e.nvec ? e.nvec : 1);
+      }
+      const uint64_t a = v - e.vec0, stop = end < v1 ? end : v1;
       if (a == 0) acc += loose_sumsq<kF32>(e, e.head, e.nvec);
       if (e.nvec) {
-        for (uint64_t i0 = a + threadIdx.x; i0 < b; i0 += kChunkVec) {
+        const uint8_t *p = (const uint8_t *)e.g + e.head * (kBytes / 8) + (a + threadIdx.x) * kBytes;
+        for (int left = (int)(stop - v) - (int)threadIdx.x; left > 0; left -= kChunkVec, p += kChunkVec * kBytes) {
           Raw<kF32> r[kVecPerThread] = {};
 #pragma unroll
-          for (int k = 0; k < kVecPerThread; ++k) {
-            const uint64_t i = i0 + (uint64_t)k * kThreads;
-            load_raw<kF32>(r[k], e.g, e.head + i * 8, i < b);
-          }
+          for (int k = 0; k < kVecPerThread; ++k) load_raw<kF32>(r[k], p + k * kThreads * kBytes, 0, left > k * kThreads);
 #pragma unroll
           for (int k = 0; k < kVecPerThread; ++k) acc += sumsq8<kF32>(r[k]);
         }
       }
-      v = e.vec0 + b;
+      v = stop;
     }
   }
   reduce_blocks(acc, partial, ticket, o, finish);
@@ -437,6 +442,15 @@ int launch_sumsq(const anc_clip_plan *pl, uint32_t grid, uint64_t piece, const N
   return ANC_OK;
 }
 
+// Vectors per piece of the norm: kPieceVec, which keeps pieces on DRAM's boundaries (596 M bf16: 172 us, 175 with
+// pieces a little shorter), or with few rounds of the resident blocks what makes all rounds full (5 M bf16: 12.6 us
+// against 14.5, 40 M f32: 31.5 against 32.5).
+uint64_t piece_of(const anc_clip_plan *pl) {
+  const uint64_t rounds = (pl->n_vec + pl->grid * kPieceVec - 1) / (pl->grid * kPieceVec);
+  if (rounds > 4) return kPieceVec;
+  return rounds ? (pl->n_vec + pl->grid * rounds - 1) / (pl->grid * rounds) : 1;
+}
+
 using ScaleKernel = void (*)(const Entry *, uint32_t, const float *, int, int);
 using FusedKernel = void (*)(const Entry *, uint32_t, double *, uint32_t *, NormOut, int, uint32_t *);
 
@@ -588,13 +602,13 @@ int anc_grad_norm(anc_clip_plan *plan, float scale, float max_norm, float eps, v
   int rc = check_scalars(scale, max_norm, eps);
   if (rc) return rc;
   anc_device_guard guard(plan->ctx->device);
-  return launch_sumsq(plan, plan->grid, kPieceVec, norm_out(plan, scale, max_norm, eps), 1, anc_pick_stream(plan->ctx, stream));
+  return launch_sumsq(plan, plan->grid, piece_of(plan), norm_out(plan, scale, max_norm, eps), 1, anc_pick_stream(plan->ctx, stream));
 }
 
 int anc_grad_sumsq(anc_clip_plan *plan, void *stream) {
   ANC_REQUIRE(plan, "plan is NULL");
   anc_device_guard guard(plan->ctx->device);
-  return launch_sumsq(plan, plan->grid, kPieceVec, norm_out(plan, 1.f, INFINITY, 0.f), 0, anc_pick_stream(plan->ctx, stream));
+  return launch_sumsq(plan, plan->grid, piece_of(plan), norm_out(plan, 1.f, INFINITY, 0.f), 0, anc_pick_stream(plan->ctx, stream));
 }
 
 int anc_grad_norm_finish(anc_clip_plan *plan, float scale, float max_norm, float eps, void *stream) {
@@ -621,8 +635,8 @@ int anc_grad_clip(anc_clip_plan *plan, float scale, float max_norm, float eps, v
   cudaStream_t st = anc_pick_stream(plan->ctx, stream);
   const NormOut o = norm_out(plan, scale, max_norm, eps);
   if (!plan->fused) {
-    const uint64_t share = (plan->n_vec + plan->clip_grid - 1) / plan->clip_grid;
-    rc = launch_sumsq(plan, plan->clip_grid, plan->clip_grid == plan->grid ? kPieceVec : share, o, 1, st);
+    const uint64_t share = std::min((plan->n_vec + plan->clip_grid - 1) / plan->clip_grid, kMostVec);
+    rc = launch_sumsq(plan, plan->clip_grid, plan->clip_grid == plan->grid ? piece_of(plan) : share, o, 1, st);
     return rc ? rc : launch_scale(plan, 1, st);
   }
   cudaLaunchConfig_t cfg = {};
