@@ -481,9 +481,8 @@ constexpr int kZeroThreads = 256;
 
 // When the whole table is written, what the SMs that do not sort do meanwhile.  Launched behind the sort without
 // waiting for it; it waits for the sort only before it ends, so that whoever waits for this kernel has the
-// sorted list too.  311 MB of zeros: 48 us alone, 6.5 TB/s.  (Reading the first rows of dy into L2 at that time
-// gave 3 us of 75 for 65536 rows of 1024 bf16 added to f32, cost 5 of 149 for 30000 rows of 4096 f32 and 9 of 66
-// beside the zeros.)
+// sorted list too.  311 MB of zeros: 48 us alone, 6.5 TB/s.  (Reading dy into L2 at that time
+// cost 9 us of 66 beside the zeros.)
 __global__ void __launch_bounds__(kZeroThreads)
 embedding_zero_kernel(ZeroArgs z) {
   pdl_trigger();
@@ -495,9 +494,12 @@ embedding_zero_kernel(ZeroArgs z) {
 constexpr int kRedThreads = 256;
 constexpr int kMaxPiece = 512;       // sorted places per block
 constexpr uint32_t kWaitPolls = 1u << 20;
+constexpr uint32_t kAheadBlocks = 296, kAheadPiece = 8192;
 
 struct RedArgs {
   const uint8_t *dy;
+  const uint8_t *ahead;          // bytes of dy to read into L2 while the list is made
+  uint64_t ahead_bytes;
   uint8_t *dw;
   uint32_t dy_pitch, dw_pitch;   // bytes from row to row
   int64_t T;
@@ -659,6 +661,13 @@ embedding_reduce_kernel(RedArgs a) {
   const int64_t p0 = (int64_t)piece * len;
   for (int i = threadIdx.x; i < 2 * parts; i += kRedThreads) open_key[i & 1][i >> 1] = a.V;
   if (l == 0) through[part] = 0;
+  if (kAdd && threadIdx.x == 0 && blockIdx.x < kAheadBlocks) {
+    const uint64_t step = (uint64_t)(gridDim.x < kAheadBlocks ? gridDim.x : kAheadBlocks) * kAheadPiece;
+    for (uint64_t o = (uint64_t)blockIdx.x * kAheadPiece; o < a.ahead_bytes; o += step) {
+      const uint32_t n = (uint32_t)(a.ahead_bytes - o < kAheadPiece ? a.ahead_bytes - o : kAheadPiece);
+      asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(a.ahead + o), "r"(n) : "memory");
+    }
+  }
   pdl_wait();
   int live = 0;      // the padding lies behind the last run
   for (int i0 = 0; i0 < len + 1; i0 += kRedThreads) {
@@ -939,6 +948,10 @@ embedding_small_kernel(RedArgs a, const void *__restrict__ ids, int ids64, int64
 // block goes from part to part (rows of 8 f32: 3085 tokens 15.6 us against 26.9 with one lane a row, 131072 43
 // against 64; rows of 56: 41 against 43, with 16 lanes 46).
 constexpr int kMinLanes = 8;
+// Adding, the blocks of the sums that are resident while the list is made read dy into L2, where dy is no more than
+// three quarters of it (rows of 1024 bf16 added to f32: 16384 tokens 32.3 us against 35.0, 32768 46.8 against 48.9, of
+// bf16 48000 50.0 against 53.1; above it goes either way: 117 MB -2 and +2 us, 134 MB -3 and +5).
+constexpr int64_t kAheadMost = 94 << 20;
 constexpr int kMinPart = 4;                  // places per part at least
 constexpr int64_t kResident = 296;           // blocks of the sums that are resident at once, two per SM
 constexpr int kSortTarget = 4;               // rounds of 32 keys per warp the sort aims at
@@ -1230,6 +1243,11 @@ int anc_embedding_grad(anc_ctx *ctx, const void *dy, int dy_dtype, int64_t dy_ld
       small ? (T * sh.slices + kRedThreads / sh.L - 1) / (kRedThreads / sh.L) : sh.pieces * sh.slices;
   ANC_REQUIRE(blocks <= 0x7FFFFFFF, "T x D too large");
   int n_attrs = write ? 1 : 0;
+  const int64_t dy_bytes = T * D * (yf ? 4 : 2), skip = (16 - ((uintptr_t)dy & 15)) & 15;
+  if (dy_ld == D && dy_bytes <= kAheadMost && dy_bytes >= 32) {
+    ra.ahead = (const uint8_t *)dy + skip;
+    ra.ahead_bytes = (uint64_t)(dy_bytes - skip) / 16 * 16;
+  }
   if (!small) {
     SortArgs sa = {};
     sa.ids = ids; sa.ids64 = i64; sa.T = (uint32_t)T; sa.V = V; sa.padding_idx = padding_idx;
