@@ -280,3 +280,75 @@ def test_gradients_larger_than_the_sweep_backwards_starts_at(ctx, g_dtype, in_pl
     if not in_place:
         out.free()
     d.free()
+
+
+@pytest.mark.parametrize("captured", [False, True])
+def test_chained_clips_in_two_launches(ctx, captured):
+    """The sweep that starts beside its norm: a plan's output is the next plan's gradient, back to back on one
+    stream, also captured; every pass sees the gradients written just before it."""
+    rng = np.random.default_rng(12)
+    n = 12_000_005
+    a, b, c = (anc.DBuf.zeros((n,), t, ctx) for t in (np.float32, np.float32, np.uint16))
+    first = anc.GradClip([dict(g=a, numel=n, out=b)], grad_dtype="f32", ctx=ctx)
+    second = anc.GradClip([dict(g=b, numel=n, out=c)], grad_dtype="f32", out_dtype="bf16", ctx=ctx)
+    hosts = [(rng.standard_normal(n) * s).astype(np.float32) for s in (1e-3, 7.0, 0.5)]
+    dev = [anc.DBuf(h, ctx) for h in hosts]
+
+    def pair():
+        first.clip(3.0, scale=0.5, stream=ctx.stream)
+        second.clip(2.0, stream=ctx.stream)
+    g = C.c_void_p()
+    if captured:
+        L.check(L.lib().anc_graph_begin(ctx.handle, ctx.stream))
+        pair()
+        L.check(L.lib().anc_graph_end(ctx.handle, ctx.stream, C.byref(g)))
+    for k in (0, 1, 2, 1, 0, 2):
+        for j in (2, k):                     # two passes without a wait between them: the second one counts
+            L.check(L.lib().anc_d2d(ctx.handle, a.ptr, dev[j].ptr, 4 * n, ctx.stream))
+            if captured:
+                L.check(L.lib().anc_graph_launch(ctx.handle, g, ctx.stream))
+            else:
+                pair()
+        ctx.sync()
+        r1, r2 = first.read(), second.read()
+        _check_norm(r1, clip_ref.norm_and_factor([hosts[k]], 3.0, scale=0.5))
+        mid = hosts[k] * np.float32(r1[1])
+        assert np.array_equal(b.to_numpy(), mid)
+        _check_norm(r2, clip_ref.norm_and_factor([mid], 2.0))
+        assert np.array_equal(c.to_numpy(), obf.rne_bits(mid * np.float32(r2[1])))
+    if captured:
+        L.check(L.lib().anc_graph_destroy(g))
+    for x in (first, second, a, b, c, *dev):
+        x.free()
+
+
+@pytest.mark.parametrize("mode", ["in place", "mixed"])
+def test_clips_in_place_in_two_launches(ctx, mode):
+    """Tensors in place beside tensors with an output of their own, repeated without waits: a second clip finds the
+    first one's gradients."""
+    rng = np.random.default_rng(13)
+    n = 9_000_001
+    ha, hb = ((rng.standard_normal(n) * 0.1).astype(np.float32) for _ in range(2))
+    a, b, out = anc.DBuf(ha, ctx), anc.DBuf(hb, ctx), anc.DBuf.zeros((n,), np.float32, ctx)
+    clip = anc.GradClip([dict(g=a, numel=n), dict(g=b, numel=n, out=b if mode == "in place" else out)],
+                        grad_dtype="f32", ctx=ctx)
+    limits = (100.0, 50.0, 20.0, 1e9)
+    for mx in limits:
+        clip.clip(mx, stream=ctx.stream)
+    ctx.sync()
+    va, vb, vo = ha, hb, None
+    for mx in limits:
+        _, f = clip_ref.norm_and_factor([va, vb], mx)
+        f = np.float32(f)
+        vo = vb * f
+        va, vb = va * f, (vo if mode == "in place" else vb)
+    # the last factor is 1: the gradients are those its norm saw
+    _check_norm(clip.read(), clip_ref.norm_and_factor([a.to_numpy(), b.to_numpy()], 1e9))
+    # each of the four factors is within 6u of the oracle's and each product within u: 28u in all
+    assert np.allclose(a.to_numpy(), va, rtol=30 * U, atol=0)
+    assert np.allclose((b if mode == "in place" else out).to_numpy(), vo, rtol=30 * U, atol=0)
+    if mode == "mixed":
+        assert np.array_equal(b.to_numpy(), hb)
+    clip.free()
+    for x in (a, b, out):
+        x.free()
