@@ -396,7 +396,7 @@ ANC_API int anc_clip_plan_destroy(anc_clip_plan *plan);
  *   table, dw (V,D), dy, out (T,D): bf16 bits or f32, rows `ld` elements apart (0: D), elements of a row
  *   contiguous, any alignment; ids (T): int32 or int64.  A negative id is padding: a zero row, no
  *   gradient; its row of dy is not read.  An id >= V sets status bit 0x8 and counts as padding.
- * Sums and products are float32, rounded once to the output type. */
+ * Sums and products are float32, rounded once to the output type; `scale` must be finite. */
 #define ANC_IDS_I32 0
 #define ANC_IDS_I64 1
 /* out[t,:] = round(scale * table[ids[t],:]) */

@@ -19,4 +19,6 @@ Parity status
   ``(f32_bits + dither16) >> 16`` is the reference's; the dither source is
   defined here and pinned by the published Philox known-answer vectors.
   For that stream: parity unpinned by the reference.
+* The gradient norm, clipping and embedding rows (``clip_ref``, ``embed_ref``) have no counterpart in the
+  reference: their formulas in float64, checked against differences where they are gradients.
 """
