@@ -142,6 +142,9 @@ class ResidentHybrid:
         self._streams = None
         self._comm_stream = None
         self._embed_work = []                  # scratch of embedding_grad; the last is the largest
+        self._acc_tied = {}                    # table fed through embedding_grad(into="acc") -> its ``tied``
+        self._acc_stale = set()                # of those, where the gradient arena may hold an earlier gradient
+        self._grads_spent = False              # a fold or a step has read the gradient arenas as they are
         self.max_grad_norm = max_grad_norm
 
     # ---------------------------------------------------------------- locations
@@ -265,20 +268,40 @@ class ResidentHybrid:
                                  ids_dtype=ids_dtype, stream=si or self.ctx.stream, ctx=self.ctx)
 
     def embedding_grad(self, name, dy, ids, T, scale=1.0, dy_dtype="bf16", ids_dtype="i64", mode="write",
-                       into="grad", padding_idx=None, si=None):
+                       into="grad", padding_idx=None, si=None, tied=None):
         """The gradient of ``embedding_lookup`` (``kernels.embedding_grad``) into the gradient arena
         (``into="grad"``) or, with mode "add", straight into the float32 accumulator (``into="acc"``, after
         ``enable_grad_accumulation``).  ``mode="add"`` onto the gradient arena is for a tied table whose head
         gradient is already there.  Calls on one engine share scratch and must be ordered; scratch grows
-        at the first call with more tokens, which must not be captured."""
+        at the first call with more tokens, which must not be captured.
+
+        With ``into="acc"`` the folds of ``accumulate_grads`` and ``finalize_grads`` still add what lies in the
+        gradient arena for the table: in every micro-batch the head's gradient of a tied table, for any other
+        table nothing.  So that an earlier gradient is never added again, every step clears the table's region of
+        the gradient arena when it has read it.  Where an earlier gradient may lie there all the same (steps were
+        taken before the first such call for the table, or a finished gradient was not stepped on) only the caller
+        knows: ``tied=True``: the head writes the region in every micro-batch, the engine never clears it;
+        ``tied=False``: nothing else writes it, the engine clears it now.  It holds for later calls too; with
+        None, as long as neither was ever said, such a call is refused."""
         V, D = self._table(name)
+        si = si or self.ctx.stream
         if into == "grad":
+            if tied is not None:
+                raise ValueError("tied goes with into='acc'")
             dw, dt = self.grad_view(name), self.grad_dtype
+            if mode == "add":
+                self._drop_stale(si, name)
+            self._acc_stale.discard(name)
         elif into == "acc":
             if getattr(self, "acc_a", None) is None:
                 raise RuntimeError("enable_grad_accumulation first")
             if mode != "add":
                 raise ValueError("the accumulator is only added to")
+            if self._grads_spent and (name not in self._acc_tied or (tied is False and self._acc_tied[name])):
+                self._acc_stale.add(name)
+            if tied is not None or name not in self._acc_tied:
+                self._acc_tied[name] = tied
+            self._drop_stale(si, name)
             _, _, o = self._loc(name)
             acc = self.acc_a if name in self.a_off else self.acc_m
             dw, dt = acc.slice_elems(o, V * D, (V, D)), "f32"
@@ -289,7 +312,26 @@ class ResidentHybrid:
             self._embed_work.append(DBuf.empty((need,), np.uint8, self.ctx))   # a captured graph may hold the old one
         kernels.embedding_grad(dy, ids, dw, T, V, D, self._embed_work[-1], scale=scale, dy_dtype=dy_dtype,
                                dw_dtype=dt, ids_dtype=ids_dtype, mode=mode, padding_idx=padding_idx,
-                               stream=si or self.ctx.stream, ctx=self.ctx)
+                               stream=si, ctx=self.ctx)
+
+    def _drop_stale(self, si, *names):
+        """Clears what an earlier window left in the gradient arena for tables that only the accumulator gathers."""
+        for n in self._acc_stale.intersection(names):
+            if self._acc_tied[n] is None:
+                raise RuntimeError(f"the gradient arena may hold an earlier gradient of {n}, which the fold would add "
+                                   "again: call embedding_grad with tied=False, or tied=True where the head writes it "
+                                   "in every micro-batch")
+            if not self._acc_tied[n]:
+                self.grad_view(n).zero_(si)
+            self._acc_stale.discard(n)
+
+    def _grads_stepped(self, si, arena=None):
+        """Behind a step (of ``arena`` "adamw" or "muon", None: both): the gradients it read are spent."""
+        self._grads_spent = True
+        for n, tied in self._acc_tied.items():
+            if not tied and arena in (None, "adamw" if n in self.a_off else "muon"):
+                self.grad_view(n).zero_(si)
+                self._acc_stale.discard(n)
 
     # ---------------------------------------------------------------- the step
     def _compute_unit(self, unit, si):
@@ -341,12 +383,14 @@ class ResidentHybrid:
                 ev.record(si)
                 L.check(lib.anc_stream_wait_event(cs, ev.handle))
                 self._gather_group(what, cs)
+            self._grads_stepped(si)
             done = evs[k]
             done.record(cs)
             L.check(lib.anc_stream_wait_event(si, done.handle))
             return
         for u in self.units:
             self._compute_unit(u, si)
+        self._grads_stepped(si)
         if multi:
             self.exchange(si)
 
@@ -363,6 +407,7 @@ class ResidentHybrid:
         for u in self.units:
             if u[0] == kind:
                 self._compute_unit(u, si)
+        self._grads_stepped(si, kind)
         if exchange and self.world > 1:
             assert self.comm is not None, "world > 1 needs a communicator"
             if kind == "adamw":
@@ -407,9 +452,11 @@ class ResidentHybrid:
     def accumulate_grads(self, si=None):
         """acc += the gradients now in the gradient arenas (one sweep per arena, all regions: a
         data-parallel replica holds local gradients for every parameter)."""
+        self._drop_stale(si, *self._acc_stale)
         for acc, g, n in ((self.acc_a, self.a_g, self.a_padded), (self.acc_m, self.m_g, self.m_total)):
             kernels.grad_accumulate(acc, g, None, n, src_dtype="bf16", stream=si, ctx=self.ctx)
         self.acc_count += 1
+        self._grads_spent = True
 
     def finalize_grads(self, si=None, scale=None, rounding="sr", seed=None, reduce=True):
         """Last micro-batch: acc += the gradients in the arenas, then (world > 1 and ``reduce``) the
@@ -434,6 +481,7 @@ class ResidentHybrid:
             kernels.grad_accumulate(acc, None, g, n, elem_offset=off, scale=scale, rounding=rounding, seed=seed,
                                     step=self.t + 1, zero_after=True, stream=si, ctx=self.ctx)
         self.acc_count = 0
+        self._acc_stale.update(n for n, tied in self._acc_tied.items() if not tied)
 
     # ---------------------------------------------------------------- graph replay
     def capture_step(self, si=None, horizon=4096):
@@ -491,6 +539,7 @@ class ResidentHybrid:
         self.t += 1
         self._graph_next += 1
         L.check(L.lib().anc_graph_launch(self.ctx.handle, self._graph, si))
+        self._grads_stepped(si)
 
     def exchange(self, si=None):
         """NCCL path: one in-place all-gather per unit."""
@@ -682,6 +731,7 @@ class ResidentHybrid:
             m_out.record(s_out)
             if cs is not None:
                 m_x.record(cs)
+        self._grads_stepped(si)
         if cs is not None:
             done_x.record(cs)
             L.check(lib.anc_stream_wait_event(si, done_x.handle))
