@@ -39,6 +39,7 @@ def _numel(shape):
 
 class ResidentHybrid:
     _clip, _max_grad_norm, _embed_work = None, None, ()
+    _acc_tied, _acc_stale, _grads_spent = {}, frozenset(), False
 
     def __init__(self, params, muon_names, no_decay_names=(), adamw_kw=None, muon_kw=None,
                  grad_dtype="bf16", rounding="sr", seed=0, rank=0, world=1, comm=None,
