@@ -521,10 +521,10 @@ int anc_clip_plan_create(anc_ctx *ctx, const anc_clip_tensor *tensors, int n_ten
       ANC_REQUIRE(t.numel <= (1ull << 48), "tensor %d: numel out of range", i);
       ANC_REQUIRE(((uintptr_t)t.g & (gs - 1)) == 0 && ((uintptr_t)t.out & (os - 1)) == 0,
                   "tensor %d: pointer not aligned to its element size", i);
-      ANC_REQUIRE(t.out || gs == os, "tensor %d: in place needs equal gradient and output types", i);
       Entry e;
       e.g = t.g;
       e.out = t.out ? t.out : const_cast<void *>(t.g);
+      ANC_REQUIRE(e.out != e.g || gs == os, "tensor %d: in place needs equal gradient and output types", i);
       all_in_place = all_in_place && e.out == e.g;
       e.numel = t.numel;
       e.vec0 = vecs;

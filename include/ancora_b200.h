@@ -359,8 +359,8 @@ ANC_API int anc_grad_accumulate(anc_ctx *ctx, float *acc, const void *src, int s
  *   out    = round(g * factor)                                        (anc_grad_clip, anc_grad_apply)
  *
  * A plan holds the table of gradient tensors (one type for all, any alignment, sizes from 0) and the block
- * sums of the reduction.  `out` NULL clips in place; an output must not overlap another tensor or output of
- * the plan, so a tensor is listed once, and `result` none of them.
+ * sums of the reduction.  `out` NULL or `out` == `g` clips in place, which needs equal types; an output must not
+ * overlap another tensor or output of the plan, so a tensor is listed once, and `result` none of them.
  * {norm, factor} are two floats in device memory: `result` when given, else inside the plan.  Squares are summed
  * in float32 by eights and in float64 above, in a fixed order: the same bits every time on one device.  A
  * NaN in a gradient makes norm and factor NaN, an infinity makes norm infinite and factor 0;
