@@ -122,6 +122,7 @@ SIGNATURES = {
     "anc_grad_sumsq": (_i, [_vp, _vp]),
     "anc_grad_norm_finish": (_i, [_vp, _f, _f, _f, _vp]),
     "anc_grad_apply": (_i, [_vp, _vp]),
+    "anc_clip_wait_selftest": (_i, [_vp, _f, C.c_uint32, C.c_uint32, _vp]),
     "anc_clip_plan_destroy": (_i, [_vp]),
     "anc_embedding_lookup": (_i, [_vp, _vp, _i, _i64, _vp, _i, _vp, _i, _i64, _i64, _i64, _i64, _f, _vp]),
     "anc_embedding_grad_workspace": (_i, [_i64, _i64, _i64, C.POINTER(_u64)]),

@@ -41,6 +41,8 @@ constexpr uint64_t kPieceVec = 2 * kChunkVec;                 // vectors per pie
 constexpr uint64_t kMostVec = 1u << 30;                        // a piece fits an int
 constexpr uint64_t kManyBytes = 400u << 20;                   // gradients from which a clip's norm has more blocks
 constexpr uint32_t kWaitPolls = 1u << 22;                     // of the one-launch clip; about a second
+constexpr uint32_t kGaveUp = 1u << 31;                        // in its ticket; above any count of blocks
+constexpr uint32_t kTestPolls = 1u << 14;
 
 // One tensor.  The norm reads elements [head, head + 8 * nvec) as vectors of eight aligned to their size (16
 // bytes of bf16, 32 of f32), and the up to 7 on either side one by one.  The scaling sweep wants input and output
@@ -347,29 +349,54 @@ grad_scale_kernel(const Entry *__restrict__ tab, uint32_t n_tab, const float *re
   ch.store(f);
 }
 
+__device__ __forceinline__ uint32_t ld_acquire(const uint32_t *p) {
+  uint32_t v;
+  asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
+  return v;
+}
+
+// Whether all blocks of the grid have counted themselves in `ticket`: the same answer in every block.  The first block
+// that gives up marks the ticket, which it can only while a block is missing; from then on the answer is no,
+// also for the blocks that arrive later.
+__device__ __forceinline__ bool all_arrived(uint32_t *ticket, uint32_t polls) {
+  uint32_t seen = 0;
+  for (uint32_t i = 0; i < polls; ++i) {
+    seen = ld_acquire(ticket);
+    if (seen >= gridDim.x) return seen == gridDim.x;
+  }
+  while (seen < gridDim.x) {             // every round that fails is one more block in the ticket, or its mark
+    const uint32_t old = atomicCAS(ticket, seen, seen | kGaveUp);
+    if (old == seen) seen |= kGaveUp;
+    else seen = old;
+  }
+  __threadfence();
+  return seen == gridDim.x;
+}
+
 // Norm and scaling in one launch: a block per chunk, all resident at once (a cooperative launch), the
 // chunk in registers while the blocks wait for one another's sums: 2.5 M elements of bf16 8.2 us against 14.3 by two
 // launches.  From about 5 M bf16 elements on the chunks are too many and there are two launches.  The wait is
-// bounded: when it runs out, status bit 0x10 is set, norm and factor are NaN and no gradient is written.
-template <bool kF32, bool kOutF32>
-__global__ void __launch_bounds__(kThreads)
+// bounded, and the blocks decide together: when it runs out, status bit 0x10 is set, norm and factor are NaN and no
+// gradient is written.  kLate, for the self-test: block `late` comes only after another one gave up.  Three blocks an
+// SM: left to itself the compiler takes registers that leave room for two.
+template <bool kF32, bool kOutF32, bool kLate>
+__global__ void __launch_bounds__(kThreads, 3)
 grad_clip_fused_kernel(const Entry *__restrict__ tab, uint32_t n_tab, double *partial, uint32_t *ticket, NormOut o,
-                       int in_place, uint32_t *status) {
+                       int in_place, uint32_t *status, uint32_t polls, uint32_t late) {
   Chunk<kF32, kOutF32> ch;
   ch.find(tab, n_tab, blockIdx.x);
   ch.load();
   double acc = block_sum(ch.sumsq());
   __shared__ bool ok;
   if (threadIdx.x == 0) {
+    if constexpr (kLate) {
+      if (blockIdx.x == late)
+        for (uint32_t i = 0; i < 64 * kTestPolls && !(ld_acquire(ticket) & kGaveUp); ++i) {}
+    }
     partial[blockIdx.x] = acc;
     __threadfence();
     atomicAdd(ticket, 1u);
-    ok = false;
-    for (uint32_t i = 0; i < kWaitPolls && !ok; ++i) {
-      uint32_t seen;
-      asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(seen) : "l"(ticket) : "memory");
-      ok = seen >= gridDim.x;
-    }
+    ok = all_arrived(ticket, polls);
     // the last block to leave makes the counters ready for the next launch
     if (atomicAdd(ticket + 1, 1u) == gridDim.x - 1) {
       ticket[0] = 0u;
@@ -466,15 +493,33 @@ uint64_t piece_of(const anc_clip_plan *pl) {
 }
 
 using ScaleKernel = void (*)(const Entry *, uint32_t, const float *, int, int);
-using FusedKernel = void (*)(const Entry *, uint32_t, double *, uint32_t *, NormOut, int, uint32_t *);
+using FusedKernel = void (*)(const Entry *, uint32_t, double *, uint32_t *, NormOut, int, uint32_t *, uint32_t, uint32_t);
 
 ScaleKernel scale_kernel(const anc_clip_plan *pl) {
   if (pl->grad_f32) return pl->out_f32 ? grad_scale_kernel<true, true> : grad_scale_kernel<true, false>;
   return pl->out_f32 ? grad_scale_kernel<false, true> : grad_scale_kernel<false, false>;
 }
+template <bool kLate>
 FusedKernel fused_kernel(const anc_clip_plan *pl) {
-  if (pl->grad_f32) return pl->out_f32 ? grad_clip_fused_kernel<true, true> : grad_clip_fused_kernel<true, false>;
-  return pl->out_f32 ? grad_clip_fused_kernel<false, true> : grad_clip_fused_kernel<false, false>;
+  if (pl->grad_f32)
+    return pl->out_f32 ? grad_clip_fused_kernel<true, true, kLate> : grad_clip_fused_kernel<true, false, kLate>;
+  return pl->out_f32 ? grad_clip_fused_kernel<false, true, kLate> : grad_clip_fused_kernel<false, false, kLate>;
+}
+
+int launch_fused(const anc_clip_plan *pl, FusedKernel kernel, const NormOut &o, uint32_t polls, uint32_t late,
+                 cudaStream_t st) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)pl->n_chunks);
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeCooperative;
+  at[0].val.cooperative = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  ANC_CUDA(cudaLaunchKernelEx(&cfg, kernel, (const Entry *)pl->d_tab, pl->n_tab, pl->d_partial, pl->d_ticket, o,
+                              pl->in_place, pl->ctx->d_status, polls, late));
+  return ANC_OK;
 }
 
 // behind_norm: backwards and, unless in place, started while the norm's last blocks run (27 M f32 to bf16 45.5 us
@@ -582,7 +627,7 @@ int anc_clip_plan_create(anc_ctx *ctx, const anc_clip_tensor *tensors, int n_ten
   cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(
       &norm_per_sm, pl->grad_f32 ? grad_sumsq_kernel<true> : grad_sumsq_kernel<false>, kThreads, 0);
   if (e == cudaSuccess)
-    e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&fused_per_sm, fused_kernel(pl), kThreads, 0);
+    e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&fused_per_sm, fused_kernel<false>(pl), kThreads, 0);
   if (e != cudaSuccess) {
     delete pl;
     return anc_cuda_fail(e, "clip kernel occupancy");
@@ -663,18 +708,22 @@ int anc_grad_clip(anc_clip_plan *plan, float scale, float max_norm, float eps, v
     rc = launch_sumsq(plan, plan->clip_grid, plan->clip_grid == plan->grid ? piece_of(plan) : share, o, 1, st);
     return rc ? rc : launch_scale(plan, 1, st);
   }
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)plan->n_chunks);
-  cfg.blockDim = dim3(kThreads);
-  cfg.stream = st;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeCooperative;
-  at[0].val.cooperative = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = 1;
-  ANC_CUDA(cudaLaunchKernelEx(&cfg, fused_kernel(plan), (const Entry *)plan->d_tab, plan->n_tab, plan->d_partial,
-                              plan->d_ticket, o, plan->in_place, plan->ctx->d_status));
-  return ANC_OK;
+  return launch_fused(plan, fused_kernel<false>(plan), o, kWaitPolls, 0, st);
+}
+
+int anc_clip_wait_selftest(anc_clip_plan *plan, float max_norm, uint32_t polls, uint32_t late, void *stream) {
+  ANC_REQUIRE(plan, "plan is NULL");
+  ANC_REQUIRE(polls > 0 && polls <= kTestPolls, "polls %u outside 1..2^14", polls);
+  int rc = check_scalars(1.f, max_norm, 0.f);
+  if (rc) return rc;
+  ANC_REQUIRE(plan->fused && plan->n_chunks > 1 && late < plan->n_chunks,
+              "needs a plan of several blocks that one launch clips, and one of its blocks");
+  anc_device_guard guard(plan->ctx->device);
+  const FusedKernel kernel = fused_kernel<true>(plan);
+  int per_sm = 0;
+  ANC_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, kThreads, 0));
+  ANC_REQUIRE(plan->n_chunks <= (uint64_t)per_sm * plan->ctx->sm_count, "plan too large for the self-test");
+  return launch_fused(plan, kernel, norm_out(plan, 1.f, max_norm, 0.f), polls, late, anc_pick_stream(plan->ctx, stream));
 }
 
 int anc_clip_plan_destroy(anc_clip_plan *plan) {

@@ -388,6 +388,10 @@ ANC_API int anc_grad_sumsq(anc_clip_plan *plan, void *stream);
 ANC_API int anc_grad_norm_finish(anc_clip_plan *plan, float scale, float max_norm, float eps, void *stream);
 /* out = round(g * factor) with the factor the last norm call left. */
 ANC_API int anc_grad_apply(anc_clip_plan *plan, void *stream);
+/* Self-test of the wait in anc_grad_clip's one launch (plans of several blocks that fit it): every block waits for
+ * `polls` reads at most (1..2^14), and block `late` comes only when another one has given up.  Afterwards status bit
+ * 0x10 is set, norm and factor are NaN, no gradient was written by any block, and the plan is ready for its next call. */
+ANC_API int anc_clip_wait_selftest(anc_clip_plan *plan, float max_norm, uint32_t polls, uint32_t late, void *stream);
 /* Waits for the device before it frees the table. */
 ANC_API int anc_clip_plan_destroy(anc_clip_plan *plan);
 
