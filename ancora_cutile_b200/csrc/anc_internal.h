@@ -53,6 +53,10 @@ static inline cudaStream_t anc_pick_stream(anc_ctx *ctx, void *stream) {
   return stream ? (cudaStream_t)stream : ctx->stream;
 }
 
+// Behind cudaMemcpy and cudaMemset of what later launches read: both may return before the device is done, and the
+// streams of the contexts do not wait for the legacy stream that does them.
+static inline cudaError_t anc_finish_setup() { return cudaStreamSynchronize(cudaStreamLegacy); }
+
 struct anc_device_guard {
   int prev;
   bool changed;

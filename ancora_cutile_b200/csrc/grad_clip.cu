@@ -644,6 +644,7 @@ int anc_clip_plan_create(anc_ctx *ctx, const anc_clip_tensor *tensors, int n_ten
   if (e == cudaSuccess && !tab.empty())
     e = cudaMemcpy(pl->d_mem, tab.data(), tab.size() * sizeof(Entry), cudaMemcpyHostToDevice);
   if (e == cudaSuccess) e = cudaMemset(pl->d_mem + tab_bytes + part_bytes, 0, 256);
+  if (e == cudaSuccess) e = anc_finish_setup();
   if (e != cudaSuccess) {
     if (pl->d_mem) cudaFree(pl->d_mem);
     delete pl;
