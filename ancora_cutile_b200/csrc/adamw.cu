@@ -343,9 +343,11 @@ static int adamw_build_chunks(anc_adamw_plan *pl, uint64_t begin, uint64_t end) 
     pl->chunk_capacity = (uint32_t)chunks.size();
     ANC_CUDA(cudaMalloc((void **)&pl->d_chunks, sizeof(Chunk) * chunks.size()));
   }
-  if (!chunks.empty())
+  if (!chunks.empty()) {
     ANC_CUDA(cudaMemcpy(pl->d_chunks, chunks.data(), sizeof(Chunk) * chunks.size(),
                         cudaMemcpyHostToDevice));
+    ANC_CUDA(anc_finish_setup());
+  }
   pl->n_chunks = (uint32_t)chunks.size();
   pl->owned_elems = owned;
   return ANC_OK;
@@ -484,6 +486,7 @@ int anc_adamw_plan_set_schedule(anc_adamw_plan *plan, const anc_adamw_scalars *t
   if (!plan->d_counter) ANC_CUDA(cudaMalloc((void **)&plan->d_counter, sizeof(unsigned long long)));
   unsigned long long t0 = first_step;
   ANC_CUDA(cudaMemcpy(plan->d_counter, &t0, sizeof(t0), cudaMemcpyHostToDevice));
+  ANC_CUDA(anc_finish_setup());
   plan->sched_first = first_step;
   plan->sched_len = (uint32_t)n;
   return ANC_OK;
@@ -500,6 +503,7 @@ int anc_adamw_plan_set_counter(anc_adamw_plan *plan, uint64_t step, void *stream
   ANC_CUDA(cudaStreamSynchronize(st));      // no launch that reads the counter is still in flight
   unsigned long long t0 = step;
   ANC_CUDA(cudaMemcpy(plan->d_counter, &t0, sizeof(t0), cudaMemcpyHostToDevice));
+  ANC_CUDA(anc_finish_setup());
   return ANC_OK;
 }
 

@@ -215,6 +215,7 @@ int anc_muon_plan_create_ex(anc_ctx *ctx, const anc_muon_weight *weights, const 
       e = cudaMemcpy(g.d_mom, mom.data(), mom.size() * sizeof(anc_mom_entry), cudaMemcpyHostToDevice);
     if (e == cudaSuccess)
       e = cudaMemcpy(g.d_upd, upd.data(), upd.size() * sizeof(anc_upd_entry), cudaMemcpyHostToDevice);
+    if (e == cudaSuccess) e = anc_finish_setup();
     if (e != cudaSuccess) {
       plan_free(pl);
       return anc_cuda_fail(e, "muon tables");

@@ -1492,6 +1492,7 @@ int get_tile_tab(anc_ctx *ctx, bool sym, bool pair, int mb, int nb, TileTab *out
   tt.count = (int)tab.size();
   ANC_CUDA(cudaMalloc((void **)&tt.d_tab, tab.size() * sizeof(uint32_t)));
   ANC_CUDA(cudaMemcpy(tt.d_tab, tab.data(), tab.size() * sizeof(uint32_t), cudaMemcpyHostToDevice));
+  ANC_CUDA(anc_finish_setup());
   gc->tabs[key] = tt;
   *out = tt;
   return ANC_OK;

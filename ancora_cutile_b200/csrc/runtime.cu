@@ -78,6 +78,7 @@ int anc_ctx_create(int device, void *stream, anc_ctx **out) {
   e = cudaMalloc(&c->d_work, c->work_bytes);
   if (e == cudaSuccess) e = cudaMalloc((void **)&c->d_status, 256);
   if (e == cudaSuccess) e = cudaMemset(c->d_status, 0, 256);
+  if (e == cudaSuccess) e = anc_finish_setup();
   if (e != cudaSuccess) return fail(anc_cuda_fail(e, "ctx workspace"));
   *out = c;
   return ANC_OK;
@@ -121,7 +122,10 @@ int anc_ctx_status(anc_ctx *ctx, uint32_t *code) {
   anc_device_guard g(ctx->device);
   ANC_CUDA(cudaStreamSynchronize(ctx->stream));
   ANC_CUDA(cudaMemcpy(code, ctx->d_status, sizeof(uint32_t), cudaMemcpyDeviceToHost));
-  if (*code) ANC_CUDA(cudaMemset(ctx->d_status, 0, sizeof(uint32_t)));
+  if (*code) {
+    ANC_CUDA(cudaMemset(ctx->d_status, 0, sizeof(uint32_t)));
+    ANC_CUDA(anc_finish_setup());        // the clear may not meet a later launch's bits
+  }
   return ANC_OK;
 }
 

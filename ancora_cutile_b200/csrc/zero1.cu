@@ -112,6 +112,7 @@ int anc_comm_create(anc_ctx *ctx, const void *id128, int rank, int world, anc_co
   }
   cudaError_t e = cudaMalloc((void **)&c->d_token, 256);
   if (e == cudaSuccess) e = cudaMemset(c->d_token, 0, 256);
+  if (e == cudaSuccess) e = anc_finish_setup();
   if (e != cudaSuccess) {
     g_nccl.CommDestroy(c->comm);
     delete c;

@@ -42,3 +42,17 @@ def test_clip_plan_is_ready_when_it_is_returned(ctx, busy, n):
     clip.free()
     d.free()
     assert ctx.status() == 0
+
+
+def test_a_new_context_does_not_clear_the_first_launchs_status(ctx, busy):
+    table, ids = anc.DBuf.zeros((4, 8), np.uint16, ctx), anc.DBuf(np.array([9, 1], np.int64), ctx)
+    out = anc.DBuf.zeros((2, 8), np.uint16, ctx)
+    busy()
+    other = anc.Context(ctx.device)
+    anc.kernels.embedding_lookup(table, ids, out, 2, 4, 8, ctx=other)                  # id 9 of a table of 4 rows
+    L.check(L.lib().anc_ctx_sync(ctx.handle, LEGACY))
+    assert other.status() == 0x8
+    assert other.status() == 0
+    for x in (table, ids, out):
+        x.free()
+    other.destroy()
