@@ -133,11 +133,12 @@ embedding_lookup_kernel(LookupArgs a) {
   for (int r = 0; r < kRows; ++r) {
     const uint32_t t = t0 + r * t_step;
     uint8_t *row = a.out + (int64_t)c0 * kOB + (uint64_t)t * a.out_pitch;
+    const float scale = id[r] >= 0 && id[r] < a.V ? a.scale : 0.f;      // a negative one would make -0 of a zero row
 #pragma unroll
     for (int q = 0; q < kOcts; ++q) {
       float f[8];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) f[k] = __fmul_rn(elem(x[r][q], k), a.scale);
+      for (int k = 0; k < 8; ++k) f[k] = __fmul_rn(elem(x[r][q], k), scale);
       store_oct<kOutF32, kVec>(row + q * 8 * L * kOB, t < a.T ? cols - q * 8 * L : 0, L, f);
     }
   }
