@@ -93,6 +93,18 @@ def dev_ptr(obj):
     raise TypeError(f"cannot take a device pointer from {type(obj).__name__}")
 
 
+def view_span(obj):
+    """Bytes from the address of a strided view to the end of its last element, by its
+    ``__cuda_array_interface__``; None where that names no strides."""
+    cai = getattr(obj, "__cuda_array_interface__", None)
+    if cai is None or cai.get("strides") is None:
+        return None
+    if 0 in cai["shape"]:
+        return 0
+    last = sum((n - 1) * s for n, s in zip(cai["shape"], cai["strides"]) if s > 0)
+    return last + np.dtype(cai["typestr"]).itemsize
+
+
 class DBuf:
     def __init__(self, arr, ctx=None):
         arr = np.ascontiguousarray(arr)

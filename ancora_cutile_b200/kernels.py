@@ -6,7 +6,7 @@ import ctypes as C
 import numpy as np
 
 from . import _lib as L
-from .buffers import dev_ptr, get_context
+from .buffers import dev_ptr, get_context, view_span
 
 _GRAD = {"bf16": L.GRAD_BF16, "f32": L.GRAD_F32}
 
@@ -74,12 +74,17 @@ _SIZE = {"bf16": 2, "f32": 4, "i32": 4, "i64": 8}
 
 
 def _buf(obj, rows, ld, D, dtype, what):
-    """Address of ``obj``; a buffer that knows its size must hold the rows it is said to."""
+    """Address of ``obj``; a buffer that knows its size must hold the rows it is said to, a strided view span them."""
     if type(obj) is int:
         return obj
     n = getattr(obj, "nbytes", None)
-    if n is not None and rows > 0 and n < ((rows - 1) * (ld or D) + D) * _SIZE[dtype]:
-        raise ValueError(f"{what} holds {n} bytes: too few for {rows} rows of {D} {dtype}")
+    if n is not None and rows > 0:
+        need = ((rows - 1) * (ld or D) + D) * _SIZE[dtype]
+        if n < need:
+            span = view_span(obj)
+            n = n if span is None else span
+        if n < need:
+            raise ValueError(f"{what} holds {n} bytes: too few for {rows} rows of {D} {dtype}, {ld or D} elements apart")
     return dev_ptr(obj)
 
 
