@@ -309,8 +309,9 @@ class ResidentHybrid:
         else:
             raise ValueError(f"into must be 'grad' or 'acc', got {into!r}")
         need = kernels.embedding_grad_workspace(T, V, D)
-        if not self._embed_work or self._embed_work[-1].nbytes < need:
-            self._embed_work.append(DBuf.empty((need,), np.uint8, self.ctx))   # a captured graph may hold the old one
+        have = self._embed_work[-1].nbytes if self._embed_work else 0
+        if have < need:                        # the old ones stay: a captured graph may hold them
+            self._embed_work.append(DBuf.empty((max(need, 2 * have),), np.uint8, self.ctx))
         kernels.embedding_grad(dy, ids, dw, T, V, D, self._embed_work[-1], scale=scale, dy_dtype=dy_dtype,
                                dw_dtype=dt, ids_dtype=ids_dtype, mode=mode, padding_idx=padding_idx,
                                stream=si, ctx=self.ctx)
