@@ -128,6 +128,7 @@ SIGNATURES = {
     "anc_embedding_grad_workspace": (_i, [_i64, _i64, _i64, C.POINTER(_u64)]),
     "anc_embedding_grad": (_i, [_vp, _vp, _i, _i64, _vp, _i, _vp, _i, _i64, _i64, _i64, _i64, _f, _i, _i64, _vp,
                                 _u64, _vp]),
+    "anc_embedding_wait_selftest": (_i, [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _vp, _u64, C.c_uint32, _vp]),
     "anc_nccl_load": (_i, [C.c_char_p]),
     "anc_nccl_unique_id": (_i, [_vp]),
     "anc_comm_create": (_i, [_vp, _vp, _i, _i, _pp]),

@@ -512,6 +512,7 @@ struct RedArgs {
   int per_part;                  // sorted places per group of L lanes
   float scale;
   uint32_t *flags;               // [piece][slice]: the partial sum of the run open at the piece's end is there
+  uint32_t raised, polls;        // what a raised flag holds (the self-test of the wait: 0), reads of a flag at most
   uint32_t *status;
 };
 
@@ -809,7 +810,7 @@ embedding_reduce_kernel(RedArgs a) {
     __syncwarp(L == 32 ? 0xFFFFFFFFu : ((1u << L) - 1u) << (threadIdx.x & 31 & ~(L - 1)));
     if (l == 0) {
       __threadfence();
-      asm volatile("st.release.gpu.global.u32 [%0], %1;" ::"l"(a.flags + (int64_t)piece * a.slices + slice), "r"(1u)
+      asm volatile("st.release.gpu.global.u32 [%0], %1;" ::"l"(a.flags + (int64_t)piece * a.slices + slice), "r"(a.raised)
                    : "memory");
     }
   };
@@ -855,7 +856,7 @@ embedding_reduce_kernel(RedArgs a) {
   bool ok = true;
   for (uint32_t q = first + threadIdx.x; q < piece; q += kRedThreads) {
     uint32_t seen = 0;
-    for (uint32_t i = 0; i < kWaitPolls && !seen; ++i)
+    for (uint32_t i = 0; i < a.polls && !seen; ++i)
       asm volatile("ld.acquire.gpu.global.u32 %0, [%1];"
                    : "=r"(seen)
                    : "l"(a.flags + (int64_t)q * a.slices + slice)
@@ -1094,85 +1095,9 @@ bool rows_are_vectors(const void *p, int64_t ld, int f32, int64_t D) {
   return (uintptr_t)p % align == 0 && D % 8 == 0 && ld % 8 == 0;
 }
 
-}  // namespace
-
-extern "C" {
-
-int anc_embedding_lookup(anc_ctx *ctx, const void *table, int table_dtype, int64_t table_ld, const void *ids,
-                         int ids_dtype, void *out, int out_dtype, int64_t out_ld, int64_t T, int64_t V, int64_t D,
-                         float scale, void *stream) {
-  ANC_REQUIRE(ctx, "ctx is NULL");
-  int rc = check_sizes(T, V, D);
-  if (!rc) rc = check_dtype(table_dtype, "table_dtype");
-  if (!rc) rc = check_dtype(out_dtype, "out_dtype");
-  if (rc) return rc;
-  ANC_REQUIRE(ids_dtype == ANC_IDS_I32 || ids_dtype == ANC_IDS_I64, "bad ids_dtype %d", ids_dtype);
-  ANC_REQUIRE(isfinite(scale), "scale must be finite");
-  if (T == 0) return ANC_OK;
-  ANC_REQUIRE(table && ids && out, "NULL argument");
-  if (table_ld == 0) table_ld = D;
-  if (out_ld == 0) out_ld = D;
-  ANC_REQUIRE(table_ld >= D && out_ld >= D && table_ld <= kMaxLd && out_ld <= kMaxLd,
-              "row strides must be at least the row length and at most 2^29");
-  const int tf = table_dtype == ANC_GRAD_F32, of = out_dtype == ANC_GRAD_F32, i64 = ids_dtype == ANC_IDS_I64;
-  ANC_REQUIRE(((uintptr_t)table & (tf ? 3 : 1)) == 0 && ((uintptr_t)out & (of ? 3 : 1)) == 0 &&
-                  ((uintptr_t)ids & (i64 ? 7 : 3)) == 0,
-              "pointer not aligned to its element size");
-  ANC_REQUIRE(!overlap(table, V, table_ld, tf ? 4 : 2, D, out, row_span(T, out_ld, of ? 4 : 2, D)) &&
-                  !overlap(out, T, out_ld, of ? 4 : 2, D, ids, T * (i64 ? 8 : 4)),
-              "the output overlaps an input");
-  anc_device_guard guard(ctx->device);
-  cudaStream_t st = anc_pick_stream(ctx, stream);
-  const bool vec = rows_are_vectors(table, table_ld, tf, D) && rows_are_vectors(out, out_ld, of, D);
-  LookupArgs a = {};
-  a.table = (const uint8_t *)table; a.ids = ids; a.out = (uint8_t *)out;
-  a.table_pitch = (uint32_t)(table_ld * (tf ? 4 : 2)); a.out_pitch = (uint32_t)(out_ld * (of ? 4 : 2));
-  a.T = (uint32_t)T; a.V = (uint32_t)V; a.ids64 = i64; a.D = (int)D; a.scale = scale; a.status = ctx->d_status;
-  a.L = 1;
-  while (a.L < 32 && a.L * 8 < D) a.L *= 2;
-  const int64_t per_lane = (D + 8 * a.L - 1) / (8 * a.L);        // octets of a row
-  const int64_t slices = (per_lane + 3) / 4;
-  const int octs = (int)((per_lane + slices - 1) / slices);
-  ANC_REQUIRE(slices <= 65535, "row length %lld out of range", (long long)D);
-  const int64_t rows = (int64_t)(32 / a.L) * (4 / octs);         // per unit
-  a.units = (uint32_t)((T + rows - 1) / rows);
-  const dim3 blocks((unsigned)((a.units + kLookupThreads / 32 - 1) / (kLookupThreads / 32)), (unsigned)slices);
-#define ANC_LOOKUP(F, O, VEC, OCTS) \
-  embedding_lookup_kernel<F, O, VEC, OCTS><<<blocks, kLookupThreads, 0, st>>>(a)
-#define ANC_LOOKUP_O(F, O, VEC)                         \
-  do {                                                  \
-    if (octs == 4) ANC_LOOKUP(F, O, VEC, 4);            \
-    else if (octs == 3) ANC_LOOKUP(F, O, VEC, 3);       \
-    else if (octs == 2) ANC_LOOKUP(F, O, VEC, 2);       \
-    else ANC_LOOKUP(F, O, VEC, 1);                      \
-  } while (0)
-#define ANC_LOOKUP_V(F, O)                              \
-  do {                                                  \
-    if (vec) ANC_LOOKUP_O(F, O, true);                  \
-    else ANC_LOOKUP_O(F, O, false);                     \
-  } while (0)
-  if (tf && of) ANC_LOOKUP_V(true, true);
-  else if (tf) ANC_LOOKUP_V(true, false);
-  else if (of) ANC_LOOKUP_V(false, true);
-  else ANC_LOOKUP_V(false, false);
-#undef ANC_LOOKUP_V
-#undef ANC_LOOKUP_O
-#undef ANC_LOOKUP
-  ANC_CUDA(cudaGetLastError());
-  return ANC_OK;
-}
-
-int anc_embedding_grad_workspace(int64_t T, int64_t V, int64_t D, uint64_t *bytes) {
-  ANC_REQUIRE(bytes, "bytes is NULL");
-  int rc = check_sizes(T, V, D);
-  if (rc) return rc;
-  *bytes = workspace_of(T, D).total;
-  return ANC_OK;
-}
-
-int anc_embedding_grad(anc_ctx *ctx, const void *dy, int dy_dtype, int64_t dy_ld, const void *ids, int ids_dtype,
+int grad_impl(anc_ctx *ctx, const void *dy, int dy_dtype, int64_t dy_ld, const void *ids, int ids_dtype,
                        void *dw, int dw_dtype, int64_t dw_ld, int64_t T, int64_t V, int64_t D, float scale, int mode,
-                       int64_t padding_idx, void *work, uint64_t work_bytes, void *stream) {
+                       int64_t padding_idx, void *work, uint64_t work_bytes, void *stream, uint32_t raised, uint32_t polls) {
   ANC_REQUIRE(ctx && dw, "NULL argument");
   int rc = check_sizes(T, V, D);
   if (!rc) rc = check_dtype(dy_dtype, "dy_dtype");
@@ -1240,6 +1165,7 @@ int anc_embedding_grad(anc_ctx *ctx, const void *dy, int dy_dtype, int64_t dy_ld
   ra.partial = (float *)(wp + ws.partial);
   ra.V = (uint32_t)V; ra.D = (int)D; ra.slices = sh.slices; ra.L = sh.L; ra.per_part = sh.per_part; ra.scale = scale;
   ra.status = ctx->d_status;
+  ra.raised = raised; ra.polls = polls;
   const int64_t blocks =
       small ? (T * sh.slices + kRedThreads / sh.L - 1) / (kRedThreads / sh.L) : sh.pieces * sh.slices;
   ANC_REQUIRE(blocks <= 0x7FFFFFFF, "T x D too large");
@@ -1334,6 +1260,96 @@ int anc_embedding_grad(anc_ctx *ctx, const void *dy, int dy_dtype, int64_t dy_ld
 #undef ANC_REDUCE_W
   ANC_CUDA(cudaGetLastError());
   return ANC_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int anc_embedding_lookup(anc_ctx *ctx, const void *table, int table_dtype, int64_t table_ld, const void *ids,
+                         int ids_dtype, void *out, int out_dtype, int64_t out_ld, int64_t T, int64_t V, int64_t D,
+                         float scale, void *stream) {
+  ANC_REQUIRE(ctx, "ctx is NULL");
+  int rc = check_sizes(T, V, D);
+  if (!rc) rc = check_dtype(table_dtype, "table_dtype");
+  if (!rc) rc = check_dtype(out_dtype, "out_dtype");
+  if (rc) return rc;
+  ANC_REQUIRE(ids_dtype == ANC_IDS_I32 || ids_dtype == ANC_IDS_I64, "bad ids_dtype %d", ids_dtype);
+  ANC_REQUIRE(isfinite(scale), "scale must be finite");
+  if (T == 0) return ANC_OK;
+  ANC_REQUIRE(table && ids && out, "NULL argument");
+  if (table_ld == 0) table_ld = D;
+  if (out_ld == 0) out_ld = D;
+  ANC_REQUIRE(table_ld >= D && out_ld >= D && table_ld <= kMaxLd && out_ld <= kMaxLd,
+              "row strides must be at least the row length and at most 2^29");
+  const int tf = table_dtype == ANC_GRAD_F32, of = out_dtype == ANC_GRAD_F32, i64 = ids_dtype == ANC_IDS_I64;
+  ANC_REQUIRE(((uintptr_t)table & (tf ? 3 : 1)) == 0 && ((uintptr_t)out & (of ? 3 : 1)) == 0 &&
+                  ((uintptr_t)ids & (i64 ? 7 : 3)) == 0,
+              "pointer not aligned to its element size");
+  ANC_REQUIRE(!overlap(table, V, table_ld, tf ? 4 : 2, D, out, row_span(T, out_ld, of ? 4 : 2, D)) &&
+                  !overlap(out, T, out_ld, of ? 4 : 2, D, ids, T * (i64 ? 8 : 4)),
+              "the output overlaps an input");
+  anc_device_guard guard(ctx->device);
+  cudaStream_t st = anc_pick_stream(ctx, stream);
+  const bool vec = rows_are_vectors(table, table_ld, tf, D) && rows_are_vectors(out, out_ld, of, D);
+  LookupArgs a = {};
+  a.table = (const uint8_t *)table; a.ids = ids; a.out = (uint8_t *)out;
+  a.table_pitch = (uint32_t)(table_ld * (tf ? 4 : 2)); a.out_pitch = (uint32_t)(out_ld * (of ? 4 : 2));
+  a.T = (uint32_t)T; a.V = (uint32_t)V; a.ids64 = i64; a.D = (int)D; a.scale = scale; a.status = ctx->d_status;
+  a.L = 1;
+  while (a.L < 32 && a.L * 8 < D) a.L *= 2;
+  const int64_t per_lane = (D + 8 * a.L - 1) / (8 * a.L);        // octets of a row
+  const int64_t slices = (per_lane + 3) / 4;
+  const int octs = (int)((per_lane + slices - 1) / slices);
+  ANC_REQUIRE(slices <= 65535, "row length %lld out of range", (long long)D);
+  const int64_t rows = (int64_t)(32 / a.L) * (4 / octs);         // per unit
+  a.units = (uint32_t)((T + rows - 1) / rows);
+  const dim3 blocks((unsigned)((a.units + kLookupThreads / 32 - 1) / (kLookupThreads / 32)), (unsigned)slices);
+#define ANC_LOOKUP(F, O, VEC, OCTS) \
+  embedding_lookup_kernel<F, O, VEC, OCTS><<<blocks, kLookupThreads, 0, st>>>(a)
+#define ANC_LOOKUP_O(F, O, VEC)                         \
+  do {                                                  \
+    if (octs == 4) ANC_LOOKUP(F, O, VEC, 4);            \
+    else if (octs == 3) ANC_LOOKUP(F, O, VEC, 3);       \
+    else if (octs == 2) ANC_LOOKUP(F, O, VEC, 2);       \
+    else ANC_LOOKUP(F, O, VEC, 1);                      \
+  } while (0)
+#define ANC_LOOKUP_V(F, O)                              \
+  do {                                                  \
+    if (vec) ANC_LOOKUP_O(F, O, true);                  \
+    else ANC_LOOKUP_O(F, O, false);                     \
+  } while (0)
+  if (tf && of) ANC_LOOKUP_V(true, true);
+  else if (tf) ANC_LOOKUP_V(true, false);
+  else if (of) ANC_LOOKUP_V(false, true);
+  else ANC_LOOKUP_V(false, false);
+#undef ANC_LOOKUP_V
+#undef ANC_LOOKUP_O
+#undef ANC_LOOKUP
+  ANC_CUDA(cudaGetLastError());
+  return ANC_OK;
+}
+
+int anc_embedding_grad_workspace(int64_t T, int64_t V, int64_t D, uint64_t *bytes) {
+  ANC_REQUIRE(bytes, "bytes is NULL");
+  int rc = check_sizes(T, V, D);
+  if (rc) return rc;
+  *bytes = workspace_of(T, D).total;
+  return ANC_OK;
+}
+
+int anc_embedding_grad(anc_ctx *ctx, const void *dy, int dy_dtype, int64_t dy_ld, const void *ids, int ids_dtype,
+                       void *dw, int dw_dtype, int64_t dw_ld, int64_t T, int64_t V, int64_t D, float scale, int mode,
+                       int64_t padding_idx, void *work, uint64_t work_bytes, void *stream) {
+  return grad_impl(ctx, dy, dy_dtype, dy_ld, ids, ids_dtype, dw, dw_dtype, dw_ld, T, V, D, scale, mode, padding_idx, work,
+                   work_bytes, stream, 1u, kWaitPolls);
+}
+
+int anc_embedding_wait_selftest(anc_ctx *ctx, const float *dy, const int64_t *ids, float *dw, int64_t T, int64_t V,
+                                int64_t D, void *work, uint64_t work_bytes, uint32_t polls, void *stream) {
+  ANC_REQUIRE(polls > 0 && polls <= (1u << 14), "polls %u outside 1..2^14", polls);
+  return grad_impl(ctx, dy, ANC_GRAD_F32, 0, ids, ANC_IDS_I64, dw, ANC_GRAD_F32, 0, T, V, D, 1.f, ANC_EMBED_ADD, -1, work,
+                   work_bytes, stream, 0u, polls);
 }
 
 }  // extern "C"

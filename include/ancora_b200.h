@@ -411,7 +411,8 @@ ANC_API int anc_embedding_lookup(anc_ctx *ctx, const void *table, int table_dtyp
 #define ANC_EMBED_ADD 1   /* dw[v,:] = round(dw[v,:] + scale * S_v) for the rows named, others untouched */
 /* S_v = sum of dy[t,:] over the tokens t with ids[t] == v and v != padding_idx (< 0: none), in an order that
  * the ids, the sizes and the alignment fix: the same bits every time.  dw and work may overlap none of the others.
- * Blocks that finish a row wait, with a limit (status bit 0x10), for the blocks that hold its other tokens.
+ * Blocks that finish a row wait, with a limit, for the blocks that hold its other tokens; should it run out, status bit
+ * 0x10 is set and such rows miss their sums, whole rows or stretches of columns.
  * `work`: caller-owned scratch of at least anc_embedding_grad_workspace(T, V, D) bytes, 16-byte aligned, contents
  * unspecified; calls that may overlap on the GPU need one each. */
 ANC_API int anc_embedding_grad_workspace(int64_t T, int64_t V, int64_t D, uint64_t *bytes);
@@ -419,6 +420,11 @@ ANC_API int anc_embedding_grad(anc_ctx *ctx, const void *dy, int dy_dtype, int64
                                int ids_dtype, void *dw, int dw_dtype, int64_t dw_ld, int64_t T, int64_t V, int64_t D,
                                float scale, int mode, int64_t padding_idx, void *work, uint64_t work_bytes,
                                void *stream);
+/* Self-test of that wait: ANC_EMBED_ADD of float32 rows by int64 ids, scale 1, but the blocks that finish a row wait for
+ * flags nobody raises and give up after `polls` reads (1..2^14).  Rows whose tokens lie within one block's piece of the
+ * sorted list are added, the others are as they were, status bit 0x10 is set, the workspace is ready for its next call. */
+ANC_API int anc_embedding_wait_selftest(anc_ctx *ctx, const float *dy, const int64_t *ids, float *dw, int64_t T, int64_t V,
+                                        int64_t D, void *work, uint64_t work_bytes, uint32_t polls, void *stream);
 
 /* ----------------------------------------------------------------- ZeRO-1 ---- */
 /* No counterpart in the reference (single GPU, ancora README.md:93).  NCCL is
