@@ -196,7 +196,7 @@ __device__ __forceinline__ void reduce_blocks(double acc, double *partial, uint3
   }
 }
 
-// Bound by the read of the gradients: 1.19 GB of bf16 in 172 us a call, 6.9 TB/s.  Resident blocks go through the arena in
+// Bound by the read of the gradients: 1.19 GB of bf16 in 176 us a call, 6.8 TB/s.  Resident blocks go through the arena in
 // pieces, in address order as far as they keep step, which DRAM likes better than one long share per block
 // (150 M bf16: 50.8 us against 52.5, 596 M: 172 against 181; pieces half or twice as long: 186 and 173).
 template <bool kF32>

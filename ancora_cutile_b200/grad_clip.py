@@ -26,7 +26,7 @@ def _buf(obj, numel, dtype, what):
 
 class GradClip:
     """tensors: list of dicts {g, numel[, out]}: device buffers (anything ``dev_ptr`` accepts) of ``grad_dtype``,
-    with ``out`` of ``out_dtype`` (default: the same type) or absent to clip in place.  ``result``: a caller's
+    with ``out`` of ``out_dtype`` (default: the same type), or absent or ``g`` itself to clip in place.  ``result``: a caller's
     device buffer of two float32 {norm, factor}; by default the plan holds them.
 
       norm   = scale * sqrt(sum of squares over all tensors)
