@@ -280,8 +280,8 @@ class ResidentHybrid:
         gradient arena for the table: in every micro-batch the head's gradient of a tied table, for any other
         table nothing.  So that an earlier gradient is never added again, every step clears the table's region of
         the gradient arena when it has read it.  Where an earlier gradient may lie there all the same (steps were
-        taken before the first such call for the table, or a finished gradient was not stepped on) only the caller
-        knows: ``tied=True``: the head writes the region in every micro-batch, the engine never clears it;
+        taken before the first such call for the table, or a finished gradient was not stepped on, and no
+        ``upload_grads`` of everything came since) only the caller knows: ``tied=True``: the head writes the region in every micro-batch, the engine never clears it;
         ``tied=False``: nothing else writes it, the engine clears it now.  It holds for later calls too; with
         None, as long as neither was ever said, such a call is refused."""
         V, D = self._table(name)
@@ -326,6 +326,11 @@ class ResidentHybrid:
             if not self._acc_tied[n]:
                 self.grad_view(n).zero_(si)
             self._acc_stale.discard(n)
+
+    def _grads_fresh(self):
+        """All gradients were written: whatever lies in the arenas is the caller's for the next fold or step."""
+        self._grads_spent = False
+        self._acc_stale = set()
 
     def _grads_stepped(self, si, arena=None):
         """Behind a step (of ``arena`` "adamw" or "muon", None: both): the gradients it read are spent."""
@@ -426,6 +431,7 @@ class ResidentHybrid:
         it = self._gdt.itemsize
         L.check(L.lib().anc_h2d(self.ctx.handle, self.a_g.ptr, pa.ptr, self.a_padded * it, si or None, 0))
         L.check(L.lib().anc_h2d(self.ctx.handle, self.m_g.ptr, pm.ptr, self.m_total * it, si or None, 0))
+        self._grads_fresh()
 
     def reduce_scatter_grads(self, si=None):
         """Data-parallel gradient reduction feeding the ZeRO-1 owners: every rank holds local
@@ -602,6 +608,8 @@ class ResidentHybrid:
         ("adamw" or "muon") restricts it to one sub-optimizer's tensors."""
         names = None if kind is None else (self.adamw_names if kind == "adamw" else self.muon_names)
         self._stage_grads(grads, names)
+        if kind is None and self.world == 1:
+            self._grads_fresh()
         return sum(self._h2d_unit(u, si) for u in self.units if kind is None or u[0] == kind)
 
     def _ensure_host_side(self):

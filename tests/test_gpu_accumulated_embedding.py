@@ -183,3 +183,17 @@ def test_tied_belongs_to_the_accumulator(win):
         win.eng.embedding_grad("embed", dy, ids, 4, tied=True)
     win.eng.embedding_grad("embed", dy, ids, 4)                    # "write": the region is a fresh gradient
     assert not win.eng.grad_view("embed").to_numpy().any()
+
+
+@pytest.mark.parametrize("full", [False, True])
+def test_an_upload_of_all_gradients_leaves_nothing_to_say(win, full):
+    """The table's region then holds what the caller put there, whatever came before."""
+    eng, st = win.eng, win.ctx.stream
+    win.write(SHP)
+    eng.step(st)
+    for k in range(2):                                             # after a step; after a window that was not stepped on
+        up = {n: win.grad(s) for n, s in SHP.items()}
+        (eng.upload_full_grads if full else eng.upload_grads)({n: obf.rne_bits(g) for n, g in up.items()}, st)
+        up["embed"] = up["embed"] + win.embed()
+        eng.finalize_grads(st, rounding="rne")
+        win.check(up, 1)
