@@ -1095,9 +1095,10 @@ bool rows_are_vectors(const void *p, int64_t ld, int f32, int64_t D) {
   return (uintptr_t)p % align == 0 && D % 8 == 0 && ld % 8 == 0;
 }
 
-int grad_impl(anc_ctx *ctx, const void *dy, int dy_dtype, int64_t dy_ld, const void *ids, int ids_dtype,
-                       void *dw, int dw_dtype, int64_t dw_ld, int64_t T, int64_t V, int64_t D, float scale, int mode,
-                       int64_t padding_idx, void *work, uint64_t work_bytes, void *stream, uint32_t raised, uint32_t polls) {
+// anc_embedding_grad; raised, polls: of the wait between blocks (RedArgs)
+int grad_impl(anc_ctx *ctx, const void *dy, int dy_dtype, int64_t dy_ld, const void *ids, int ids_dtype, void *dw,
+              int dw_dtype, int64_t dw_ld, int64_t T, int64_t V, int64_t D, float scale, int mode, int64_t padding_idx,
+              void *work, uint64_t work_bytes, void *stream, uint32_t raised, uint32_t polls) {
   ANC_REQUIRE(ctx && dw, "NULL argument");
   int rc = check_sizes(T, V, D);
   if (!rc) rc = check_dtype(dy_dtype, "dy_dtype");

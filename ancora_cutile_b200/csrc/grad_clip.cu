@@ -375,7 +375,7 @@ __device__ __forceinline__ bool all_arrived(uint32_t *ticket, uint32_t polls) {
 
 // Norm and scaling in one launch: a block per chunk, all resident at once (a cooperative launch), the
 // chunk in registers while the blocks wait for one another's sums: 2.5 M elements of bf16 8.2 us against 14.3 by two
-// launches.  From about 5 M bf16 elements on the chunks are too many and there are two launches.  The wait is
+// launches.  From 3.6 M elements on the chunks are too many and there are two launches.  The wait is
 // bounded, and the blocks decide together: when it runs out, status bit 0x10 is set, norm and factor are NaN and no
 // gradient is written.  kLate, for the self-test: block `late` comes only after another one gave up.  Three blocks an
 // SM: left to itself the compiler takes registers that leave room for two.
